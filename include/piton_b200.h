@@ -76,9 +76,10 @@ PITON_B200_API int piton_b200_memset(uint64_t dst, int value, size_t bytes, void
    after `timeout_s` seconds instead of blocking for ever
    (the counterpart of piton_rt.c:150-189's 20 s launch timeout). */
 PITON_B200_API int piton_b200_stream_wait(void *stream, double timeout_s);
-/* Device-side status of the current device's tensor-core kernels, then reset to 0:
-   0 = ok, else the bounded wait that ran out (1 producer, 2 MMA, 3 epilogue, 4 drain).
-   Those kernels never trap or spin for ever: they record this, drain and return. */
+/* Device-side status of the current device's tensor-core and paged-cache kernels, then reset to 0:
+   0 = ok, else the bounded wait that ran out (1 producer, 2 MMA, 3 epilogue, 4 drain) or what a
+   paged-cache kernel found out of range and did not follow (16 a page-table entry, 17 a position
+   or offset).  Those kernels never trap or spin for ever: they record this, drain and return. */
 PITON_B200_API int piton_b200_device_status(int *status);
 
 /* ---- vector add: examples/kernels.py:6-15 add_kernel ---- */
@@ -351,6 +352,81 @@ PITON_B200_API int piton_b200_tinygpt_generate(const piton_tinygpt_args *args, v
 /* Instantiated graphs cached on the current device; piton_b200_graph_cache_clear() destroys them. */
 PITON_B200_API int piton_b200_graph_cache_entries(int *entries);
 PITON_B200_API int piton_b200_graph_cache_clear(void);
+
+/* ---- serving operators: a paged 8-bit key / value cache and 4-bit weights (no counterpart in the
+   reference; they stand beside its attention, examples/attention.py:75-113, and dense layers,
+   examples/nn_kernels.py:23-74) ----
+   The cache: codes uint8 (e4m3) [num_pages, kv_heads, page_size, head_dim], contiguous and 16-byte
+   aligned, for the keys and for the values, and scales float [num_pages, kv_heads] for each; element =
+   code * scale of its page and head, scales are powers of two in [2^-120, 2^120].  page_size 16, 32, 64
+   or 128; head_dim 32, 64 or 128 (ENOTSUP otherwise).  Token p of sequence b is in page
+   table[b * table_stride + p / page_size], slot p % page_size.  A table entry outside [0, num_pages) or a
+   position past the table is not followed: those tokens are neither written nor attended, and
+   piton_b200_device_status reports it. */
+#define PITON_B200_TYPE_F32 0  /* element types of activations */
+#define PITON_B200_TYPE_F16 1
+#define PITON_B200_TYPE_BF16 2
+
+/* Appends the new tokens' keys and values, the keys rotated by position on the way, and rotates the
+   queries.  Sequence b's new tokens are [cu[b], cu[b + 1]) of k, v and q (tokens / batch each when cu is
+   0) and take positions starts[b], starts[b] + 1, ...  Rotation by the rows of cos and sin (float
+   [rope_len, rot_dim / 2], row = position; rot_dim 0: none): (x1, x2) becomes (x1 c - x2 s, x2 c + x1 s)
+   for the pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) with `interleaved`; elements from rot_dim on stay.
+   A block (page, head) takes the least scale that holds its new values and is at least its old one while
+   the page holds older tokens; those are requantised when it grows.  A non-finite value is stored as NaN
+   and leaves the scale alone.  A page that is written belongs to one sequence.  lengths[b] (optional, not
+   `starts`) = starts[b] + new tokens of b. */
+typedef struct {
+    uint64_t k, v;              /* [tokens, kv_heads, head_dim] of `type`, unit stride along head_dim */
+    uint64_t q, q_out;          /* [tokens, q_heads, head_dim], or both 0 */
+    uint64_t k_codes, v_codes, k_scale, v_scale;
+    uint64_t table, starts, cu, lengths; /* int32_t: [batch, table_width], [batch], [batch + 1] or 0, [batch] or 0 */
+    uint64_t cos_table, sin_table;
+    int64_t batch, tokens, kv_heads, q_heads, head_dim, page_size, num_pages, table_width, table_stride;
+    int64_t stride_kt, stride_kh, stride_vt, stride_vh, stride_qt, stride_qh, stride_ot, stride_oh;
+    int64_t rot_dim, rope_len;
+    int32_t type, interleaved;
+    uint32_t flags;             /* 0 */
+    uint32_t _pad;
+} piton_kv_append_args;
+PITON_B200_API int piton_b200_kv_append(const piton_kv_append_args *args, void *stream);
+
+/* Attention over the cache.  Sequence b holds lengths[b] tokens, the last of them its query tokens
+   [cu[b], cu[b + 1]) (tokens / batch each when cu is 0): query i of n is at position p = lengths[b] - n + i
+   and attends keys p - window < j <= p (window 0: all up to p).  Query head h uses key head
+   h / (q_heads / kv_heads).  out = softmax(sm_scale q k) v, rows without keys 0; lse (optional): the natural
+   logarithm of the row's sum of exponentials, -inf for rows without keys.  max_length and max_new are
+   bounds of the lengths and of the query tokens a sequence, used to size the launch (0: the table's width
+   and `tokens`); a longer sequence is still attended in full, more query tokens than max_new are not
+   computed. */
+typedef struct {
+    uint64_t q, out;            /* [tokens, q_heads, head_dim] of `type`, unit stride along head_dim */
+    uint64_t lse;               /* float [tokens, q_heads] or 0 */
+    uint64_t k_codes, v_codes, k_scale, v_scale;
+    uint64_t table, lengths, cu; /* int32_t */
+    double sm_scale;
+    int64_t batch, tokens, q_heads, kv_heads, head_dim, page_size, num_pages, table_width, table_stride;
+    int64_t stride_qt, stride_qh, stride_ot, stride_oh;
+    int64_t window, max_length, max_new;
+    uint64_t workspace;         /* device scratch of piton_b200_kv_attention_workspace_size() bytes, 16-byte aligned */
+    uint64_t workspace_bytes;
+    int32_t type;
+    uint32_t flags;             /* 0 */
+} piton_kv_attention_args;
+PITON_B200_API size_t piton_b200_kv_attention_workspace_size(const piton_kv_attention_args *args);
+PITON_B200_API int piton_b200_kv_attention(const piton_kv_attention_args *args, void *stream);
+
+/* y[rows, outer] = x[rows, inner] W^T (+ bias), W[n, k] = scales[n, k / group] * (code[n, k] - zero[n, k / group]).
+   Codes are 4 bits, two per byte along k (even k in the low half), rows stride_codes bytes apart; group 32,
+   64 or 128; zeros uint8 (any value), or 0 for zero point 8.  x, bias and y are of `type`, scales of `scale_type`. */
+typedef struct {
+    uint64_t x, codes, scales, zeros, bias, y;
+    int64_t rows, inner, outer;
+    int64_t stride_x, stride_codes, stride_scales, stride_zeros, stride_y;
+    int32_t group, type, scale_type;
+    uint32_t flags;             /* 0 */
+} piton_matvec_w4_args;
+PITON_B200_API int piton_b200_matvec_w4(const piton_matvec_w4_args *args, void *stream);
 
 #ifdef __cplusplus
 }

@@ -41,6 +41,7 @@
 
 #include "attention.cuh"
 #include "common.cuh"
+#include "decode.cuh"
 #include "gemm_tc.cuh"
 #include "sm100.cuh"
 
@@ -1185,9 +1186,11 @@ int tc_status_read_and_clear(int *status) {
 
 extern "C" int piton_b200_device_status(int *status) {
     PITON_REQUIRE(status != nullptr, "status is NULL");
-    int gemm = 0, attn = 0, rc;
+    int gemm = 0, attn = 0, append = 0, cached = 0, rc;
     if ((rc = piton::tc_status_read_and_clear(&gemm)) != PITON_B200_OK) return rc;
     if ((rc = piton::attention_tc_status_read_and_clear(&attn)) != PITON_B200_OK) return rc;
-    *status = gemm ? gemm : attn;
+    if ((rc = piton::decode::kv_append_status_read_and_clear(&append)) != PITON_B200_OK) return rc;
+    if ((rc = piton::decode::kv_attention_status_read_and_clear(&cached)) != PITON_B200_OK) return rc;
+    *status = gemm ? gemm : attn ? attn : append ? append : cached;
     return PITON_B200_OK;
 }

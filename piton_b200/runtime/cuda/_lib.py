@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get("PITON_B200_LIB", os.path.join(PKG, "libpiton_b200.so"
 
 OK, EINVAL, ECUDA, ETIMEOUT, ENOTSUP, ENOMEM, EWORKSPACE = 0, -1, -2, -3, -4, -5, -6
 QPU_ROUNDING, FORCE_SIMT, CUDA_GRAPH = 0x1, 0x2, 0x4
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 32 << 20   # PITON_B200_NOALLOC_SCRATCH_BYTES
 
 u64, i64, i32, u32, f64 = C.c_uint64, C.c_int64, C.c_int32, C.c_uint32, C.c_double
@@ -101,6 +102,33 @@ class TinyGPTArgs(C.Structure):
                 ("n_head", i32), ("ctx", i32), ("flags", u32)]
 
 
+class KvAppendArgs(C.Structure):
+    _fields_ = [("k", u64), ("v", u64), ("q", u64), ("q_out", u64), ("k_codes", u64), ("v_codes", u64),
+                ("k_scale", u64), ("v_scale", u64), ("table", u64), ("starts", u64), ("cu", u64), ("lengths", u64),
+                ("cos_table", u64), ("sin_table", u64), ("batch", i64), ("tokens", i64), ("kv_heads", i64),
+                ("q_heads", i64), ("head_dim", i64), ("page_size", i64), ("num_pages", i64), ("table_width", i64),
+                ("table_stride", i64), ("stride_kt", i64), ("stride_kh", i64), ("stride_vt", i64),
+                ("stride_vh", i64), ("stride_qt", i64), ("stride_qh", i64), ("stride_ot", i64), ("stride_oh", i64),
+                ("rot_dim", i64), ("rope_len", i64), ("type", i32), ("interleaved", i32), ("flags", u32),
+                ("_pad", u32)]
+
+
+class KvAttentionArgs(C.Structure):
+    _fields_ = [("q", u64), ("out", u64), ("lse", u64), ("k_codes", u64), ("v_codes", u64), ("k_scale", u64),
+                ("v_scale", u64), ("table", u64), ("lengths", u64), ("cu", u64), ("sm_scale", f64), ("batch", i64),
+                ("tokens", i64), ("q_heads", i64), ("kv_heads", i64), ("head_dim", i64), ("page_size", i64),
+                ("num_pages", i64), ("table_width", i64), ("table_stride", i64), ("stride_qt", i64),
+                ("stride_qh", i64), ("stride_ot", i64), ("stride_oh", i64), ("window", i64), ("max_length", i64),
+                ("max_new", i64), ("workspace", u64), ("workspace_bytes", u64), ("type", i32), ("flags", u32)]
+
+
+class MatvecW4Args(C.Structure):
+    _fields_ = [("x", u64), ("codes", u64), ("scales", u64), ("zeros", u64), ("bias", u64), ("y", u64),
+                ("rows", i64), ("inner", i64), ("outer", i64), ("stride_x", i64), ("stride_codes", i64),
+                ("stride_scales", i64), ("stride_zeros", i64), ("stride_y", i64), ("group", i32), ("type", i32),
+                ("scale_type", i32), ("flags", u32)]
+
+
 # name -> (restype, argtypes); every function include/piton_b200.h declares
 PROTOTYPES = {
     "piton_b200_abi_version": (C.c_int, []),
@@ -146,13 +174,19 @@ PROTOTYPES = {
     "piton_b200_tinygpt_generate": (C.c_int, [C.POINTER(TinyGPTArgs), C.c_void_p]),
     "piton_b200_graph_cache_entries": (C.c_int, [C.POINTER(C.c_int)]),
     "piton_b200_graph_cache_clear": (C.c_int, []),
+    "piton_b200_kv_append": (C.c_int, [C.POINTER(KvAppendArgs), C.c_void_p]),
+    "piton_b200_kv_attention_workspace_size": (C.c_size_t, [C.POINTER(KvAttentionArgs)]),
+    "piton_b200_kv_attention": (C.c_int, [C.POINTER(KvAttentionArgs), C.c_void_p]),
+    "piton_b200_matvec_w4": (C.c_int, [C.POINTER(MatvecW4Args), C.c_void_p]),
 }
 
 STRUCTS = {"piton_allgather_args": AllgatherArgs, "piton_add_args": AddArgs, "piton_softmax_args": SoftmaxArgs, "piton_matmul_args": MatmulArgs,
            "piton_dense_args": DenseArgs, "piton_mlp_args": MlpArgs, "piton_attention_args": AttentionArgs,
            "piton_layernorm_args": LayernormArgs, "piton_tinygpt_args": TinyGPTArgs,
            "piton_elementwise_args": ElementwiseArgs, "piton_idiv_args": IdivArgs,
-           "piton_row_reduce_args": RowReduceArgs, "piton_transpose_args": TransposeArgs, "piton_life_args": LifeArgs}
+           "piton_row_reduce_args": RowReduceArgs, "piton_transpose_args": TransposeArgs, "piton_life_args": LifeArgs,
+           "piton_kv_append_args": KvAppendArgs, "piton_kv_attention_args": KvAttentionArgs,
+           "piton_matvec_w4_args": MatvecW4Args}
 
 _lib = None
 
