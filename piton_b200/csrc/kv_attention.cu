@@ -1,7 +1,21 @@
 // Attention of a few query tokens per sequence over the paged 8-bit cache (kv_append.cu's layout).
 //
-// A CTA takes one query row (token, head); its warps walk the keys in turn, each with its own
-// running maximum and sum of the softmax in fp32, and join at the end.
+// For every row (query token, head): s_j = scale q . k_j over the keys it sees, o = sum_j softmax(s)_j v_j,
+// in one pass over the keys with the running maximum and sum of the softmax.  Each key and value byte is
+// read once per 16 rows, and a row tile does 4 D flops per 2 D bytes, so the cache's bytes bound it.
+//
+// A CTA takes up to 16 rows that share a key head (row = token * group + head of the group) and a range of keys;
+// its four warps take 32 keys at a time in turn, each with its own softmax state, and never wait for one
+// another before the end.  With the scores computed as S^T = K Q^T and the output as O^T = V^T P^T, keys and
+// dimensions are the 16-row side of mma.m16n8k16 and the rows its 8-column side, so one query token's group of
+// heads fills an instruction.  Every e4m3 code is exact in fp16: queries are scaled by a power of two per row
+// and rounded to fp16 (fp32 ones split into two halves, 22 bits), so are the weights p (times 2^14), and the
+// products are exact in the fp32 accumulators, which hold 32 keys at most before they are added to O.
+//
+// The order of dimensions inside an MMA's k index is free as long as K and Q agree, so every lane copies
+// (cp.async) just the 16 bytes of a key row that its own fragment holds, and the same for V with dimension
+// blocks: shared memory is each lane's private queue, read back without bank conflicts and without any
+// barrier, and its depth (16 KB a warp) is what covers the memory latency.
 #include "decode.cuh"
 
 namespace piton {
@@ -11,7 +25,10 @@ __device__ int g_cached_status = 0;
 
 namespace {
 
-constexpr int THREADS = 128, WARPS = THREADS / 32;
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int KEYS = 32;                 // keys of a stage: two 16-key tiles, each inside one page
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr uint32_t BAD_PAGE = 0x7FC0DEADu;   // in a stage's scale slot: the tile's page was not followed
 
 struct CachedParams {
     const void *q;
@@ -20,71 +37,545 @@ struct CachedParams {
     const uint8_t *kc, *vc;
     const float *ks, *vs;
     const int32_t *table, *lengths, *cu;
-    int64_t batch, tokens, q_heads, kv_heads, page_size, num_pages, table_width, table_stride;
-    int64_t sqt, sqh, sot, soh;
-    int64_t window, uniform, max_new;
+    float *part_o;                       // [splits][tokens * q_heads][D], splits > 1 only
+    float2 *part_ml;                     // [splits][tokens * q_heads]
+    int64_t tokens, num_pages, table_stride, sqt, sqh, sot, soh, window, uniform, chunk;
+    int32_t q_heads, kv_heads, group, page_log2, table_width, row_tiles, splits;
     float scale;
 };
 
 __device__ __forceinline__ void record_status(int code) { atomicCAS(&g_cached_status, 0, code); }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) kv_attention_kernel(const CachedParams p) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t b = blockIdx.z, i = blockIdx.y, h = blockIdx.x, kvh = h / (p.q_heads / p.kv_heads);
+template <int D> struct Geometry {
+    static constexpr int KB = D >= 64 ? 16 : D / 4;     // bytes of a key row in one copy of a lane
+    static constexpr int KC = D / (4 * KB);             // such copies per row
+    static constexpr int VB = D / 8;                    // bytes of a value row that a lane takes
+    static constexpr int STAGES = 256 / D;              // 16 KB in flight a warp at every D
+    static constexpr int KBYTES = KEYS * D, STAGE_BYTES = 2 * KBYTES;
+    static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
+    static constexpr int SMEM = RING + WARPS * STAGES * 16;   // and four scales a stage: K, V of either tile
+};
+
+template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool on) {
+    const int size = on ? N : 0;                        // the rest of the N bytes is filled with zeros
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(size), "n"(N) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], uint32_t at) {
+    if constexpr (WORDS == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    else if constexpr (WORDS == 2)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+}
+// Two e4m3 codes (low and high byte) as two fp16 values: exact.
+__device__ __forceinline__ uint32_t halves(uint32_t two) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"((uint16_t)two));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// What the fp16 halves of `packed` leave of (lo, hi), as fp16 again.
+__device__ __forceinline__ uint32_t pack_rest(uint32_t packed, float lo, float hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&packed));
+    return pack(lo - f.x, hi - f.y);
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// NaN codes (7F and FF) of a word: a set high bit in each such byte.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// The rows of a tile that a lane holds in its score and output fragments: columns 2 j and 2 j + 1 of each of the NQ
+// 8-row groups; the keys [first, pos] that each sees.
+template <int NQ> struct Rows {
+    int32_t first[NQ][2], pos[NQ][2];
+};
+
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(const CachedParams p) {
+    using G = Geometry<D>;
+    constexpr bool SPLIT = sizeof(T) == 4;              // fp32 rows: queries and weights as pairs of halves
+    constexpr int R = 8 * NQ, KW = G::KB / 4, VW = G::VB / 4, MT = D / 16, KT = D / 16;
+    extern __shared__ __align__(16) uint8_t ring[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+    const int64_t b = blockIdx.z;
+    const int kvh = blockIdx.y, tile = blockIdx.x % p.row_tiles, split = blockIdx.x / p.row_tiles;
     const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
-    if (i >= sp.n) return;
-    const int64_t pos = (int64_t)p.lengths[b] - sp.n + i;
-    const int64_t first = p.window ? max(pos - p.window + 1, (int64_t)0) : 0;
-    const T *q = reinterpret_cast<const T *>(p.q) + (sp.t0 + i) * p.sqt + h * p.sqh;
-    float qv[E], o[E] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) qv[e] = to_float(q[lane * E + e]) * p.scale;
-    for (int64_t j = first + warp; j <= pos; j += WARPS) {
-        const int64_t place = j / p.page_size;
-        if (place >= p.table_width) {
-            if (lane == 0) record_status(STATUS_BAD_POSITION);
-            break;
-        }
-        const int64_t page = p.table[b * p.table_stride + place];
-        if (page < 0 || page >= p.num_pages) {
-            if (lane == 0) record_status(STATUS_BAD_PAGE);
-            continue;
-        }
-        const int64_t block = page * p.kv_heads + kvh, at = (block * p.page_size + j % p.page_size) * D + lane * E;
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += qv[e] * e4m3_to_float(p.kc[at + e]);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= p.ks[block];
-        const float m2 = fmaxf(m, s), f = m2 == -INFINITY ? 1.0f : expf(m - m2);
-        const float w = s == -INFINITY ? 0.0f : expf(s - m2), vw = w * p.vs[block];
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + vw * e4m3_to_float(p.vc[at + e]);
-        m = m2;
+    const int64_t rows = sp.n * p.group;
+    const int64_t row0 = (int64_t)tile * R;
+    if (row0 >= rows) return;
+    const int live = (int)min((int64_t)R, rows - row0);
+    // positions are below 2^31 (lengths are int32); a row past the tile's last repeats the last one
+    const int32_t length = p.lengths[b];
+    const int32_t before = length - (int32_t)sp.n;      // position of query token 0
+    auto pos_of = [&](int r) { return before + (int32_t)((row0 + min(r, live - 1)) / p.group); };
+    auto first_of = [&](int32_t pos) { return p.window ? (int32_t)max((int64_t)pos - p.window + 1, (int64_t)0) : 0; };
+    const int32_t pos_lo = pos_of(0), pos_hi = pos_of(R - 1);
+    const int32_t first_lo = first_of(pos_lo), first_hi = first_of(pos_hi);
+    int64_t end = (int64_t)pos_hi + 1;                  // no row of the tile sees a key outside [first_lo, end)
+    const int64_t held = (int64_t)p.table_width << p.page_log2;
+    if (end > held) {
+        if (threadIdx.x == 0) record_status(STATUS_BAD_POSITION);
+        end = held;
     }
-    __shared__ float so[WARPS][D], sm[WARPS], sl[WARPS];
+    const int64_t begin = (int64_t)(first_lo & ~(KEYS - 1)) + (int64_t)split * p.chunk;
+    const int64_t stop = split == p.splits - 1 ? end : min(end, begin + p.chunk);
+    const int64_t mine = begin + warp * KEYS;
+    const int stages = stop > mine ? (int)((stop - mine + KEYS * WARPS - 1) / (KEYS * WARPS)) : 0;
+
+    // ---- this lane's copies ----
+    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * (G::STAGES * G::STAGE_BYTES);
+    const uint32_t scales0 = (uint32_t)__cvta_generic_to_shared(ring) + G::RING + warp * (G::STAGES * 16);
+    const int32_t page_mask = (1 << p.page_log2) - 1;
+    int32_t ids = -1, ids_next = -1;                    // pages of the 32 tiles of 16 stages, lane by lane
+    auto load_ids = [&](int s0) {                       // stages s0 .. s0 + 15
+        const int64_t key = mine + (int64_t)(s0 + (lane >> 1)) * (KEYS * WARPS) + 16 * (lane & 1);
+        if (key >= stop || key + 15 < first_lo) return -1;
+        const int32_t id = p.table[b * p.table_stride + (key >> p.page_log2)];
+        if (id >= 0 && id < p.num_pages) return id;
+        record_status(STATUS_BAD_PAGE);
+        return -1;
+    };
+    auto issue_k = [&](int s) {
+        if (s < stages) {
+            if ((s & 15) == 0) {
+                ids = s == 0 ? load_ids(0) : ids_next;
+                ids_next = load_ids(s + 16);
+            }
+            const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
+            const uint32_t at = ring0 + (s % G::STAGES) * G::STAGE_BYTES;
 #pragma unroll
-    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
+            for (int t = 0; t < 2; ++t) {
+                const int32_t id = __shfl_sync(0xffffffffu, ids, 2 * (s & 15) + t);
+                const int64_t key = key0 + 16 * t, block = (int64_t)max(id, 0) * p.kv_heads + kvh;
+                const uint8_t *src = p.kc + ((block << p.page_log2) + (key & page_mask)) * D;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = g + 8 * r;
+                    const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
+#pragma unroll
+                    for (int c = 0; c < G::KC; ++c)
+                        copy_async<G::KB>(at + (((2 * t + r) * G::KC + c) * 32 + lane) * G::KB, src + row * D + c * 64 + j * G::KB, on);
+                }
+                if (lane < 2) {                         // lane 0: the K scale, lane 1: the V scale
+                    const uint32_t to = scales0 + (s % G::STAGES) * 16 + (2 * t + lane) * 4;
+                    if (id >= 0) copy_async<4>(to, (lane ? p.vs : p.ks) + block, true);
+                    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(BAD_PAGE) : "memory");
+                }
+            }
+        }
+        commit();
+    };
+    auto issue_v = [&](int s) {
+        if (s < stages) {
+            const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
+            const uint32_t at = ring0 + (s % G::STAGES) * G::STAGE_BYTES + G::KBYTES;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int32_t id = __shfl_sync(0xffffffffu, ids, 2 * (s & 15) + t);
+                const int64_t key = key0 + 16 * t, block = (int64_t)max(id, 0) * p.kv_heads + kvh;
+                const uint8_t *src = p.vc + ((block << p.page_log2) + (key & page_mask)) * D;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 2 * j + (r & 1) + 8 * (r >> 1);
+                    const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
+                    copy_async<G::VB>(at + ((4 * t + r) * 32 + lane) * G::VB, src + row * D + g * G::VB, on);
+                }
+            }
+        }
+        commit();
+    };
+    for (int s = 0; s < G::STAGES; ++s) {
+        issue_k(s);
+        issue_v(s);
+    }
+
+    // ---- the queries: B fragments, scaled by a power of two per row ----
+    uint32_t qh[NQ][KT][2], ql[SPLIT ? NQ : 1][KT][2];
+    float factor[NQ][2];                                // scale * log2(e) / (the row's power of two)
+    Rows<NQ> seen;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int64_t r = row0 + min(8 * n + g, live - 1);
+        const T *q = reinterpret_cast<const T *>(p.q) + (sp.t0 + r / p.group) * p.sqt + (kvh * p.group + r % p.group) * p.sqh;
+        float x[KT][4], top = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+            const T *at = q + (k / KW) * 64 + j * G::KB + 4 * (k % KW);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[k][e] = to_float(at[e]);
+                top = fmaxf(top, isfinite(x[k][e]) ? fabsf(x[k][e]) : 0.0f);
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the row's largest magnitude in [2^14, 2^15)
+        const int up = top == 0.0f ? 0 : min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -112), 112);
+        const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float lo = x[k][2 * e] * f, hi = x[k][2 * e + 1] * f;
+                qh[n][k][e] = pack(lo, hi);
+                if constexpr (SPLIT) ql[n][k][e] = pack_rest(qh[n][k][e], lo, hi);
+            }
+        const float own = p.scale * LOG2E * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            factor[n][e] = __shfl_sync(0xffffffffu, own, 4 * (2 * j + e));
+            seen.pos[n][e] = pos_of(8 * n + 2 * j + e);
+            seen.first[n][e] = first_of(seen.pos[n][e]);
+        }
+    }
+
+    float o[MT][NQ][4], m[NQ][2], l[NQ][2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.0f;
+
+#pragma unroll 1
+    for (int s = 0; s < stages; ++s) {
+        const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
+        const uint32_t at = ring0 + (s % G::STAGES) * G::STAGE_BYTES;
+        wait<2 * G::STAGES - 1>();
+        __syncwarp();                                   // the scales were copied by lanes 0 and 1
+        uint32_t sc[4];
+        load_words(sc, scales0 + (s % G::STAGES) * 16);
+        const bool bad[2] = {sc[0] == BAD_PAGE, sc[2] == BAD_PAGE};
+        const float kscale[2] = {__uint_as_float(sc[0]), __uint_as_float(sc[2])};
+        // both tiles' V scales relative to the larger, so that the weights keep fp16's range
+        float vs0 = bad[0] ? 0.0f : __uint_as_float(sc[1]), vs1 = bad[1] ? 0.0f : __uint_as_float(sc[3]);
+        float vtop = fmaxf(vs0, vs1);
+        if (!(vtop > 0.0f && vtop < INFINITY)) vtop = 1.0f;
+        const float weight[2] = {vs0 == vtop ? 16384.0f : vs0 / vtop * 16384.0f, vs1 == vtop ? 16384.0f : vs1 / vtop * 16384.0f};
+        const float back = vtop * (1.0f / 16384.0f);
+
+        // ---- scores ----
+        float c[2][NQ][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[t][n][e] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < G::KC; ++h) {
+                uint32_t w0[KW], w1[KW];
+                load_words(w0, at + (((2 * t) * G::KC + h) * 32 + lane) * G::KB);
+                load_words(w1, at + (((2 * t + 1) * G::KC + h) * 32 + lane) * G::KB);
+#pragma unroll
+                for (int k = 0; k < KW; ++k) {
+                    const uint32_t a[4] = {halves(w0[k]), halves(w1[k]), halves(w0[k] >> 16), halves(w1[k] >> 16)};
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        mma(c[t][n], a, qh[n][h * KW + k][0], qh[n][h * KW + k][1]);
+                        if constexpr (SPLIT) mma(c[t][n], a, ql[n][h * KW + k][0], ql[n][h * KW + k][1]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        issue_k(s + G::STAGES);
+
+        // ---- softmax ----
+        const bool edge = key0 < first_hi || key0 + KEYS - 1 > pos_lo || key0 + KEYS > stop || bad[0] || bad[1];
+        uint32_t ph[2][NQ][2], pl[2][SPLIT ? NQ : 1][2], vis[2][NQ][2];
+        float alpha[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[t][n][e] = c[t][n][e] * factor[n][e & 1] * kscale[t];
+            uint32_t off = 0;                           // bit 4 t + e: this score's key is not seen by its row
+            if (edge) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int64_t key = key0 + 16 * t + g + 8 * (e >> 1);
+                        const bool on = !bad[t] && key >= seen.first[n][e & 1] && key <= seen.pos[n][e & 1] && key < stop;
+                        if (!on) off |= 1u << (4 * t + e), c[t][n][e] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float top = fmaxf(fmaxf(c[0][n][e], c[0][n][e + 2]), fmaxf(c[1][n][e], c[1][n][e + 2]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                const float now = fmaxf(m[n][e], top), ref = now == -INFINITY ? 0.0f : now;
+                alpha[n][e] = ex2(m[n][e] - ref);
+                m[n][e] = now;
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int x = e; x < 4; x += 2) {
+                        const float w = ex2(c[t][n][x] - ref);
+                        sum += w;
+                        c[t][n][x] = w * weight[t];
+                    }
+                l[n][e] = l[n][e] * alpha[n][e] + sum;
+            }
+            if (edge) {                                 // a scale that is NaN reaches only the rows that see its keys
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (off >> (4 * t + e) & 1) c[t][n][e] = 0.0f;
+                    const uint32_t v = ~off >> (4 * t);
+                    vis[t][n][0] = transposed((v & 1 ? 0x3C00u : 0u) | (v & 2 ? 0x3C000000u : 0u));
+                    vis[t][n][1] = transposed((v & 4 ? 0x3C00u : 0u) | (v & 8 ? 0x3C000000u : 0u));
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t hi = pack(c[t][n][2 * e], c[t][n][2 * e + 1]);
+                    ph[t][n][e] = transposed(hi);
+                    if constexpr (SPLIT) pl[t][n][e] = transposed(pack_rest(hi, c[t][n][2 * e], c[t][n][2 * e + 1]));
+                }
+        }
+
+        // ---- values ----
+        wait<2 * G::STAGES - 1>();
+        uint32_t v[2][4][VW];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) load_words(v[t][r], at + G::KBYTES + ((4 * t + r) * 32 + lane) * G::VB);
+        // A fragments of the m-tiles 2 w and 2 w + 1 (dimensions g VB + 4 w ... + 3) from a word of four keys
+        auto fragments = [](uint32_t (&a)[2][4], uint32_t k0, uint32_t k1, uint32_t k8, uint32_t k9) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t x = __byte_perm(k0, k1, i ? 0x7362 : 0x5140), y = __byte_perm(k8, k9, i ? 0x7362 : 0x5140);
+                a[i][0] = halves(x), a[i][1] = halves(x >> 16), a[i][2] = halves(y), a[i][3] = halves(y >> 16);
+            }
+        };
+        bool special = false;
+        if (edge) {                                     // NaN codes: 0 * NaN must not reach a row that does not see the key
+            uint32_t any = 0;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) any |= nan_codes(v[t][r][w]);
+            special = __any_sync(0xffffffffu, any != 0);
+        }
+        if (special) {                                  // count the NaN that each row sees, then take the codes as zeros
+#pragma unroll 1
+            for (int w = 0; w < VW; ++w) {
+                uint32_t a[2][2][4];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    uint32_t one[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        uint32_t x = v[t][r][0];
+#pragma unroll
+                        for (int y = 1; y < VW; ++y) x = w == y ? v[t][r][y] : x;
+                        one[r] = (nan_codes(x) >> 7) * 0x38u;              // e4m3's 1.0
+                    }
+                    fragments(a[t], one[0], one[1], one[2], one[3]);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        float count[4] = {};
+                        mma(count, a[0][i], vis[0][n][0], vis[0][n][1]);
+                        mma(count, a[1][i], vis[1][n][0], vis[1][n][1]);
+#pragma unroll
+                        for (int y = 0; y < VW; ++y)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (w == y && count[e] != 0.0f) o[2 * y + i][n][e] = __int_as_float(0x7FC00000);
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) v[t][r][w] &= ~((nan_codes(v[t][r][w]) >> 7) * 0xFFu);
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+            uint32_t a[2][2][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) fragments(a[t], v[t][0][w], v[t][1][w], v[t][2][w], v[t][3][w]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    float acc[4] = {};
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        mma(acc, a[t][i], ph[t][n][0], ph[t][n][1]);
+                        if constexpr (SPLIT) mma(acc, a[t][i], pl[t][n][0], pl[t][n][1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[2 * w + i][n][e] = fmaf(o[2 * w + i][n][e], alpha[n][e & 1], acc[e] * back);
+                }
+        }
+        issue_v(s + G::STAGES);
+    }
+    wait<0>();
+
+    // ---- join the warps ----
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+        }
+    __syncthreads();                                    // the queues are free
+    float *so = reinterpret_cast<float *>(ring);        // [WARPS][R][D], then [WARPS][R] of (m, l)
+    float2 *sml = reinterpret_cast<float2 *>(so + WARPS * R * D);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = 8 * n + 2 * j + e;
+            if (g == 0) sml[warp * R + r] = make_float2(m[n][e], l[n][e]);
+            float *to = so + (warp * R + r) * D + g * G::VB;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) *reinterpret_cast<float2 *>(to + 2 * i) = make_float2(o[i][n][e], o[i][n][e + 2]);
+        }
     __syncthreads();
-    float top = -INFINITY, total = 0.0f;
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm[w]);
-    float f[WARPS];
-    for (int w = 0; w < WARPS; ++w) {
-        f[w] = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - top);
-        total += f[w] * sl[w];
+    for (int x = threadIdx.x; x < live * D; x += THREADS) {
+        const int r = x / D, d = x % D;
+        float top = -INFINITY, total = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sml[w * R + r].x);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float2 ml = sml[w * R + r];
+            if (ml.y == 0.0f) continue;                 // saw no key
+            const float f = ex2(ml.x - top);
+            total += ml.y * f;
+            sum += so[(w * R + r) * D + d] * f;
+        }
+        const int64_t t = sp.t0 + (row0 + r) / p.group, h = kvh * p.group + (row0 + r) % p.group;
+        if (p.splits == 1) {
+            reinterpret_cast<T *>(p.out)[t * p.sot + h * p.soh + d] = from_float<T>(total == 0.0f ? 0.0f : sum / total);
+            if (p.lse && d == 0) p.lse[t * p.q_heads + h] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
+        } else {
+            const int64_t at = (int64_t)split * p.tokens * p.q_heads + t * p.q_heads + h;
+            p.part_o[at * D + d] = sum;
+            if (d == 0) p.part_ml[at] = make_float2(top, total);
+        }
     }
-    T *out = reinterpret_cast<T *>(p.out) + (sp.t0 + i) * p.sot + h * p.soh;
-    for (int d = threadIdx.x; d < D; d += THREADS) {
-        float acc = 0.0f;
-        for (int w = 0; w < WARPS; ++w) acc += f[w] == 0.0f ? 0.0f : f[w] * so[w][d];
-        out[d] = from_float<T>(total == 0.0f ? 0.0f : acc / total);
+}
+
+// Joins the splits of the keys: a warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS) kv_attention_join_kernel(const CachedParams p) {
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = p.tokens * p.q_heads, row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    float top = -INFINITY, total = 0.0f, sum[D / 32] = {};
+    for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[s * rows + row].x);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 ml = p.part_ml[s * rows + row];
+        if (ml.y == 0.0f) continue;
+        const float f = ex2(ml.x - top);
+        total += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) sum[e] += p.part_o[(s * rows + row) * D + e * 32 + lane] * f;
     }
-    if (p.lse && threadIdx.x == 0) p.lse[(sp.t0 + i) * p.q_heads + h] = total == 0.0f ? -INFINITY : top + logf(total);
+    const int64_t t = row / p.q_heads, h = row % p.q_heads;
+    T *out = reinterpret_cast<T *>(p.out) + t * p.sot + h * p.soh;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) out[e * 32 + lane] = from_float<T>(total == 0.0f ? 0.0f : sum[e] / total);
+    if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
+}
+
+// How a call is cut: NQ 8-row groups a tile, row tiles a (sequence, key head), splits of the keys.
+struct Plan {
+    int nq;
+    int64_t row_tiles, splits, chunk;
+};
+
+Plan plan_of(const piton_kv_attention_args *a) {
+    Plan plan;
+    const int64_t most_new = a->cu ? (a->max_new ? a->max_new : a->tokens) : a->tokens / a->batch;
+    const int64_t rows = most_new * (a->q_heads / a->kv_heads);
+    plan.nq = rows <= 8 ? 1 : 2;
+    plan.row_tiles = cdiv(rows, 8 * plan.nq);
+    // keys that a row tile can see, as far as the host knows
+    int64_t span = a->max_length ? a->max_length : a->table_width * a->page_size;
+    span = span < a->table_width * a->page_size ? span : a->table_width * a->page_size;
+    if (a->window && a->window + most_new + KEYS < span) span = a->window + most_new + KEYS;
+    // enough CTAs for every SM's three (two) and no split below 256 keys
+    const int64_t units = plan.row_tiles * a->kv_heads * a->batch, slots = (int64_t)num_sms() * (plan.nq == 1 ? 3 : 2);
+    int64_t splits = units >= slots ? 1 : slots / units;
+    const int64_t most = cdiv(span, 256);
+    splits = splits < most ? splits : most;
+    if (splits < 1) splits = 1;
+    plan.chunk = cdiv(cdiv(span, splits), KEYS * WARPS) * (KEYS * WARPS);
+    if (plan.chunk == 0) plan.chunk = KEYS * WARPS;
+    plan.splits = span > 0 ? cdiv(span, plan.chunk) : 1;
+    return plan;
+}
+
+template <typename T, int D, int NQ> int launch(const CachedParams &p, int64_t batch, cudaStream_t s) {
+    using G = Geometry<D>;
+    static_assert(WARPS * 8 * NQ * (D * 4 + 8) <= G::RING, "the warps' results fit the queues");
+    static bool known[64];
+    int dev = 0;
+    PITON_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !known[dev]) {
+        PITON_CUDA(cudaFuncSetAttribute(kv_attention_kernel<T, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+        if (dev >= 0 && dev < 64) known[dev] = true;
+    }
+    const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)p.kv_heads, (unsigned)batch);
+    kv_attention_kernel<T, D, NQ><<<grid, THREADS, G::SMEM, s>>>(p);
+    if (p.splits == 1) return check_launch("kv_attention");
+    kv_attention_join_kernel<T, D><<<(unsigned)cdiv(p.tokens * p.q_heads, WARPS), THREADS, 0, s>>>(p);
+    return check_launch("kv_attention", 2);
+}
+
+template <typename T, int D> int launch(const CachedParams &p, int nq, int64_t batch, cudaStream_t s) {
+    return nq == 1 ? launch<T, D, 1>(p, batch, s) : launch<T, D, 2>(p, batch, s);
 }
 
 }  // namespace
@@ -113,7 +604,8 @@ int check_attention(const piton_kv_attention_args *a) {
                   "bad shape");
     PITON_REQUIRE(a->q_heads % a->kv_heads == 0, "%lld query heads over %lld key heads", (long long)a->q_heads,
                   (long long)a->kv_heads);
-    PITON_REQUIRE(a->batch <= 65535 && a->tokens < (1ll << 31) && a->q_heads <= (1 << 16) && a->num_pages < (1ll << 31),
+    PITON_REQUIRE(a->batch <= 65535 && a->tokens < (1ll << 31) && a->q_heads <= 65535 && a->num_pages < (1ll << 31) &&
+                      a->table_width < (1ll << 31),
                   "batch, tokens, heads or pages too large");
     if ((a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) ||
         (a->page_size != 16 && a->page_size != 32 && a->page_size != 64 && a->page_size != 128))
@@ -126,7 +618,11 @@ int check_attention(const piton_kv_attention_args *a) {
 
 }  // namespace
 
-extern "C" size_t piton_b200_kv_attention_workspace_size(const piton_kv_attention_args *) { return 0; }
+extern "C" size_t piton_b200_kv_attention_workspace_size(const piton_kv_attention_args *a) {
+    if (check_attention(a) != PITON_B200_OK || a->batch == 0 || a->tokens == 0) return 0;
+    const Plan plan = plan_of(a);
+    return plan.splits == 1 ? 0 : (size_t)(plan.splits * a->tokens * a->q_heads) * (a->head_dim + 2) * sizeof(float);
+}
 
 extern "C" int piton_b200_kv_attention(const piton_kv_attention_args *a, void *stream) {
     if (int rc = check_attention(a)) return rc;
@@ -134,6 +630,14 @@ extern "C" int piton_b200_kv_attention(const piton_kv_attention_args *a, void *s
     PITON_REQUIRE(a->q && a->out && a->k_codes && a->v_codes && a->k_scale && a->v_scale && a->table && a->lengths,
                   "NULL pointer");
     PITON_REQUIRE(a->k_codes % 16 == 0 && a->v_codes % 16 == 0, "codes are not 16-byte aligned");
+    const Plan plan = plan_of(a);
+    const int64_t rows = a->tokens * a->q_heads;
+    const uint64_t need = plan.splits == 1 ? 0 : (uint64_t)(plan.splits * rows) * (a->head_dim + 2) * sizeof(float);
+    if (need && (!a->workspace || a->workspace_bytes < need))
+        return set_error(PITON_B200_EWORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes,
+                         (unsigned long long)need);
+    PITON_REQUIRE(a->workspace % 16 == 0 || !need, "workspace is not 16-byte aligned");
+    PITON_REQUIRE(plan.row_tiles * plan.splits < (1ll << 31) && cdiv(rows, WARPS) < (1ll << 31), "too many blocks");
     CachedParams p;
     p.q = reinterpret_cast<const void *>(a->q);
     p.out = reinterpret_cast<void *>(a->out);
@@ -145,21 +649,20 @@ extern "C" int piton_b200_kv_attention(const piton_kv_attention_args *a, void *s
     p.table = reinterpret_cast<const int32_t *>(a->table);
     p.lengths = reinterpret_cast<const int32_t *>(a->lengths);
     p.cu = reinterpret_cast<const int32_t *>(a->cu);
-    p.batch = a->batch; p.tokens = a->tokens; p.q_heads = a->q_heads; p.kv_heads = a->kv_heads;
-    p.page_size = a->page_size; p.num_pages = a->num_pages; p.table_width = a->table_width; p.table_stride = a->table_stride;
+    p.part_o = reinterpret_cast<float *>(a->workspace);
+    p.part_ml = reinterpret_cast<float2 *>(p.part_o + plan.splits * rows * a->head_dim);
+    p.tokens = a->tokens; p.num_pages = a->num_pages; p.table_stride = a->table_stride;
     p.sqt = a->stride_qt; p.sqh = a->stride_qh; p.sot = a->stride_ot; p.soh = a->stride_oh;
-    p.window = a->window;
-    p.uniform = a->cu ? 0 : a->tokens / a->batch;
-    p.max_new = a->cu ? (a->max_new ? a->max_new : a->tokens) : p.uniform;
+    p.window = a->window; p.uniform = a->cu ? 0 : a->tokens / a->batch; p.chunk = plan.chunk;
+    p.q_heads = (int32_t)a->q_heads; p.kv_heads = (int32_t)a->kv_heads; p.group = p.q_heads / p.kv_heads;
+    p.page_log2 = a->page_size == 16 ? 4 : a->page_size == 32 ? 5 : a->page_size == 64 ? 6 : 7;
+    p.table_width = (int32_t)a->table_width; p.row_tiles = (int32_t)plan.row_tiles; p.splits = (int32_t)plan.splits;
     p.scale = (float)a->sm_scale;
-    PITON_REQUIRE(p.max_new <= 65535, "%lld query tokens a sequence", (long long)p.max_new);
-    const dim3 grid((unsigned)a->q_heads, (unsigned)p.max_new, (unsigned)a->batch);
     return with_type(a->type, [&](auto t) {
         using T = decltype(t);
         cudaStream_t s = as_stream(stream);
-        if (a->head_dim == 32) kv_attention_kernel<T, 32><<<grid, THREADS, 0, s>>>(p);
-        else if (a->head_dim == 64) kv_attention_kernel<T, 64><<<grid, THREADS, 0, s>>>(p);
-        else kv_attention_kernel<T, 128><<<grid, THREADS, 0, s>>>(p);
-        return check_launch("kv_attention");
+        if (a->head_dim == 32) return launch<T, 32>(p, plan.nq, a->batch, s);
+        if (a->head_dim == 64) return launch<T, 64>(p, plan.nq, a->batch, s);
+        return launch<T, 128>(p, plan.nq, a->batch, s);
     });
 }
