@@ -1,240 +1,485 @@
 // y = x W^T (+ bias) with 4-bit weights W[n, k] = scale[n, k / group] (code[n, k] - zero[n, k / group]), for a few rows x.
 //
 // The codes are read once (N K / 2 bytes) and bound the product up to about 16 rows, so everything is
-// arranged around streaming them.  A warp takes 16 weight rows and a share of the inner dimension in blocks of
-// 128; its lanes copy 16 bytes of a row each (cp.async, zero-filled past the row's end) into a queue of their own
-// warp, three or more blocks deep, so no warp waits for another before the end.  A code minus its zero point is exact in
-// fp16 (the nibble is put into the low bits of 1024's significand), weights are the 16-row side of mma.m16n8k16 and
-// the rows of x its 8-column side, and each group's sum is scaled in fp32: no weight is ever rounded.
-// 16-bit rows of x enter as they are (scaled by a power of two per row and block); fp32 rows as two
-// fp16 halves (22 bits).
+// arranged around streaming them with few instructions a byte.  A warp takes 16 R weight rows in steps of 256 inner
+// elements (128 bytes of a row), copied with cp.async into a queue of its own, so no warp waits for another while it
+// streams.  The sums over a group are taken exactly in integers: a nibble is a byte after one mask, and the rows of x
+// are laid out once per CTA in shared memory as fixed-point numbers of their block's largest magnitude, two signed
+// 8-bit digits for 16-bit types (error below 2^-16 of that magnitude, where the types' own roundings are 2^-9 and
+// 2^-12 of each element) and three for fp32 (2^-24).  Codes are the 16-row side of the integer mma.m16n8k32
+// and the digits of x its 8-column side; what the accumulators hold is less than 2^22, so started at the bits of
+// 1.5 2^23 they are read back as floats by one subtraction.  The zero point's share, zero * sum(x), and the group's
+// scale are applied in fp32.  Against products with fp16 or bf16 weights (built first) this takes 3 instead of 9 or 11
+// instructions per 8 codes, and instruction issue is what bounds the kernel.  A block of x with a non-finite element
+// makes its row of y NaN.
+//
+// A matrix with many rows gives every warp rows of its own (warps along the rows); one with few splits each
+// CTA's inner dimension over its eight warps (warps along the inner dimension).  Either way a cluster of CTAs
+// may split the inner dimension further, and adds its parts through distributed shared memory in a fixed order.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
 #include "decode.cuh"
 
 namespace piton {
 namespace decode {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
-constexpr int BLOCK = 128;                  // inner elements of a block: 64 bytes of each of 16 rows
-constexpr int QUAD = 80;                    // bytes a row takes in the queue: 64 and 16 that keep reads free of bank conflicts
-constexpr int SLOT = 16 * QUAD;
+constexpr int BLOCK = 128;                  // inner elements that share a scale of x
+constexpr int LINE = 128;                   // bytes of a weight row in a step: two blocks
+constexpr int MAX_PARTS = 8;
 
 struct MatvecParams {
     const void *x, *scales, *bias;
     const uint8_t *codes, *zeros;
     void *y;
-    int64_t rows, inner, outer, sx, sc, ss, sz, sy;
-    int32_t group_log2, scale_type, aligned;
+    int64_t rows, outer, sx, sc, ss, sz, sy;
+    int32_t inner, group_log2, scale_type, codes_align, x_aligned;
+    int32_t span, phase;                    // steps of a CTA's part, and of what shared memory holds of x at a time
 };
 
-__device__ __forceinline__ float load_scale(const void *p, int32_t type, int64_t i) {
-    if (type == PITON_B200_TYPE_F32) return reinterpret_cast<const float *>(p)[i];
-    if (type == PITON_B200_TYPE_F16) return to_float(reinterpret_cast<const __half *>(p)[i]);
-    return to_float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
+// An integer v below 2^22 in magnitude, kept as MAGIC + v, read as a float is 1.5 2^23 + v.
+constexpr int32_t MAGIC = 0x4B400000;
+__device__ __forceinline__ float value_of(int32_t v) { return __int_as_float(v) - 12582912.0f; }
+
+// d = a b + d, or a b + MAGIC.
+template <bool FIRST> __device__ __forceinline__ void mma(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    const int32_t c[4] = {FIRST ? MAGIC : d[0], FIRST ? MAGIC : d[1], FIRST ? MAGIC : d[2], FIRST ? MAGIC : d[3]};
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint32_t pack_rest(uint32_t packed, float lo, float hi) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&packed));
-    return pack(lo - f.x, hi - f.y);
+// `count` bytes of the 16, one by one and at any alignment; the rest becomes 0.
+__device__ __forceinline__ void copy16_slow(uint32_t dst, const uint8_t *src, int count) {
+#pragma unroll 1
+    for (int w = 0; w < 4; ++w) {
+        uint32_t word = 0;
+        for (int i = 0; i < 4; ++i)
+            if (4 * w + i < count) word |= (uint32_t)src[4 * w + i] << (8 * i);
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 4 * w), "r"(word) : "memory");
+    }
 }
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
+__device__ __forceinline__ uint4 load16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
 }
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
+template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], uint32_t at) {
+    if constexpr (WORDS == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    else if constexpr (WORDS == 2)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
 
-// The zero point of a group as the two constants that turn nibbles into code - zero.
-struct Zero {
-    uint32_t low, high;                     // 1024 + zero and -(64 + zero), twice each
+// NT tiles of 8 rows of x, R tiles of 16 weight rows a warp, GROUPS = 128 / group scales of a weight row in a block.
+template <typename T, int NT, int R, int GROUPS> struct Shape {
+    // Of each group's 32 WORDS elements in a block lane j takes the 8 WORDS from 8 WORDS j on: WORDS words of codes.
+    static constexpr int WORDS = 4 / GROUPS;
+    static constexpr int SLOT = 16 * R * LINE, STAGES = R == 1 ? 4 : 2, QUEUES = WARPS * STAGES * SLOT;
+    static constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;               // of x; the first holds the most
+    static constexpr int SUMS = 8 * NT * 16 * R;                        // outputs of a warp's tile
+    // x in shared memory, per row: 16 bytes for every 8 elements (their first two digits), 8 more for fp32 (the third), and per
+    // block a scale and each group's sum; paddings put rows that are read together into different banks
+    static constexpr int META = 1 + GROUPS;                             // words of a block
+    __host__ __device__ static constexpr int pitch(int steps) { return steps * 512 + 64; }
+    __host__ __device__ static constexpr int pitch3(int steps) { return DIGITS == 3 ? steps * 256 + 32 : 0; }
+    // shared memory: queues (in the end the warps' sums), x
+    static_assert(WARPS * SUMS * 4 <= QUEUES, "the sums fit");
+    static int64_t smem(int64_t rows, int64_t steps) {
+        return QUEUES + rows * (steps * (512 + (DIGITS == 3 ? 256 : 0) + 2 * META * 4) + 96);
+    }
 };
-__device__ __forceinline__ Zero zero_of(uint32_t z) {
-    const __half2 a = __half2half2(__uint2half_rn(1024 + z)), b = __half2half2(__int2half_rn(-(int)(64 + z)));
-    return {*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b)};
-}
-// The eight codes of a word less the zero point, as pairs (0, 4), (1, 5), (2, 6), (3, 7).
-__device__ __forceinline__ void weights_of(uint32_t (&h)[4], uint32_t w, const Zero &z) {
-    const uint32_t sixteenth = 0x2C002C00u;
-    h[0] = hsub2((w & 0x000F000Fu) | 0x64006400u, z.low);                          // 1024 + code
-    h[1] = hfma2((w & 0x00F000F0u) | 0x64006400u, sixteenth, z.high);              // 1024 + 16 code
-    w >>= 8;
-    h[2] = hsub2((w & 0x000F000Fu) | 0x64006400u, z.low);
-    h[3] = hfma2((w & 0x00F000F0u) | 0x64006400u, sixteenth, z.high);
-}
 
-// NT tiles of 8 rows of x; GROUPS = 128 / group scales of a weight row in a block.
-template <typename T, int NT, int GROUPS, int STAGES>
-__global__ void __launch_bounds__(THREADS) matvec_w4_kernel(const MatvecParams p) {
-    constexpr bool SPLIT = sizeof(T) == 4;
-    constexpr int CHUNKS = 4 / GROUPS;                      // 32-element chunks of a block that share a scale
-    extern __shared__ __align__(16) uint8_t queue[];
+// ALONG_K: the CTA's warps share 16 R weight rows and split the inner dimension; otherwise each has rows of its own.
+template <typename T, int NT, int R, int GROUPS, bool ALONG_K>
+__global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParams p) {
+    using S = Shape<T, NT, R, GROUPS>;
+    constexpr int WORDS = S::WORDS, STAGES = S::STAGES, STRIDE = ALONG_K ? WARPS : 1, DIGITS = S::DIGITS, STEP = 2 * BLOCK;
+    extern __shared__ __align__(128) uint8_t queue[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (8 * NT);
-    const int64_t blocks = (p.inner + BLOCK - 1) / BLOCK, bytes = (p.inner + 1) / 2;
-    const int mine = blocks > warp ? (int)((blocks - warp + WARPS - 1) / WARPS) : 0;
-    const uint8_t *slots = queue + warp * (STAGES * SLOT);
-    const uint32_t at0 = (uint32_t)__cvta_generic_to_shared(slots);
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    const int64_t m0 = (int64_t)blockIdx.y * (8 * NT);
+    const int x_rows = (int)min((int64_t)(8 * NT), p.rows - m0);
+    const int step0 = part * p.span, steps = max(min(p.span, (p.inner + STEP - 1) / STEP - step0), 0);   // this CTA's
+    const int own0 = ALONG_K ? warp : 0, own = steps > own0 ? (steps - own0 + STRIDE - 1) / STRIDE : 0;  // this warp's
 
-    // lane (g, j): bytes 16 j ... 16 j + 15 of a block of weight rows n0 + g and n0 + g + 8
-    auto issue = [&](int s) {
-        if (s < mine) {
-            const int64_t byte = (int64_t)(warp + s * WARPS) * (BLOCK / 2) + 16 * j;
-            const int64_t left = bytes - byte;
-            const int size = left >= 16 ? 16 : (left > 0 ? (int)left : 0);
+    // A warp's weight rows; the last ones are moved back to end with the matrix, so that all 16 R exist (R > 1 only where outer
+    // >= 16 R); rows that are computed twice come out the same both times.
+    const int64_t tile = (int64_t)(blockIdx.x / parts) * (ALONG_K ? 1 : WARPS) + (ALONG_K ? 0 : warp);
+    const int64_t n0 = min(tile * (16 * R), max(p.outer - 16 * R, (int64_t)0));
+    const int rows = (int)min((int64_t)(16 * R), p.outer - n0);
+    // the weight row (and that + 8) of a tile that fragment row g is: rows that are read together lie in different banks
+    const int row = WORDS == 4 ? (g & 1) << 2 | g >> 1 : WORDS == 2 ? (g & 3) << 1 | g >> 2 : g;
+
+    // ---- the queue: in a slot, row r's 128 bytes lie at 128 r, its 16-byte pieces exchanged by r % 8 ----
+    const uint32_t at0 = (uint32_t)__cvta_generic_to_shared(queue) + warp * (STAGES * S::SLOT);
+    const uint8_t *codes = p.codes + n0 * p.sc + (int64_t)(step0 + own0) * LINE;
+    const uint32_t copy_at = (lane >> 3) * LINE + ((lane & 7) ^ (lane >> 3)) * 16;
+    uint32_t fill = at0;
+    int issued = 0;
+    auto issue = [&]() {
+        if (issued < own) {
+            const bool whole = (step0 + own0 + issued * STRIDE + 1) * STEP <= p.inner;
+            if (whole && p.codes_align == 16) {                         // 4 rows a copy, 8 lanes each
+                const uint8_t *src = codes + (lane >> 3) * p.sc + 16 * (lane & 7);
+                const uint32_t dst[2] = {fill + copy_at, (fill + copy_at) ^ 64};     // rows r and r + 4: pieces exchanged by 4
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t n = n0 + g + 8 * r;
-                const int have = n < p.outer ? size : 0;
-                const uint8_t *src = p.codes + (have ? n * p.sc + byte : 0);
-                const uint32_t dst = at0 + (s % STAGES) * SLOT + (g + 8 * r) * QUAD + 16 * j;
-                if (p.aligned) {
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
-                } else {                                    // rows that do not start on 16 bytes: byte by byte
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t word = 0;
-                        for (int i = 0; i < 4; ++i)
-                            if (4 * w + i < have) word |= (uint32_t)src[4 * w + i] << (8 * i);
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 4 * w), "r"(word) : "memory");
-                    }
+                for (int i = 0; i < 4 * R; ++i) {
+                    if (R > 1 || 4 * i + (lane >> 3) < rows) copy16(dst[i & 1] + 512 * i, src);
+                    src += 4 * p.sc;
+                }
+            } else if (whole && p.codes_align == 4) {                   // a row a copy
+                const uint8_t *src = codes + 4 * lane;
+#pragma unroll 8
+                for (int r = 0; r < 16 * R; ++r) {
+                    if (R > 1 || r < rows) copy4(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src);
+                    src += p.sc;
+                }
+            } else {                                                    // the last step, or rows that are not aligned
+                const int left = (p.inner + 1) / 2 - (step0 + own0 + issued * STRIDE) * LINE - 16 * (lane & 7);
+#pragma unroll 1
+                for (int r = lane >> 3; r < rows; r += 4) {
+                    const uint32_t dst = fill + 128 * r + ((lane & 7) ^ (r & 7)) * 16;
+                    const uint8_t *src = codes + r * p.sc + 16 * (lane & 7);
+                    if (p.codes_align == 16 && left >= 16) copy16(dst, src);
+                    else copy16_slow(dst, src, left);
                 }
             }
+            codes += STRIDE * LINE;
+            ++issued;
+            fill = fill == at0 + (STAGES - 1) * S::SLOT ? at0 : fill + S::SLOT;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) issue(s);
+    for (int s = 0; s < STAGES - 1; ++s) issue();
 
-    float acc[NT][4];
+    // ---- scales and zero points, a load ahead: lane (g, j) holds those of its 2 R weight rows for one group in four: with
+    // group 128 the four groups of two steps, with 64 those of a step, with 32 those of a block (two loads a step); zero points
+    // of the rows share a word, four bits each ----
+    constexpr int LOADS = GROUPS == 4 ? 2 : 1, AHEAD = GROUPS == 1 ? 2 : 1;    // loads in a step, steps of a load
+    uint32_t scale[LOADS][2 * R], scale_next[LOADS][2 * R], zeros[LOADS], zeros_next[LOADS];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int l = 0; l < LOADS; ++l) zeros[l] = zeros_next[l] = 0x88888888u;
+    const int groups = (p.inner + (1 << p.group_log2) - 1) >> p.group_log2;
+    const int64_t scale_row = (n0 + row) * p.ss, zero_row = (n0 + row) * p.sz;
+    auto fetch = [&](int turn) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
-
-#pragma unroll 1
-    for (int s = 0; s < mine; ++s) {
-        const int64_t blk = warp + (int64_t)s * WARPS, k0 = blk * BLOCK;
-        // scales and zero points of weight rows n0 + g and n0 + g + 8
-        float scale[GROUPS][2];
-        Zero zero[GROUPS][2];
+        for (int l = 0; l < LOADS; ++l) {
+            const int step = step0 + own0 + (turn + (GROUPS == 1 ? j >> 1 : 0)) * STRIDE;
+            const int group = step * (2 * GROUPS) + (GROUPS == 1 ? j & 1 : 4 * l + j);
+            const bool in = turn + (GROUPS == 1 ? j >> 1 : 0) < own && group < groups;
+            if (p.scale_type == PITON_B200_TYPE_F32) {
+                const uint32_t *at = reinterpret_cast<const uint32_t *>(p.scales) + scale_row + group;
 #pragma unroll
-        for (int q = 0; q < GROUPS; ++q)
+                for (int h = 0; h < 2 * R; ++h) scale_next[l][h] = in && row + 8 * h < rows ? at[8 * h * p.ss] : 0;
+            } else {
+                const uint16_t *at = reinterpret_cast<const uint16_t *>(p.scales) + scale_row + group;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t n = n0 + g + 8 * r, group = (k0 >> p.group_log2) + q;
-                const bool on = n < p.outer && (group << p.group_log2) < p.inner;
-                scale[q][r] = on ? load_scale(p.scales, p.scale_type, n * p.ss + group) : 0.0f;
-                zero[q][r] = zero_of(on && p.zeros ? p.zeros[n * p.sz + group] : 8);
+                for (int h = 0; h < 2 * R; ++h) scale_next[l][h] = in && row + 8 * h < rows ? at[8 * h * p.ss] : 0;
             }
-        // rows of x: lane (g, j) holds row m0 + 8 t + g, elements 8 j ... 8 j + 7 of each 32-element chunk, scaled by a
-        // power of two that brings the block's largest magnitude into [2^14, 2^15)
-        uint32_t xh[NT][4][4], xl[SPLIT ? NT : 1][4][4];
-        float back[NT][2];                                  // of rows 2 j and 2 j + 1, the columns of the accumulators
+            if (p.zeros) {
+                const uint8_t *at = p.zeros + zero_row + group;
+                zeros_next[l] = 0;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int64_t m = m0 + 8 * t + g;
-            const T *x = reinterpret_cast<const T *>(p.x) + (m < p.rows ? m * p.sx : 0);
-            float v[4][8], top = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int64_t k = k0 + 32 * c + 8 * j + e;
-                    v[c][e] = m < p.rows && k < p.inner ? to_float(x[k]) : 0.0f;
-                    top = fmaxf(top, isfinite(v[c][e]) ? fabsf(v[c][e]) : 0.0f);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int up = top == 0.0f ? 0 : min(max(14 + 127 - (int)(__float_as_uint(top) >> 23), -112), 112);
-            const float f = __uint_as_float((uint32_t)(127 + up) << 23), inv = __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float lo = v[c][e] * f, hi = v[c][e + 4] * f;
-                    xh[t][c][e] = pack(lo, hi);
-                    if constexpr (SPLIT) xl[t][c][e] = pack_rest(xh[t][c][e], lo, hi);
-                }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) back[t][e] = __shfl_sync(0xffffffffu, inv, 4 * (2 * j + e));
+                for (int h = 0; h < 2 * R; ++h) zeros_next[l] |= (in && row + 8 * h < rows ? at[8 * h * p.sz] & 15u : 0u) << (4 * h);
+            }
         }
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-        __syncwarp();
-        const uint32_t at = at0 + (s % STAGES) * SLOT + g * QUAD + 4 * j;
+    };
+    fetch(0);
+
+    // ---- x in shared memory ----
+    uint8_t *xs = queue + S::QUEUES;
+    uint8_t *x3 = xs + x_rows * S::pitch(p.phase);
+    float *meta = reinterpret_cast<float *>(x3 + x_rows * S::pitch3(p.phase));      // [x row][block of the phase][META]
+    // Lays out steps phase0 ... of the part: per row and block 16 units of 8 elements, unit 4 c + j for word c of lane j (word w
+    // of group q: c = q WORDS + w), which faces elements 32 WORDS q + 8 WORDS j + 8 w ... of the block. A unit's bytes
+    // are its elements 0, 2, 4, 6 (the low nibbles of the word) and 1, 3, 5, 7.
+    auto lay_out = [&](int phase0) {
+        const int count = 2 * min(p.phase, steps - phase0), units = x_rows * count * 16;
+        for (int u0 = 0; u0 < units; u0 += THREADS) {
+            const int u = u0 + threadIdx.x, unit = u & 15, c = unit >> 2, b = (u >> 4) % count, m = (u >> 4) / count;
+            const int k = (2 * (step0 + phase0) + b) * BLOCK + c / WORDS * (32 * WORDS) + 8 * WORDS * (unit & 3) + 8 * (c % WORDS);
+            const bool in = u < units;
+            const T *src = reinterpret_cast<const T *>(p.x) + (m0 + (in ? m : 0)) * p.sx + k;
+            T v[8];
+            if (in && k + 8 <= p.inner && p.x_aligned) {
 #pragma unroll
-        for (int q = 0; q < GROUPS; ++q) {
-            float part[NT][4];
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(src)[i];
+            } else {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int i = 0; i < 8; ++i) v[i] = in && k + i < p.inner ? src[i] : from_float<T>(0.0f);
+            }
+            float f[8], top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) part[t][e] = 0.0f;
+            for (int i = 0; i < 8; ++i) {
+                f[i] = to_float(v[i]);
+                top = fmaxf(top, isfinite(f[i]) ? fabsf(f[i]) : INFINITY);
+            }
 #pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) {
-                const int c = q * CHUNKS + i;
-                uint32_t w0, w1, h0[4], h1[4];              // word j of chunk c: elements 8 j ... 8 j + 7 of its 32
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(at + 16 * c) : "memory");
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(at + 16 * c + 8 * QUAD) : "memory");
-                weights_of(h0, w0, zero[q][0]);
-                weights_of(h1, w1, zero[q][1]);
+            for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // the largest magnitude becomes 127 in the first digit and 0 in the others
+            constexpr float LIMIT = DIGITS == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
+            const bool finite = top < INFINITY;
+            const float up = !finite ? 0.0f : fminf(LIMIT / fmaxf(top, 1e-37f), 8.5070592e37f), down = !finite ? __int_as_float(0x7FC00000) : 1.0f / up;
+            uint32_t digit[3][2] = {};
+            int32_t sum = 0;
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const uint32_t a[4] = {h0[e], h1[e], h0[e + 1], h1[e + 1]};
+            for (int i = 0; i < 8; ++i) {
+                int32_t q = finite ? __float2int_rn(f[i] * up) : 0;
+                sum += q;
+#pragma unroll
+                for (int d = DIGITS - 1; d >= 0; --d) {
+                    const int32_t low = d ? (int32_t)(int8_t)q : q;     // the remainder in -128 ... 127
+                    q = (q - low) >> 8;
+                    digit[d][i & 1] |= (uint32_t)(low & 255) << (8 * (i >> 1));
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < 4 * WORDS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);    // a group's units: below 2^30
+            if (in) {
+                *reinterpret_cast<uint4 *>(xs + m * S::pitch(p.phase) + (b * 16 + unit) * 16) = make_uint4(digit[0][0], digit[0][1], digit[1][0], digit[1][1]);
+                if constexpr (DIGITS == 3) *reinterpret_cast<uint2 *>(x3 + m * S::pitch3(p.phase) + (b * 16 + unit) * 8) = make_uint2(digit[2][0], digit[2][1]);
+                float *to = meta + (m * 2 * p.phase + b) * S::META;
+                if (unit == 0) to[0] = down;
+                if (unit % (4 * WORDS) == 0) to[1 + unit / (4 * WORDS)] = (float)sum;
+            }
+        }
+    };
+    // rows of x past the last read the last: a column of the product depends on its own row alone
+    uint32_t x_at[NT], x3_at[NT];
+    const float *meta_at[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int m = min(8 * t + g, x_rows - 1);
+        x_at[t] = (uint32_t)__cvta_generic_to_shared(xs) + m * S::pitch(p.phase) + 16 * j;
+        x3_at[t] = (uint32_t)__cvta_generic_to_shared(x3) + m * S::pitch3(p.phase) + 8 * j;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) meta_at[t][e] = meta + min(8 * t + 2 * j + e, x_rows - 1) * (2 * p.phase * S::META);
+    }
+
+    float acc[R][NT][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[r][t][e] = 0.0f;
+
+    uint32_t slot = at0;
+    int turn = 0;
+#pragma unroll 1
+    for (int phase0 = 0; phase0 < steps; phase0 += p.phase) {
+        if (phase0) __syncthreads();                                    // the last phase's x has been read
+        lay_out(phase0);
+        __syncthreads();
+        const int phase_end = min(phase0 + p.phase, steps);
+#pragma unroll 1
+        for (; own0 + turn * STRIDE < phase_end; ++turn) {
+            if (AHEAD == 1 || !(turn & 1)) {
+#pragma unroll
+                for (int l = 0; l < LOADS; ++l) {
+                    zeros[l] = zeros_next[l];
+                    if (p.scale_type == PITON_B200_TYPE_F32) {
+#pragma unroll
+                        for (int h = 0; h < 2 * R; ++h) scale[l][h] = scale_next[l][h];
+                    } else if (p.scale_type == PITON_B200_TYPE_BF16) {
+#pragma unroll
+                        for (int h = 0; h < 2 * R; ++h) scale[l][h] = scale_next[l][h] << 16;
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 2 * R; ++h) scale[l][h] = __float_as_uint(__half2float(__ushort_as_half((uint16_t)scale_next[l][h])));
+                    }
+                }
+                fetch(turn + AHEAD);
+            }
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();                                               // every lane's copies, and the slot that is filled next has been read
+            issue();
+            const int b0 = 2 * (own0 + turn * STRIDE - phase0);         // block of the phase
+            const uint32_t wat = slot + row * LINE;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float back[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) back[t][e] = meta_at[t][e][(b0 + b) * S::META];
+#pragma unroll
+                for (int q = 0; q < GROUPS; ++q) {
+                    uint4 x12[NT][WORDS];
+                    uint2 x3v[NT][WORDS];
+                    float x_sum[NT][2];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        mma(part[t], a, xh[t][c][e], xh[t][c][e + 1]);
-                        if constexpr (SPLIT) mma(part[t], a, xl[t][c][e], xl[t][c][e + 1]);
+#pragma unroll
+                        for (int i = 0; i < WORDS; ++i) {
+                            x12[t][i] = load16(x_at[t] + (b0 + b) * 256 + (q * WORDS + i) * 64);
+                            x3v[t][i] = make_uint2(0, 0);
+                            if constexpr (DIGITS == 3)
+                                asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x3v[t][i].x), "=r"(x3v[t][i].y)
+                                             : "r"(x3_at[t] + (b0 + b) * 128 + (q * WORDS + i) * 32) : "memory");
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) x_sum[t][e] = meta_at[t][e][(b0 + b) * S::META + 1 + q];
+                    }
+                    constexpr int LAST = LOADS - 1;
+                    const int load = GROUPS == 4 ? b & LAST : 0;
+                    const int from = (lane & ~3) | (GROUPS == 1 ? (turn & 1) * 2 + b : GROUPS == 2 ? 2 * b + q : q);
+                    const uint32_t z = __shfl_sync(0xffffffffu, zeros[load], from);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        float s2[2], z2[2];
+                        uint32_t w[2][WORDS];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            s2[h] = __uint_as_float(__shfl_sync(0xffffffffu, scale[load][2 * r + h], from));
+                            z2[h] = value_of(MAGIC | (z >> (8 * r + 4 * h) & 15));
+                            // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of row 16 r + row + 8 h
+                            const int piece = 4 * b + WORDS * q + (WORDS * j >> 2);
+                            load_words(w[h], wat + (16 * r + 8 * h) * LINE + ((piece ^ (row & 7)) * 16) + (4 * WORDS * j & 15));
+                        }
+                        int32_t sum[NT][DIGITS][4];
+#pragma unroll
+                        for (int i = 0; i < WORDS; ++i) {
+                            constexpr uint32_t LOW = 0x0F0F0F0Fu;
+                            const uint32_t a[4] = {w[0][i] & LOW, w[1][i] & LOW, w[0][i] >> 4 & LOW, w[1][i] >> 4 & LOW};
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                const uint32_t x[6] = {x12[t][i].x, x12[t][i].y, x12[t][i].z, x12[t][i].w, x3v[t][i].x, x3v[t][i].y};
+#pragma unroll
+                                for (int d = 0; d < DIGITS; ++d) {
+                                    if (i == 0) mma<true>(sum[t][d], a, x[2 * d], x[2 * d + 1]);
+                                    else mma<false>(sum[t][d], a, x[2 * d], x[2 * d + 1]);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float v = value_of(sum[t][0][e]);
+#pragma unroll
+                                for (int d = 1; d < DIGITS; ++d) v = fmaf(v, 256.0f, value_of(sum[t][d][e]));
+                                v = fmaf(-z2[e >> 1], x_sum[t][e & 1], v);
+                                acc[r][t][e] = fmaf(v, back[t][e & 1] * s2[e >> 1], acc[r][t][e]);
+                            }
                     }
                 }
             }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[t][e] += part[t][e] * back[t][e & 1] * scale[q][e >> 1];
+            slot = slot == at0 + (STAGES - 1) * S::SLOT ? at0 : slot + S::SLOT;
         }
-        __syncwarp();                                       // every lane has read the slot that is filled next
-        issue(s + STAGES - 1);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- the warps' and the cluster's sums ----
+    __syncthreads();                                                    // the queues are free
+    float *sums = reinterpret_cast<float *>(queue);                     // [warp][8 NT rows of x][16 R weight rows]
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sums[warp * S::SUMS + (8 * t + 2 * j + (e & 1)) * (16 * R) + 16 * r + row + 8 * (e >> 1)] = acc[r][t][e];
     __syncthreads();
-    float *sums = reinterpret_cast<float *>(queue);         // [WARPS][8 NT rows of x][16 weight rows]
+    constexpr int ADD = ALONG_K ? WARPS : 1, TILES = WARPS / ADD;       // warps that share a tile, tiles of the CTA
+    if (ALONG_K && parts > 1) {
+        for (int i = threadIdx.x; i < S::SUMS; i += THREADS) {
+            float sum = 0.0f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sums[(warp * 8 * NT + 8 * t + 2 * j + (e & 1)) * 16 + g + 8 * (e >> 1)] = acc[t][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 128 * NT; i += THREADS) {
-        const int64_t m = m0 + (i >> 4), n = n0 + (i & 15);
-        if (m >= p.rows || n >= p.outer) continue;
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) sum += sums[w * 128 * NT + i];
-        if (p.bias) sum += to_float(reinterpret_cast<const T *>(p.bias)[n]);
-        reinterpret_cast<T *>(p.y)[m * p.sy + n] = from_float<T>(sum);
+            for (int w = 0; w < ADD; ++w) sum += sums[w * S::SUMS + i];
+            sums[i] = sum;                                              // read by this thread alone before
+        }
     }
+    if (parts > 1) cluster.sync();
+    // CTA `part` stores its share of the outputs
+    const int outputs = TILES * x_rows * (16 * R), share = (outputs + parts - 1) / parts;
+    for (int i = part * share + threadIdx.x; i < min((part + 1) * share, outputs); i += THREADS) {
+        const int n = i % (16 * R), m = i / (16 * R) % x_rows, w = i / (16 * R * x_rows);
+        const int64_t t = (int64_t)(blockIdx.x / parts) * TILES + w;
+        if (t * (16 * R) >= p.outer) continue;
+        const int64_t at = min(t * (16 * R), max(p.outer - 16 * R, (int64_t)0)) + n;
+        if (at >= p.outer) continue;
+        float sum = 0.0f;
+        float *from = sums + w * S::SUMS + m * (16 * R) + n;
+        if (parts > 1) {
+            for (int c = 0; c < parts; ++c) sum += *cluster.map_shared_rank(from, c);
+        } else {
+#pragma unroll
+            for (int x = 0; x < ADD; ++x) sum += from[x * S::SUMS];
+        }
+        if (p.bias) sum += to_float(reinterpret_cast<const T *>(p.bias)[at]);
+        reinterpret_cast<T *>(p.y)[(m0 + m) * p.sy + at] = from_float<T>(sum);
+    }
+    if (parts > 1) cluster.sync();                                      // shared memory stays until the others have read it
 }
 
-template <typename T, int NT, int GROUPS> int launch(const MatvecParams &p, cudaStream_t s) {
-    constexpr int STAGES = 4, SMEM = WARPS * STAGES * SLOT;
-    static_assert(WARPS * 128 * NT * 4 <= SMEM && SMEM <= 48 * 1024, "the warps' sums fit the queues");
-    const dim3 grid((unsigned)cdiv(p.outer, 16), (unsigned)cdiv(p.rows, 8 * NT));
-    matvec_w4_kernel<T, NT, GROUPS, STAGES><<<grid, THREADS, SMEM, s>>>(p);
+template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(MatvecParams p, int parts, cudaStream_t s) {
+    using S = Shape<T, NT, R, GROUPS>;
+    const int64_t x_rows = p.rows < 8 * NT ? p.rows : 8 * NT;
+    p.span = (int32_t)cdiv(cdiv(p.inner, 2 * BLOCK), parts);
+    // x whole, or as many of its steps as leave room for a second CTA
+    p.phase = p.span > 0 ? p.span : 1;
+    while (S::smem(x_rows, p.phase) > 113 * 1024 && p.phase > 1) p.phase = (p.phase + 1) / 2;
+    static bool known[64];
+    int dev = 0;
+    PITON_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !known[dev]) {
+        PITON_CUDA(cudaFuncSetAttribute(matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
+        if (dev >= 0 && dev < 64) known[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(cdiv(p.outer, ALONG_K ? 16 * R : 16 * R * WARPS) * parts), (unsigned)cdiv(p.rows, 8 * NT));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = (size_t)S::smem(x_rows, p.phase);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)parts;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    PITON_CUDA(cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K>, p));
     return check_launch("matvec_w4");
 }
 
-template <typename T, int NT> int launch(const MatvecParams &p, cudaStream_t s) {
-    return p.group_log2 == 7 ? launch<T, NT, 1>(p, s) : p.group_log2 == 6 ? launch<T, NT, 2>(p, s) : launch<T, NT, 4>(p, s);
+template <typename T, int NT, int R, bool ALONG_K> int launch(const MatvecParams &p, int parts, cudaStream_t s) {
+    return p.group_log2 == 7 ? launch<T, NT, R, 1, ALONG_K>(p, parts, s)
+           : p.group_log2 == 6 ? launch<T, NT, R, 2, ALONG_K>(p, parts, s) : launch<T, NT, R, 4, ALONG_K>(p, parts, s);
+}
+
+template <typename T, int NT> int launch(MatvecParams p, cudaStream_t s) {
+    const int64_t tiles = cdiv(p.outer, 16), sms = num_sms(), steps = cdiv(p.inner, 2 * BLOCK);
+    const int64_t most = steps < MAX_PARTS ? steps : MAX_PARTS;
+    // Warps along the rows from 2 x 148 tiles of 16 weight rows on, in as many parts of the inner dimension as two CTAs an SM
+    // take in one wave (28000 x 8192, bf16, one row: 2 parts 29.4 us, 1 part 36.6, 4 parts 32.2; warps along the inner
+    // dimension 40); below that along the inner dimension (4096 x 4096: 6.2 us, along the rows 6.2 to 9), split
+    // further only while SMs are idle and every warp keeps two steps (1024 x 8192: 4 parts 5.5 us, 1 part 7.8).
+    int64_t parts = 1;
+    if (tiles >= 2 * sms) {
+        const int64_t groups = cdiv(tiles, 2 * WARPS);
+        parts = 2 * sms / groups;
+        parts = parts > most ? most : parts < 1 ? 1 : parts;
+        return launch<T, NT, 2, false>(p, (int)parts, s);
+    }
+    while (2 * parts <= most && tiles * 2 * parts <= 2 * sms && steps >= WARPS * 2 * parts) parts *= 2;
+    return launch<T, NT, 1, true>(p, (int)parts, s);
 }
 
 }  // namespace
@@ -251,7 +496,7 @@ extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream)
     PITON_REQUIRE(a->scale_type >= PITON_B200_TYPE_F32 && a->scale_type <= PITON_B200_TYPE_BF16, "unknown scale type %d",
                   a->scale_type);
     PITON_REQUIRE(a->rows >= 0 && a->inner >= 0 && a->outer >= 0, "bad shape");
-    PITON_REQUIRE(a->rows <= 65535 && a->outer < (1ll << 31) && a->inner < (1ll << 31), "rows, inner or outer too large");
+    PITON_REQUIRE(a->rows <= 65535 && a->outer < (1ll << 31) && a->inner <= (1ll << 30), "rows, inner or outer too large");
     if (a->group != 32 && a->group != 64 && a->group != 128)
         return set_error(PITON_B200_ENOTSUP, "group %d (32, 64, 128)", a->group);
     if (a->rows == 0 || a->outer == 0) return PITON_B200_OK;
@@ -263,10 +508,12 @@ extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream)
     p.zeros = reinterpret_cast<const uint8_t *>(a->zeros);
     p.bias = reinterpret_cast<const void *>(a->bias);
     p.y = reinterpret_cast<void *>(a->y);
-    p.rows = a->rows; p.inner = a->inner; p.outer = a->outer;
+    p.rows = a->rows; p.inner = (int32_t)a->inner; p.outer = a->outer;
     p.sx = a->stride_x; p.sc = a->stride_codes; p.ss = a->stride_scales; p.sz = a->stride_zeros; p.sy = a->stride_y;
     p.group_log2 = a->group == 32 ? 5 : a->group == 64 ? 6 : 7; p.scale_type = a->scale_type;
-    p.aligned = a->codes % 16 == 0 && a->stride_codes % 16 == 0;
+    const uint64_t where = a->codes | (a->outer == 1 ? 0 : (uint64_t)a->stride_codes);   // the rows' alignment
+    p.codes_align = where % 16 == 0 ? 16 : where % 4 == 0 ? 4 : 1;
+    p.x_aligned = a->x % 16 == 0 && (a->rows == 1 || a->stride_x * (a->type == PITON_B200_TYPE_F32 ? 4 : 2) % 16 == 0);
     return with_type(a->type, [&](auto t) {
         using T = decltype(t);
         cudaStream_t s = as_stream(stream);
