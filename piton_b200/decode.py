@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -53,12 +54,41 @@ class PagedKV(NamedTuple):
         return cls(*codes, *scales)
 
 
-def _type_of(name: str, t) -> int:
-    try:
-        return _TYPES[t.dtype]
-    except (KeyError, AttributeError):
-        raise TypeError(f"{name}: expected a float32, float16 or bfloat16 CUDA tensor, got "
-                        f"{getattr(t, 'dtype', type(t).__name__)}") from None
+# A decode step makes these calls every few microseconds, so the ordinary call evaluates one condition
+# over everything it needs and packs the C struct with one format; only where the condition fails are
+# the arguments looked at one by one (the _refuse_* functions), to say what is wrong.
+
+_LETTERS = {_lib.u64: "Q", _lib.i64: "q", _lib.i32: "i", _lib.u32: "I", _lib.f64: "d"}
+
+
+def _packer(struct_type):
+    """Packs the fields of a ctypes struct, in order, into bytes."""
+    s = struct.Struct("@" + "".join(_LETTERS[t] for _, t in struct_type._fields_))
+    assert s.size == C.sizeof(struct_type)
+    return s.pack
+
+
+_pack_append, _pack_attention, _pack_matvec = map(_packer, (_lib.KvAppendArgs, _lib.KvAttentionArgs, _lib.MatvecW4Args))
+_ENTRY = {}
+
+
+def _entry(name: str, restype=C.c_int, *rest):
+    """The library's function taking a packed struct."""
+    f = lib()[name]
+    f.restype, f.argtypes = restype, [C.c_char_p, *rest]
+    _ENTRY[name] = f
+    return f
+
+
+def _call(name: str, packed: bytes, index: int) -> None:
+    f = _ENTRY.get(name) or _entry(name, C.c_int, C.c_void_p)
+    if torch.cuda.current_device() == index:
+        rc = f(packed, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(packed, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name[len("piton_b200_"):])
 
 
 def _need(ok: bool, message: str) -> None:
@@ -66,62 +96,57 @@ def _need(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _rows(name: str, t, dtype, heads: Optional[int], dim: int, device):
-    """Shape and strides of a [tokens, heads, dim] operand with unit stride along dim."""
-    if t.dtype != dtype or t.device != device:
-        raise TypeError(f"{name}: expected {dtype} on {device}, got {t.dtype} on {t.device}")
+def _type_of(name: str, t) -> int:
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dtype not in _TYPES:
+        raise TypeError(f"{name}: expected a float32, float16 or bfloat16 CUDA tensor, got "
+                        f"{f'{t.dtype} on {t.device}' if isinstance(t, torch.Tensor) else type(t).__name__}")
+    return _TYPES[t.dtype]
+
+
+def _refuse_tensor(name: str, t, dtypes, index: int) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != index:
+        raise TypeError(f"{name}: expected {' or '.join(map(str, dtypes))} on cuda:{index}, got "
+                        f"{f'{t.dtype} on {t.device}' if isinstance(t, torch.Tensor) else type(t).__name__}")
+
+
+def _refuse_rows(name: str, t, dtype, heads, dim: int, index: int) -> None:
+    _refuse_tensor(name, t, (dtype,), index)
     _need(t.dim() == 3 and t.shape[2] == dim and (heads is None or t.shape[1] == heads),
           f"{name}: shape {tuple(t.shape)}, expected [tokens, {'heads' if heads is None else heads}, {dim}]")
-    st, sh, sd = t.stride()
-    _need(sd == 1, f"{name}: the last dimension must have unit stride")
-    return st, sh
+    _need(t.stride(2) == 1, f"{name}: the last dimension must have unit stride")
 
 
-def _int32(name: str, t, device, *shape):
-    """An int32 index tensor of this shape, unit stride in its last dimension."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device:
-        raise TypeError(f"{name}: expected an int32 tensor on {device}")
-    _need(t.shape == shape and (t.numel() <= 1 or t.stride(-1) == 1),
-          f"{name}: shape {tuple(t.shape)}, strides {t.stride()}, expected {list(shape)} with unit stride")
-    return t.data_ptr()
-
-
-def _cache(cache, device):
+def _refuse_cache(cache, index: int) -> None:
     k, v, ks, vs = cache
-    shape = k.shape
-    if k.dtype not in _CODES or v.dtype not in _CODES or ks.dtype != torch.float32 or vs.dtype != torch.float32:
-        raise TypeError("cache: expected float8_e4m3fn (or uint8) codes and float32 scales")
-    if k.device != device or v.device != device or ks.device != device or vs.device != device:
-        raise TypeError(f"cache: every tensor must be on {device}")
-    _need(len(shape) == 4 and v.shape == shape, "cache: codes must be [pages, kv_heads, page_size, head_dim], k and v alike")
-    _need(ks.shape == shape[:2] and vs.shape == shape[:2], "cache: scales must be [pages, kv_heads]")
-    _need(k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous(),
-          "cache: tensors must be contiguous")
-    return shape, (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())
+    for name, t, dtypes in (("k", k, _CODES), ("v", v, _CODES), ("k_scale", ks, (torch.float32,)),
+                            ("v_scale", vs, (torch.float32,))):
+        _refuse_tensor(f"cache {name}", t, dtypes, index)
+        _need(t.is_contiguous(), f"cache {name}: must be contiguous")
+    _need(k.dim() == 4 and v.shape == k.shape, "cache: codes must be [pages, kv_heads, page_size, head_dim], k and v alike")
+    _need(ks.shape == k.shape[:2] and vs.shape == k.shape[:2], "cache: scales must be [pages, kv_heads]")
 
 
-def _table(table, device):
-    if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.device != device:
-        raise TypeError(f"table: expected an int32 tensor on {device}")
-    _need(table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1), "table: expected [batch, width], rows contiguous")
-    return table.shape[0], table.shape[1], table.stride(0)
+def _refuse_indices(table, vectors, cu, batch: int, tokens: int, index: int) -> None:
+    for name, t, size in vectors + ((("cu", cu, batch + 1),) if cu is not None else ()):
+        _refuse_tensor(name, t, (torch.int32,), index)
+        _need(t.dim() == 1 and t.shape[0] == size and t.is_contiguous(), f"{name}: expected {size} contiguous int32, got "
+              f"shape {tuple(t.shape)}, strides {t.stride()}")
+    _need(cu is not None or (tokens % batch == 0 if batch else tokens == 0),
+          f"{tokens} tokens are not the same number for each of {batch} sequences: pass cu")
 
 
-def _call(fname: str, args, device, what: str) -> None:
-    index = device.index
-    if torch.cuda.current_device() == index:
-        rc = getattr(lib(), fname)(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = getattr(lib(), fname)(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        check(rc, what)
+def _table(table, index: int):
+    """(batch, width, row stride) of a page table."""
+    if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.get_device() != index:
+        _refuse_tensor("table", table, (torch.int32,), index)
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table: expected [batch, width], rows contiguous")
+    batch, width = table.shape
+    return batch, width, table.stride(0)
 
 
-def _cuda_device(name: str, t):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
-        raise TypeError(f"{name}: expected a CUDA tensor")
-    return t.device
+def _same(t, dtype, index: int) -> bool:
+    return t.dtype is dtype and t.get_device() == index
 
 
 def kv_append(k, v, cache, table, starts, *, cu=None, cos=None, sin=None, interleaved: bool = False, q=None):
@@ -138,43 +163,59 @@ def kv_append(k, v, cache, table, starts, *, cu=None, cos=None, sin=None, interl
     A block (page and head) has one scale: the least power of two that holds its values within e4m3's 448;
     when new values make it grow, the block's older codes are requantised.  Non-finite values are stored
     as NaN and do not move the scale."""
-    device = _cuda_device("k", k)
     kind = _type_of("k", k)
-    shape, (kc, vc, ks, vs) = _cache(cache, device)
+    index, dtype = k.get_device(), k.dtype
+    kc, vc, ks, vs = cache
+    shape = kc.shape
+    if len(shape) != 4:
+        _refuse_cache(cache, index)
     pages, heads, page, dim = shape
-    skt, skh = _rows("k", k, k.dtype, heads, dim, device)
-    svt, svh = _rows("v", v, k.dtype, heads, dim, device)
+    batch, width, stride = _table(table, index)
     tokens = k.shape[0]
-    _need(v.shape[0] == tokens, f"k has {tokens} tokens, v {v.shape[0]}")
-    batch, width, stride = _table(table, device)
-    starts_at = _int32("starts", starts, device, batch)
-    cu_at = 0 if cu is None else _int32("cu", cu, device, batch + 1)
-    _need(cu is not None or (tokens % batch == 0 if batch else tokens == 0),
-          f"{tokens} tokens are not the same number for each of {batch} sequences: pass cu")
+    if not (k.dim() == 3 and k.shape == v.shape and k.shape[1] == heads and k.shape[2] == dim and v.dtype is dtype and
+            v.get_device() == index and k.stride(2) == 1 and v.stride(2) == 1 and
+            kc.dtype in _CODES and vc.dtype in _CODES and vc.shape == shape and ks.shape == shape[:2] == vs.shape and
+            _same(ks, torch.float32, index) and _same(vs, torch.float32, index) and kc.get_device() == index and
+            vc.get_device() == index and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and
+            vs.is_contiguous() and _same(starts, torch.int32, index) and starts.shape == (batch,) and
+            starts.is_contiguous() and
+            ((batch and tokens % batch == 0) if cu is None else
+             _same(cu, torch.int32, index) and cu.shape == (batch + 1,) and cu.is_contiguous())):
+        _refuse_rows("k", k, dtype, heads, dim, index)
+        _refuse_rows("v", v, dtype, heads, dim, index)
+        _need(v.shape[0] == tokens, f"k has {tokens} tokens, v {v.shape[0]}")
+        _refuse_cache(cache, index)
+        _refuse_indices(table, (("starts", starts, batch),), cu, batch, tokens, index)
     rot = rope_len = cos_at = sin_at = 0
-    _need((cos is None) == (sin is None), "pass both cos and sin, or neither")
-    if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            if t.dtype != torch.float32 or t.device != device:
-                raise TypeError(f"{name}: expected float32 on {device}")
-            _need(t.dim() == 2 and t.is_contiguous() and 2 * t.shape[1] <= dim and t.shape == cos.shape,
-                  f"{name}: expected a contiguous [positions, at most {dim // 2}]")
-        rope_len, rot = cos.shape[0], 2 * cos.shape[1]
+    if cos is not None or sin is not None:
+        _need(cos is not None and sin is not None, "pass both cos and sin, or neither")
+        if not (_same(cos, torch.float32, index) and _same(sin, torch.float32, index) and cos.dim() == 2 and
+                cos.shape == sin.shape and 2 * cos.shape[1] <= dim and cos.is_contiguous() and sin.is_contiguous()):
+            _refuse_tensor("cos", cos, (torch.float32,), index)
+            _refuse_tensor("sin", sin, (torch.float32,), index)
+            raise ValueError(f"cos, sin: expected two contiguous [positions, at most {dim // 2}], got {tuple(cos.shape)} and "
+                             f"{tuple(sin.shape)}")
+        rope_len, rot = cos.shape
+        rot *= 2
         cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
     q_heads = q_at = out_at = sqt = sqh = 0
     out = None
     if q is not None:
-        sqt, sqh = _rows("q", q, k.dtype, None, dim, device)
-        _need(q.shape[0] == tokens, f"k has {tokens} tokens, q {q.shape[0]}")
+        if not (_same(q, dtype, index) and q.dim() == 3 and q.shape[2] == dim and q.shape[0] == tokens and q.stride(2) == 1):
+            _refuse_rows("q", q, dtype, None, dim, index)
+            raise ValueError(f"k has {tokens} tokens, q {q.shape[0]}")
         q_heads = q.shape[1]
-        out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=device)
+        sqt, sqh, _ = q.stride()
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         q_at, out_at = q.data_ptr(), out.data_ptr()
-    lengths = torch.empty(batch, dtype=torch.int32, device=device)
-    a = _lib.KvAppendArgs(k.data_ptr(), v.data_ptr(), q_at, out_at, kc, vc, ks, vs, table.data_ptr(), starts_at, cu_at,
-                          lengths.data_ptr(), cos_at, sin_at, batch, tokens, heads, q_heads, dim, page, pages, width,
-                          stride, skt, skh, svt, svh, sqt, sqh, q_heads * dim, dim, rot, rope_len, kind,
-                          1 if interleaved else 0, 0, 0)
-    _call("piton_b200_kv_append", a, device, "kv_append")
+    lengths = torch.empty_like(starts)
+    skt, skh, _ = k.stride()
+    svt, svh, _ = v.stride()
+    _call("piton_b200_kv_append",
+          _pack_append(k.data_ptr(), v.data_ptr(), q_at, out_at, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+                       table.data_ptr(), starts.data_ptr(), 0 if cu is None else cu.data_ptr(), lengths.data_ptr(), cos_at,
+                       sin_at, batch, tokens, heads, q_heads, dim, page, pages, width, stride, skt, skh, svt, svh, sqt, sqh,
+                       q_heads * dim, dim, rot, rope_len, kind, 1 if interleaved else 0, 0, 0), index)
     return out, lengths
 
 
@@ -189,29 +230,41 @@ def kv_attention(q, cache, table, lengths, *, cu=None, scale: Optional[float] = 
     lengths known to the host) and ``max_new`` (of the query tokens a sequence, with ``cu``) size the launch;
     by default the table's width and the number of tokens bound them.  With ``return_lse`` also the float32
     [tokens, heads] logarithms of the rows' sums of exponentials (-inf for rows that see no key)."""
-    device = _cuda_device("q", q)
     kind = _type_of("q", q)
-    shape, (kc, vc, ks, vs) = _cache(cache, device)
+    index = q.get_device()
+    kc, vc, ks, vs = cache
+    shape = kc.shape
+    if len(shape) != 4:
+        _refuse_cache(cache, index)
     pages, kv_heads, page, dim = shape
-    sqt, sqh = _rows("q", q, q.dtype, None, dim, device)
-    tokens, heads = q.shape[0], q.shape[1]
-    batch, width, stride = _table(table, device)
-    lengths_at = _int32("lengths", lengths, device, batch)
-    cu_at = 0 if cu is None else _int32("cu", cu, device, batch + 1)
-    _need(cu is not None or (tokens % batch == 0 if batch else tokens == 0),
-          f"{tokens} tokens are not the same number for each of {batch} sequences: pass cu")
-    _need(window >= 0 and max_length >= 0 and max_new >= 0, "window, max_length and max_new must not be negative")
-    out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=device)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
-    a = _lib.KvAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, kc, vc, ks, vs,
-                             table.data_ptr(), lengths_at, cu_at, 1.0 / math.sqrt(dim) if scale is None else scale,
-                             batch, tokens, heads, kv_heads, dim, page, pages, width, stride, sqt, sqh, heads * dim, dim,
-                             window, max_length, max_new, 0, 0, kind, 0)
-    need = lib().piton_b200_kv_attention_workspace_size(C.byref(a))
+    batch, width, stride = _table(table, index)
+    if not (q.dim() == 3 and q.shape[2] == dim and q.stride(2) == 1 and
+            kc.dtype in _CODES and vc.dtype in _CODES and vc.shape == shape and ks.shape == shape[:2] == vs.shape and
+            _same(ks, torch.float32, index) and _same(vs, torch.float32, index) and kc.get_device() == index and
+            vc.get_device() == index and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and
+            vs.is_contiguous() and _same(lengths, torch.int32, index) and lengths.shape == (batch,) and
+            lengths.is_contiguous() and window >= 0 and max_length >= 0 and max_new >= 0 and
+            ((batch and q.shape[0] % batch == 0) if cu is None else
+             _same(cu, torch.int32, index) and cu.shape == (batch + 1,) and cu.is_contiguous())):
+        _refuse_rows("q", q, q.dtype, None, dim, index)
+        _refuse_cache(cache, index)
+        _refuse_indices(table, (("lengths", lengths, batch),), cu, batch, q.shape[0], index)
+        _need(window >= 0 and max_length >= 0 and max_new >= 0, "window, max_length and max_new must not be negative")
+    tokens, heads, _ = q.shape
+    sqt, sqh, _ = q.stride()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    args = (q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(),
+            vs.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0 if cu is None else cu.data_ptr(),
+            dim ** -0.5 if scale is None else scale, batch, tokens, heads, kv_heads, dim, page, pages, width, stride, sqt, sqh,
+            heads * dim, dim, window, max_length, max_new)
+    packed = _pack_attention(*args, 0, 0, kind, 0)
+    need = (_ENTRY.get("piton_b200_kv_attention_workspace_size") or
+            _entry("piton_b200_kv_attention_workspace_size", C.c_size_t))(packed)
     if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=device)   # of this call's stream, so calls never share it
-        a.workspace, a.workspace_bytes = scratch.data_ptr(), need
-    _call("piton_b200_kv_attention", a, device, "kv_attention")
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)   # of this call's stream, so calls never share it
+        packed = _pack_attention(*args, scratch.data_ptr(), need, kind, 0)
+    _call("piton_b200_kv_attention", packed, index)
     return (out, lse) if return_lse else out
 
 
@@ -223,42 +276,43 @@ def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
     the same shape, the low four bits count; zero point 8 without) per group of 32, 64 or 128: W = scale * (code - zero).  ``bias``
     [outer] of x's type.  Rows of every operand may be strided.  Accumulates in 32 bits, returns x's type.
     Meant for few rows: the weights are read again for every 16."""
-    device = _cuda_device("x", x)
     kind = _type_of("x", x)
+    index, dtype = x.get_device(), x.dtype
     flat = x.dim() == 1
-    _need(x.dim() in (1, 2), f"x: shape {tuple(x.shape)}, expected [rows, inner] or [inner]")
-    rows, inner = (1, x.shape[0]) if flat else x.shape
-    _need(x.shape[-1] <= 1 or x.stride(-1) == 1, "x: the last dimension must have unit stride")
-    if codes.dtype != torch.uint8 or codes.device != device:
-        raise TypeError(f"codes: expected uint8 on {device}, got {codes.dtype} on {codes.device}")
-    _need(codes.dim() == 2 and codes.shape[1] == (inner + 1) // 2 and (codes.shape[1] <= 1 or codes.stride(1) == 1),
-          f"codes: shape {tuple(codes.shape)}, expected [outer, {(inner + 1) // 2}] with unit stride")
-    outer = codes.shape[0]
+    if x.dim() not in (1, 2):
+        raise ValueError(f"x: shape {tuple(x.shape)}, expected [rows, inner] or [inner]")
+    inner = x.shape[-1]
     if group not in (32, 64, 128):
         raise NotImplementedError(f"group {group}: 32, 64 or 128")
-    groups = -(-inner // group)
-    scale_kind = _type_of("scales", scales)
-    if scales.device != device:
-        raise TypeError(f"scales: expected a tensor on {device}")
-    _need(scales.shape == (outer, groups) and (groups <= 1 or scales.stride(1) == 1),
-          f"scales: shape {tuple(scales.shape)}, expected {[outer, groups]} with unit stride")
-    zeros_at = bias_at = zero_stride = 0
-    if zeros is not None:
-        if zeros.dtype != torch.uint8 or zeros.device != device:
-            raise TypeError(f"zeros: expected uint8 on {device}")
-        _need(zeros.shape == (outer, groups) and (groups <= 1 or zeros.stride(1) == 1),
-              f"zeros: shape {tuple(zeros.shape)}, expected {[outer, groups]} with unit stride")
-        zeros_at, zero_stride = zeros.data_ptr(), zeros.stride(0)
-    if bias is not None:
-        if bias.dtype != x.dtype or bias.device != device:
-            raise TypeError(f"bias: expected {x.dtype} on {device}")
-        _need(bias.shape == (outer,) and (outer <= 1 or bias.stride(0) == 1), f"bias: expected [{outer}] with unit stride")
-        bias_at = bias.data_ptr()
-    y = torch.empty(outer if flat else (rows, outer), dtype=x.dtype, device=device)
-    a = _lib.MatvecW4Args(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), zeros_at, bias_at, y.data_ptr(), rows, inner,
-                          outer, 0 if flat else x.stride(0), codes.stride(0), scales.stride(0), zero_stride, outer, group,
-                          kind, scale_kind, 0)
-    _call("piton_b200_matvec_w4", a, device, "matvec_w4")
+    if not isinstance(codes, torch.Tensor) or codes.dim() != 2:
+        _refuse_tensor("codes", codes, (torch.uint8,), index)
+        raise ValueError(f"codes: shape {tuple(codes.shape)}, expected [outer, {(inner + 1) // 2}]")
+    outer, groups = codes.shape[0], -(-inner // group)
+    shape = (outer, groups)
+    if not (_same(codes, torch.uint8, index) and codes.shape[1] == (inner + 1) // 2 and
+            (codes.stride(1) == 1 or codes.shape[1] <= 1) and (x.stride(-1) == 1 or inner <= 1) and
+            scales.dtype in _TYPES and scales.get_device() == index and scales.shape == shape and
+            (groups <= 1 or scales.stride(1) == 1) and
+            (zeros is None or (_same(zeros, torch.uint8, index) and zeros.shape == shape and
+                               (groups <= 1 or zeros.stride(1) == 1))) and
+            (bias is None or (_same(bias, dtype, index) and bias.shape == (outer,) and (outer <= 1 or bias.stride(0) == 1)))):
+        _refuse_tensor("codes", codes, (torch.uint8,), index)
+        _refuse_tensor("scales", scales, tuple(_TYPES), index)
+        if zeros is not None:
+            _refuse_tensor("zeros", zeros, (torch.uint8,), index)
+        if bias is not None:
+            _refuse_tensor("bias", bias, (dtype,), index)
+        raise ValueError(f"x {tuple(x.shape)}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}, zeros "
+                         f"{None if zeros is None else tuple(zeros.shape)}, bias {None if bias is None else tuple(bias.shape)}: "
+                         f"expected codes [{outer}, {(inner + 1) // 2}], scales and zeros {list(shape)}, bias [{outer}], each with "
+                         f"unit stride in its last dimension")
+    rows = 1 if flat else x.shape[0]
+    y = x.new_empty(outer if flat else (rows, outer))
+    _call("piton_b200_matvec_w4",
+          _pack_matvec(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+                       0 if bias is None else bias.data_ptr(), y.data_ptr(), rows, inner, outer, 0 if flat else x.stride(0),
+                       codes.stride(0), scales.stride(0), 0 if zeros is None else zeros.stride(0), outer, group, kind,
+                       _TYPES[scales.dtype], 0), index)
     return y
 
 
