@@ -1,11 +1,15 @@
 // Appending to a paged 8-bit cache: keys rotated by position, keys and values quantised to e4m3
 // with a power-of-two scale per (page, head), queries rotated in the same launch.
 //
-// A unit is one page that one sequence's new tokens touch; a CTA takes one (unit, head, key or
-// value): the block's largest finite magnitude, its scale, the older tokens requantised where the
-// scale grows, the new tokens' codes.  The scale is a power of two, so dividing by it is exact and a
+// A unit is one page that one sequence's new tokens touch; a task is one (unit, head, key or value):
+// the block's largest finite magnitude, its scale, the older tokens requantised where the scale
+// grows, the new tokens' codes.  The scale is a power of two, so dividing by it is exact and a
 // growing scale moves old codes without a second rounding until they reach e4m3's subnormals; the
 // format's relative precision does not depend on where in a binade the scale sits.
+//
+// The bytes in and out bound it.  Every element is read once, 16 bytes at a time: a thread takes a pair of
+// 16-byte pieces whose elements rotate with one another, keeps the rotated values in registers until the
+// block's scale is known, and reads its rows of the rotation tables once for all heads that it walks.
 #include "decode.cuh"
 
 namespace piton {
@@ -168,6 +172,309 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendParams p
     if (tid == 0) *scale = s;
 }
 
+
+// ---- rows on 16 bytes ----
+
+// V = 16 / sizeof(T) elements a piece; pair u of a head's dim / (2 V): pieces at V u and rot / 2 + V u where they rotate in
+// halves, else two neighbouring pieces from 2 V u on (interleaved pairs, or past rot).
+template <typename T> struct Pair {
+    static constexpr int V = 16 / sizeof(T);
+    float a[V], b[V];
+};
+struct PairPlace {
+    int a, b;              // element offsets in the head
+    bool turns, inside;    // rotates; with pairs inside a piece
+};
+template <typename T> __device__ __forceinline__ PairPlace place_of(int u, int rot, bool interleaved) {
+    constexpr int V = 16 / sizeof(T);
+    const bool turns = 2 * V * u < rot, halves = turns && !interleaved;
+    return {halves ? V * u : 2 * V * u, halves ? (rot >> 1) + V * u : 2 * V * u + V, turns, interleaved};
+}
+__device__ __forceinline__ void unpack(float (&f)[4], const uint4 &r, float) {
+    f[0] = __uint_as_float(r.x), f[1] = __uint_as_float(r.y), f[2] = __uint_as_float(r.z), f[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void unpack(float (&f)[8], const uint4 &r, __half) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        f[2 * i] = x.x, f[2 * i + 1] = x.y;
+    }
+}
+__device__ __forceinline__ void unpack(float (&f)[8], const uint4 &r, __nv_bfloat16) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+}
+template <typename T> __device__ __forceinline__ uint4 packed(const float (&f)[16 / sizeof(T)]) {
+    T v[16 / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) v[i] = from_float<T>(f[i]);
+    return *reinterpret_cast<const uint4 *>(v);
+}
+__device__ __forceinline__ uint4 load_stream(const void *p) { return __ldcs(reinterpret_cast<const uint4 *>(p)); }
+
+// Rotates a pair by its row of the tables (c, s: V values from element V u of the row).
+template <typename T> __device__ __forceinline__ void turn(Pair<T> &x, const float (&c)[Pair<T>::V], const float (&s)[Pair<T>::V], const PairPlace &at) {
+    constexpr int V = Pair<T>::V;
+    if (!at.turns) return;
+    if (at.inside) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float a0 = x.a[i], a1 = x.a[i + 1], b0 = x.b[i], b1 = x.b[i + 1];
+            x.a[i] = __fsub_rn(__fmul_rn(a0, c[i / 2]), __fmul_rn(a1, s[i / 2]));
+            x.a[i + 1] = __fadd_rn(__fmul_rn(a1, c[i / 2]), __fmul_rn(a0, s[i / 2]));
+            x.b[i] = __fsub_rn(__fmul_rn(b0, c[(V + i) / 2]), __fmul_rn(b1, s[(V + i) / 2]));
+            x.b[i + 1] = __fadd_rn(__fmul_rn(b1, c[(V + i) / 2]), __fmul_rn(b0, s[(V + i) / 2]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float a = x.a[i], b = x.b[i];
+            x.a[i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+            x.b[i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
+        }
+    }
+}
+template <int V> __device__ __forceinline__ void load_row(float (&f)[V], const float *p) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        const float4 r = __ldg(reinterpret_cast<const float4 *>(p + i));
+        f[i] = r.x, f[i + 1] = r.y, f[i + 2] = r.z, f[i + 3] = r.w;
+    }
+}
+template <int V> __device__ __forceinline__ void store_codes(uint8_t *to, const float (&f)[V], float inv) {
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+        float2 y = make_float2(f[i] * inv, f[i + 1] * inv);
+        y.x = isfinite(f[i]) ? y.x : __int_as_float(0x7FC00000);
+        y.y = isfinite(f[i + 1]) ? y.y : __int_as_float(0x7FC00000);
+        const uint32_t two = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+        if (i % 4 == 0) w[i / 4] = two;
+        else w[i / 4] |= two << 16;
+    }
+    if constexpr (V == 4) *reinterpret_cast<uint32_t *>(to) = w[0];
+    else *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+}
+
+constexpr int WIDE = 256;      // threads of a CTA
+
+// A task by TT threads (a warp or the CTA), at most PASSES pairs a thread; the CTA's tasks are `heads_each` heads of one unit,
+// one after the other (TT = WIDE) or WIDE / 32 of the list, a warp each.
+template <typename T, int D, int TT, int PASSES>
+__global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASSES == 4 ? 2 : 1) kv_append_wide_kernel(const AppendParams p, int heads_each, int q_pieces) {
+    constexpr int V = 16 / sizeof(T), UPH = D / (2 * V);             // pairs of a head
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (blockIdx.x >= p.unit_blocks) {                               // queries: a warp per token and piece of the heads
+        const int64_t item = ((int64_t)blockIdx.x - p.unit_blocks) * (WIDE / 32) + (tid >> 5);
+        const int64_t t = item / q_pieces;
+        if (t >= p.tokens) return;
+        const int64_t b = sequence_of_token(p, t);
+        const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
+        const int64_t pos = (int64_t)p.starts[b] + t - sp.t0;
+        if (p.rot != 0 && (pos < 0 || pos >= p.rope_len || t < sp.t0 || t >= sp.t0 + sp.n)) {
+            if (lane == 0) record_status(STATUS_BAD_POSITION);
+            return;
+        }
+        constexpr int SIDE = 32 / UPH;                               // heads at once
+        const int u = lane % UPH;
+        const PairPlace at = place_of<T>(u, p.rot, p.interleaved);
+        float c[V], s[V];
+        if (at.turns) {
+            load_row(c, p.cos_table + pos * (p.rot >> 1) + V * u);
+            load_row(s, p.sin_table + pos * (p.rot >> 1) + V * u);
+        }
+        const T *x = reinterpret_cast<const T *>(p.q) + t * p.sqt;
+        T *y = reinterpret_cast<T *>(p.q_out) + t * p.sot;
+        const int heads = (int)p.q_heads, step = SIDE * q_pieces;
+        int h = (int)(item % q_pieces) * SIDE + lane / UPH;
+        for (; h < heads; h += 2 * step) {                           // two heads in flight
+            const bool more = h + step < heads;
+            const T *x0 = x + h * p.sqh, *x1 = x + (int64_t)(h + step) * p.sqh;
+            const uint4 a0 = load_stream(x0 + at.a), b0 = load_stream(x0 + at.b);
+            uint4 a1 = {}, b1 = {};
+            if (more) a1 = load_stream(x1 + at.a), b1 = load_stream(x1 + at.b);
+            Pair<T> v;
+            unpack(v.a, a0, T());
+            unpack(v.b, b0, T());
+            turn<T>(v, c, s, at);
+            T *y0 = y + h * p.soh, *y1 = y + (int64_t)(h + step) * p.soh;
+            *reinterpret_cast<uint4 *>(y0 + at.a) = packed<T>(v.a);
+            *reinterpret_cast<uint4 *>(y0 + at.b) = packed<T>(v.b);
+            if (more) {
+                unpack(v.a, a1, T());
+                unpack(v.b, b1, T());
+                turn<T>(v, c, s, at);
+                *reinterpret_cast<uint4 *>(y1 + at.a) = packed<T>(v.a);
+                *reinterpret_cast<uint4 *>(y1 + at.b) = packed<T>(v.b);
+            }
+        }
+        return;
+    }
+    const int worker = tid % TT;
+    const int pieces = (int)((p.kv_heads + heads_each - 1) / heads_each);    // of a unit's heads, keys and values apart
+    const int64_t task = TT == WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (WIDE / TT) + tid / TT;
+    const int64_t unit = task / (2 * pieces);
+    if (unit >= p.units) return;
+    const int which = (int)(task % (2 * pieces)) & 1, head0 = ((int)(task % (2 * pieces)) >> 1) * heads_each;
+    int64_t b, j;
+    if (!p.cu) {
+        const int64_t each = p.units / p.batch;
+        b = unit / each;
+        j = unit % each;
+    } else {
+        int64_t lo = 0, hi = p.batch - 1;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) >> 1;
+            if (first_unit(p, mid) <= unit) lo = mid;
+            else hi = mid - 1;
+        }
+        b = lo;
+        j = unit - first_unit(p, b);
+    }
+    const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
+    const int64_t start = p.starts[b], end = start + sp.n;
+    if (j == 0 && head0 == 0 && which == 0 && worker == 0 && p.lengths) p.lengths[b] = (int32_t)end;
+    if (start < 0) {
+        if (worker == 0) record_status(STATUS_BAD_POSITION);
+        return;
+    }
+    const int64_t place = start / p.page_size + j, page0 = place * p.page_size;
+    const int64_t lo = max(start, page0), hi = min(end, page0 + p.page_size);
+    if (lo >= hi) return;
+    if (place >= p.table_width || (which == 0 && p.rot && hi > p.rope_len)) {
+        if (worker == 0) record_status(STATUS_BAD_POSITION);
+        return;
+    }
+    const int64_t page = p.table[b * p.table_stride + place];
+    if (page < 0 || page >= p.num_pages) {
+        if (worker == 0) record_status(STATUS_BAD_PAGE);
+        return;
+    }
+    const int rot = which == 0 ? p.rot : 0, count = (int)(hi - lo), held = (int)(lo - page0), u = worker % UPH;
+    const PairPlace at = place_of<T>(u, rot, p.interleaved);
+    constexpr int TOKENS = TT / UPH;                                 // a pass
+    const int token = worker / UPH;
+    const int64_t st = p.st[which], sh = p.sh[which];
+    const T *x = reinterpret_cast<const T *>(which == 0 ? p.k : p.v) + (sp.t0 + lo - start + token) * st;
+    const float *c_row = p.cos_table + (lo + token) * (rot >> 1) + V * u, *s_row = p.sin_table + (lo + token) * (rot >> 1) + V * u;
+    __shared__ float red[2][WIDE / 32];
+    uint4 raw[PASSES][2];
+    auto load = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+            if (i * TOKENS + token < count) {
+                raw[i][0] = load_stream(x + i * TOKENS * st + h * sh + at.a);
+                raw[i][1] = load_stream(x + i * TOKENS * st + h * sh + at.b);
+            }
+    };
+    load(head0);
+    const int head1 = min(head0 + heads_each, (int)p.kv_heads);
+#pragma unroll 1
+    for (int h = head0; h < head1; ++h) {
+        Pair<T> v[PASSES];
+        float a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+            if (i * TOKENS + token < count) {
+                unpack(v[i].a, raw[i][0], T());
+                unpack(v[i].b, raw[i][1], T());
+                if (at.turns) {                                      // the rows stay in L1 from head to head
+                    float c[V], s[V];
+                    load_row(c, c_row + i * TOKENS * (rot >> 1));
+                    load_row(s, s_row + i * TOKENS * (rot >> 1));
+                    turn<T>(v[i], c, s, at);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) a = fmaxf(a, fmaxf(finite_abs(v[i].a[e]), finite_abs(v[i].b[e])));
+            }
+        if (h + 1 < head1) load(h + 1);
+        uint8_t *codes = p.codes[which] + (page * p.kv_heads + h) * p.page_size * D;
+        float *scale = p.scale[which] + page * p.kv_heads + h;
+        const float before = held ? *scale : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        if constexpr (TT > 32) {
+            float *r = red[(h - head0) & 1];                         // the other one may still be read for the last head
+            if (lane == 0) r[tid >> 5] = a;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WIDE / 32; ++w) a = fmaxf(a, r[w]);
+        }
+        const float s = fmaxf(block_scale(a), before);
+        const float inv = 1.0f / s;                                  // a power of two: exact
+        if (held && s > before) {
+            const float ratio = before * inv;
+            for (int i = worker * 4; i < held * D; i += TT * 4) {
+                uchar4 old = *reinterpret_cast<const uchar4 *>(codes + i);
+                old.x = float_to_e4m3(e4m3_to_float(old.x) * ratio), old.y = float_to_e4m3(e4m3_to_float(old.y) * ratio);
+                old.z = float_to_e4m3(e4m3_to_float(old.z) * ratio), old.w = float_to_e4m3(e4m3_to_float(old.w) * ratio);
+                *reinterpret_cast<uchar4 *>(codes + i) = old;
+            }
+        }
+        codes += (held + token) * D;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+            if (i * TOKENS + token < count) {
+                store_codes(codes + i * TOKENS * D + at.a, v[i].a, inv);
+                store_codes(codes + i * TOKENS * D + at.b, v[i].b, inv);
+            }
+        if constexpr (TT > 32) {
+            if (tid == 0) *scale = s;
+        } else {
+            __syncwarp();                                            // every lane has read the old scale
+            if (lane == 0) *scale = s;
+        }
+    }
+}
+
+// Whether rows can be read and written 16 bytes at a time, in pairs of pieces that rotate with one another.
+bool wide_enough(const piton_kv_append_args *a, int size) {
+    const int64_t v = 16 / size;
+    if (a->rot_dim % (2 * v)) return false;
+    uint64_t bits = a->k | a->v;
+    for (int64_t s : {a->stride_kt, a->stride_kh, a->stride_vt, a->stride_vh}) bits |= (uint64_t)s * size;
+    if (a->q_heads) {
+        bits |= a->q | a->q_out;
+        for (int64_t s : {a->stride_qt, a->stride_qh, a->stride_ot, a->stride_oh}) bits |= (uint64_t)s * size;
+    }
+    if (a->rot_dim) bits |= a->cos_table | a->sin_table;
+    return bits % 16 == 0;
+}
+
+template <typename T, int D, int TT, int PASSES> int launch_wide(AppendParams p, cudaStream_t s) {
+    constexpr int UPH = D / (2 * (16 / (int)sizeof(T))), SIDE = 32 / UPH;
+    const int64_t sms = num_sms();
+    // a CTA walks up to 4 heads, while that leaves four CTAs an SM
+    int64_t heads_each = 1;
+    if (TT == WIDE) {
+        heads_each = p.units * 2 * p.kv_heads / (4 * sms);
+        heads_each = heads_each < 1 ? 1 : heads_each > 4 ? 4 : heads_each;
+    }
+    const int64_t tasks = p.units * 2 * cdiv(p.kv_heads, heads_each);
+    p.unit_blocks = cdiv(tasks, WIDE / TT);
+    // a warp walks a token's query heads, in pieces while there are not 32 warps an SM
+    int64_t q_pieces = 1;
+    while (q_pieces * SIDE < p.q_heads && p.tokens * q_pieces < 32 * sms) q_pieces *= 2;
+    const int64_t blocks = p.unit_blocks + (p.q_heads ? cdiv(p.tokens * q_pieces, WIDE / 32) : 0);
+    PITON_REQUIRE(blocks < (1ll << 31), "too many blocks: %lld", (long long)blocks);
+    kv_append_wide_kernel<T, D, TT, PASSES><<<(unsigned)blocks, WIDE, 0, s>>>(p, (int)heads_each, (int)q_pieces);
+    return check_launch("kv_append");
+}
+
+template <typename T, int D> int launch_wide(const AppendParams &p, cudaStream_t s) {
+    constexpr int UPH = D / (2 * (16 / (int)sizeof(T)));
+    // pairs of a task at most: what a warp's four passes hold is a warp's, more is a CTA's
+    const int64_t most = (p.cu || p.uniform > p.page_size ? p.page_size : p.uniform) * UPH;
+    if (most <= 32) return launch_wide<T, D, 32, 1>(p, s);
+    if (most <= 128) return launch_wide<T, D, 32, 4>(p, s);
+    if (most <= WIDE) return launch_wide<T, D, WIDE, 1>(p, s);
+    if (most <= 2 * WIDE) return launch_wide<T, D, WIDE, 2>(p, s);
+    if (most <= 4 * WIDE) return launch_wide<T, D, WIDE, 4>(p, s);
+    return launch_wide<T, D, WIDE, 8>(p, s);
+}
+
 }  // namespace
 
 int kv_append_status_read_and_clear(int *status) {
@@ -235,6 +542,12 @@ extern "C" int piton_b200_kv_append(const piton_kv_append_args *a, void *stream)
     p.unit_blocks = p.units * 2 * a->kv_heads;
     const int64_t blocks = p.unit_blocks + cdiv(a->tokens * a->q_heads, THREADS / 32);
     PITON_REQUIRE(blocks < (1ll << 31), "too many blocks: %lld", (long long)blocks);
+    if (wide_enough(a, a->type == PITON_B200_TYPE_F32 ? 4 : 2))
+        return with_type(a->type, [&](auto t) {
+            using T = decltype(t);
+            cudaStream_t q = as_stream(stream);
+            return p.dim == 32 ? launch_wide<T, 32>(p, q) : p.dim == 64 ? launch_wide<T, 64>(p, q) : launch_wide<T, 128>(p, q);
+        });
     return with_type(a->type, [&](auto t) {
         kv_append_kernel<decltype(t)><<<(unsigned)blocks, THREADS, 0, as_stream(stream)>>>(p);
         return check_launch("kv_append");
