@@ -206,11 +206,32 @@ __device__ __forceinline__ void unpack(float (&f)[8], const uint4 &r, __nv_bfloa
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
 }
-template <typename T> __device__ __forceinline__ uint4 packed(const float (&f)[16 / sizeof(T)]) {
-    T v[16 / sizeof(T)];
+__device__ __forceinline__ uint4 packed(const float (&f)[4], float) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 packed(const float (&f)[8], __half) {
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 16 / (int)sizeof(T); ++i) v[i] = from_float<T>(f[i]);
-    return *reinterpret_cast<const uint4 *>(v);
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 packed(const float (&f)[8], __nv_bfloat16) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The larger magnitude; NaN if one is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+    return d;
 }
 __device__ __forceinline__ uint4 load_stream(const void *p) { return __ldcs(reinterpret_cast<const uint4 *>(p)); }
 
@@ -243,13 +264,15 @@ template <int V> __device__ __forceinline__ void load_row(float (&f)[V], const f
         f[i] = r.x, f[i + 1] = r.y, f[i + 2] = r.z, f[i + 3] = r.w;
     }
 }
-template <int V> __device__ __forceinline__ void store_codes(uint8_t *to, const float (&f)[V], float inv) {
+template <int V> __device__ __forceinline__ void store_codes(uint8_t *to, const float (&f)[V], float inv, bool all_finite) {
     uint32_t w[V / 4];
 #pragma unroll
     for (int i = 0; i < V; i += 2) {
         float2 y = make_float2(f[i] * inv, f[i + 1] * inv);
-        y.x = isfinite(f[i]) ? y.x : __int_as_float(0x7FC00000);
-        y.y = isfinite(f[i + 1]) ? y.y : __int_as_float(0x7FC00000);
+        if (!all_finite) {
+            y.x = isfinite(f[i]) ? y.x : __int_as_float(0x7FC00000);
+            y.y = isfinite(f[i + 1]) ? y.y : __int_as_float(0x7FC00000);
+        }
         const uint32_t two = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
         if (i % 4 == 0) w[i / 4] = two;
         else w[i / 4] |= two << 16;
@@ -300,14 +323,14 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
             unpack(v.b, b0, T());
             turn<T>(v, c, s, at);
             T *y0 = y + h * p.soh, *y1 = y + (int64_t)(h + step) * p.soh;
-            *reinterpret_cast<uint4 *>(y0 + at.a) = packed<T>(v.a);
-            *reinterpret_cast<uint4 *>(y0 + at.b) = packed<T>(v.b);
+            *reinterpret_cast<uint4 *>(y0 + at.a) = packed(v.a, T());
+            *reinterpret_cast<uint4 *>(y0 + at.b) = packed(v.b, T());
             if (more) {
                 unpack(v.a, a1, T());
                 unpack(v.b, b1, T());
                 turn<T>(v, c, s, at);
-                *reinterpret_cast<uint4 *>(y1 + at.a) = packed<T>(v.a);
-                *reinterpret_cast<uint4 *>(y1 + at.b) = packed<T>(v.b);
+                *reinterpret_cast<uint4 *>(y1 + at.a) = packed(v.a, T());
+                *reinterpret_cast<uint4 *>(y1 + at.b) = packed(v.b, T());
             }
         }
         return;
@@ -359,7 +382,7 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
     const int64_t st = p.st[which], sh = p.sh[which];
     const T *x = reinterpret_cast<const T *>(which == 0 ? p.k : p.v) + (sp.t0 + lo - start + token) * st;
     const float *c_row = p.cos_table + (lo + token) * (rot >> 1) + V * u, *s_row = p.sin_table + (lo + token) * (rot >> 1) + V * u;
-    __shared__ float red[2][WIDE / 32];
+    __shared__ float red[3][WIDE / 32];
     uint4 raw[PASSES][2];
     auto load = [&](int h) {
 #pragma unroll
@@ -387,20 +410,34 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
                     turn<T>(v[i], c, s, at);
                 }
 #pragma unroll
-                for (int e = 0; e < V; ++e) a = fmaxf(a, fmaxf(finite_abs(v[i].a[e]), finite_abs(v[i].b[e])));
+                for (int e = 0; e < V; ++e) a = max_abs(max_abs(a, v[i].a[e]), v[i].b[e]);
             }
         if (h + 1 < head1) load(h + 1);
         uint8_t *codes = p.codes[which] + (page * p.kv_heads + h) * p.page_size * D;
         float *scale = p.scale[which] + page * p.kv_heads + h;
         const float before = held ? *scale : 0.0f;
+        auto over_task = [&](float x, float *r) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        if constexpr (TT > 32) {
-            float *r = red[(h - head0) & 1];                         // the other one may still be read for the last head
-            if (lane == 0) r[tid >> 5] = a;
-            __syncthreads();
+            for (int o = 16; o > 0; o >>= 1) x = max_abs(x, __shfl_xor_sync(0xffffffffu, x, o));
+            if constexpr (TT > 32) {
+                if (lane == 0) r[tid >> 5] = x;
+                __syncthreads();
 #pragma unroll
-            for (int w = 0; w < WIDE / 32; ++w) a = fmaxf(a, r[w]);
+                for (int w = 0; w < WIDE / 32; ++w) x = max_abs(x, r[w]);
+            }
+            return x;
+        };
+        a = over_task(a, red[(h - head0) & 1]);                      // (the other one may still be read for the last head)
+        const bool all_finite = a < INFINITY;
+        if (!all_finite) {                                           // the scale is that of the finite values
+            a = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i)
+                if (i * TOKENS + token < count)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) a = fmaxf(a, fmaxf(finite_abs(v[i].a[e]), finite_abs(v[i].b[e])));
+            a = over_task(a, red[2]);
+            if constexpr (TT > 32) __syncthreads();                  // red[2] has been read
         }
         const float s = fmaxf(block_scale(a), before);
         const float inv = 1.0f / s;                                  // a power of two: exact
@@ -417,8 +454,8 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
 #pragma unroll
         for (int i = 0; i < PASSES; ++i)
             if (i * TOKENS + token < count) {
-                store_codes(codes + i * TOKENS * D + at.a, v[i].a, inv);
-                store_codes(codes + i * TOKENS * D + at.b, v[i].b, inv);
+                store_codes(codes + i * TOKENS * D + at.a, v[i].a, inv, all_finite);
+                store_codes(codes + i * TOKENS * D + at.b, v[i].b, inv, all_finite);
             }
         if constexpr (TT > 32) {
             if (tid == 0) *scale = s;
