@@ -26,7 +26,6 @@ __device__ int g_cached_status = 0;
 namespace {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int KEYS = 32;                 // keys of a stage: two 16-key tiles, each inside one page
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr uint32_t BAD_PAGE = 0x7FC0DEADu;   // in a stage's scale slot: the tile's page was not followed
 
@@ -50,12 +49,18 @@ template <int D> struct Geometry {
     static constexpr int KB = D >= 64 ? 16 : D / 4;     // bytes of a key row in one copy of a lane
     static constexpr int KC = D / (4 * KB);             // such copies per row
     static constexpr int VB = D / 8;                    // bytes of a value row that a lane takes
-    static constexpr int STAGES = 256 / D;              // 16 KB in flight a warp at every D
-    static constexpr int KBYTES = KEYS * D, STAGE_BYTES = 2 * KBYTES;
+    static constexpr int TILES = 256 / D, KEYS = 16 * TILES;  // of a stage: 16-key tiles, each inside one page; 8 KB at every D
+    static constexpr int STAGES = 2, KBYTES = KEYS * D, STAGE_BYTES = 2 * KBYTES;
     static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
-    static constexpr int SMEM = RING + WARPS * STAGES * 16;   // and four scales a stage: K, V of either tile
+    static constexpr int SCALES = 8 * TILES;            // bytes of a stage's K and V scales, tile by tile
+    static constexpr int SMEM = RING + WARPS * STAGES * SCALES;
+    static constexpr int RUN = 32 / TILES;              // stages whose page numbers the lanes hold at a time
 };
 
+template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
 template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool on) {
     const int size = on ? N : 0;                        // the rest of the N bytes is filled with zeros
     if constexpr (N == 16)
@@ -74,10 +79,15 @@ template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WO
     else
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
-// Two e4m3 codes (low and high byte) as two fp16 values: exact.
-__device__ __forceinline__ uint32_t halves(uint32_t two) {
+// Two e4m3 codes, bytes 0 and 1 (or 2 and 3) of a word, as two fp16 values: exact.
+__device__ __forceinline__ uint32_t halves(uint32_t word) {
     uint32_t d;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"((uint16_t)two));
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(word));
+    return d;
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t word) {
+    uint32_t d;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(d) : "r"(word));
     return d;
 }
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -117,9 +127,10 @@ template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(const CachedParams p) {
     using G = Geometry<D>;
     constexpr bool SPLIT = sizeof(T) == 4;              // fp32 rows: queries and weights as pairs of halves
-    constexpr int R = 8 * NQ, KW = G::KB / 4, VW = G::VB / 4, MT = D / 16, KT = D / 16;
+    constexpr int R = 8 * NQ, KW = G::KB / 4, VW = G::VB / 4, MT = D / 16, KT = D / 16, TILES = G::TILES, KEYS = G::KEYS;
     extern __shared__ __align__(16) uint8_t ring[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+    if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;");    // the join may take its place, and waits
     const int64_t b = blockIdx.z;
     const int kvh = blockIdx.y, tile = blockIdx.x % p.row_tiles, split = blockIdx.x / p.row_tiles;
     const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
@@ -147,43 +158,64 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
 
     // ---- this lane's copies ----
     const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * (G::STAGES * G::STAGE_BYTES);
-    const uint32_t scales0 = (uint32_t)__cvta_generic_to_shared(ring) + G::RING + warp * (G::STAGES * 16);
+    const uint32_t scales0 = (uint32_t)__cvta_generic_to_shared(ring) + G::RING + warp * (G::STAGES * G::SCALES);
     const int32_t page_mask = (1 << p.page_log2) - 1;
-    int32_t ids = -1, ids_next = -1;                    // pages of the 32 tiles of 16 stages, lane by lane
-    auto load_ids = [&](int s0) {                       // stages s0 .. s0 + 15
-        const int64_t key = mine + (int64_t)(s0 + (lane >> 1)) * (KEYS * WARPS) + 16 * (lane & 1);
+    const uint32_t k_slot = ring0 + lane * G::KB, v_slot = ring0 + G::KBYTES + lane * G::VB;
+    const uint8_t *k_lane = p.kc + g * D + j * G::KB, *v_lane = p.vc + 2 * j * D + g * G::VB;
+    int32_t ids = -1, ids_next = -1;                    // pages of the 32 tiles of RUN stages, lane by lane
+    uint32_t off_run = 0;                               // which of them are not to be read
+    auto load_ids = [&](int s0) {                       // stages s0 .. s0 + RUN - 1
+        const int64_t key = mine + (int64_t)(s0 + lane / TILES) * (KEYS * WARPS) + 16 * (lane % TILES);
         if (key >= stop || key + 15 < first_lo) return -1;
         const int32_t id = p.table[b * p.table_stride + (key >> p.page_log2)];
         if (id >= 0 && id < p.num_pages) return id;
         record_status(STATUS_BAD_PAGE);
         return -1;
     };
+    auto whole = [&](int64_t key0, int s) {             // every key of the stage exists
+        return key0 >= first_lo && key0 + KEYS <= stop && !(off_run >> (TILES * (s % G::RUN)) & ((1u << TILES) - 1));
+    };
+    auto offset_of = [&](int32_t id, int64_t key) {     // of a key's row in either array of codes
+        return (((int64_t)max(id, 0) * p.kv_heads + kvh << p.page_log2) + (key & page_mask)) * D;
+    };
     auto issue_k = [&](int s) {
         if (s < stages) {
-            if ((s & 15) == 0) {
+            if (s % G::RUN == 0) {
                 ids = s == 0 ? load_ids(0) : ids_next;
-                ids_next = load_ids(s + 16);
+                off_run = __ballot_sync(0xffffffffu, ids < 0);
+                ids_next = load_ids(s + G::RUN);
             }
             const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
-            const uint32_t at = ring0 + (s % G::STAGES) * G::STAGE_BYTES;
+            const uint32_t at = k_slot + (s % G::STAGES) * G::STAGE_BYTES;
+            const bool all = whole(key0, s);
+            if (all) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int32_t id = __shfl_sync(0xffffffffu, ids, 2 * (s & 15) + t);
-                const int64_t key = key0 + 16 * t, block = (int64_t)max(id, 0) * p.kv_heads + kvh;
-                const uint8_t *src = p.kc + ((block << p.page_log2) + (key & page_mask)) * D;
+                for (int t = 0; t < TILES; ++t) {
+                    const uint8_t *src = k_lane + offset_of(__shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t), key0 + 16 * t);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int row = g + 8 * r;
-                    const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
-#pragma unroll
-                    for (int c = 0; c < G::KC; ++c)
-                        copy_async<G::KB>(at + (((2 * t + r) * G::KC + c) * 32 + lane) * G::KB, src + row * D + c * 64 + j * G::KB, on);
+                    for (int i = 0; i < 2 * G::KC; ++i)     // row g + 8 r, piece c: i = r KC + c
+                        copy_async<G::KB>(at + (2 * t * G::KC + i) * 32 * G::KB, src + i / G::KC * 8 * D + i % G::KC * 64);
                 }
-                if (lane < 2) {                         // lane 0: the K scale, lane 1: the V scale
-                    const uint32_t to = scales0 + (s % G::STAGES) * 16 + (2 * t + lane) * 4;
-                    if (id >= 0) copy_async<4>(to, (lane ? p.vs : p.ks) + block, true);
-                    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(BAD_PAGE) : "memory");
+            } else {
+#pragma unroll 1
+                for (int t = 0; t < TILES; ++t) {
+                    const int32_t id = __shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t);
+                    const int64_t key = key0 + 16 * t;
+                    const uint8_t *src = k_lane + offset_of(id, key);
+#pragma unroll
+                    for (int i = 0; i < 2 * G::KC; ++i) {
+                        const int row = g + i / G::KC * 8;
+                        const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
+                        copy_async<G::KB>(at + (2 * t * G::KC + i) * 32 * G::KB, on ? src + i / G::KC * 8 * D + i % G::KC * 64 : p.kc, on);
+                    }
                 }
+            }
+            // lane 2 t: tile t's K scale, lane 2 t + 1: its V scale
+            const int32_t id = __shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + (lane >> 1) % TILES);
+            if (lane < 2 * TILES) {
+                const uint32_t to = scales0 + (s % G::STAGES) * G::SCALES + lane * 4;
+                if (id >= 0) copy_async<4>(to, (lane & 1 ? p.vs : p.ks) + ((int64_t)id * p.kv_heads + kvh));
+                else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(BAD_PAGE) : "memory");
             }
         }
         commit();
@@ -191,17 +223,28 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     auto issue_v = [&](int s) {
         if (s < stages) {
             const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
-            const uint32_t at = ring0 + (s % G::STAGES) * G::STAGE_BYTES + G::KBYTES;
+            const uint32_t at = v_slot + (s % G::STAGES) * G::STAGE_BYTES;
+            const bool all = whole(key0, s);
+            if (all) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int32_t id = __shfl_sync(0xffffffffu, ids, 2 * (s & 15) + t);
-                const int64_t key = key0 + 16 * t, block = (int64_t)max(id, 0) * p.kv_heads + kvh;
-                const uint8_t *src = p.vc + ((block << p.page_log2) + (key & page_mask)) * D;
+                for (int t = 0; t < TILES; ++t) {
+                    const uint8_t *src = v_lane + offset_of(__shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t), key0 + 16 * t);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 2 * j + (r & 1) + 8 * (r >> 1);
-                    const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
-                    copy_async<G::VB>(at + ((4 * t + r) * 32 + lane) * G::VB, src + row * D + g * G::VB, on);
+                    for (int r = 0; r < 4; ++r)             // rows 2 j + (r & 1) + 8 (r >> 1)
+                        copy_async<G::VB>(at + (4 * t + r) * 32 * G::VB, src + ((r & 1) + 8 * (r >> 1)) * D);
+                }
+            } else {
+#pragma unroll 1
+                for (int t = 0; t < TILES; ++t) {
+                    const int32_t id = __shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t);
+                    const int64_t key = key0 + 16 * t;
+                    const uint8_t *src = v_lane + offset_of(id, key);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = 2 * j + (r & 1) + 8 * (r >> 1);
+                        const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
+                        copy_async<G::VB>(at + (4 * t + r) * 32 * G::VB, on ? src + ((r & 1) + 8 * (r >> 1)) * D : p.vc, on);
+                    }
                 }
             }
         }
@@ -270,21 +313,27 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
         const uint32_t at = ring0 + (s % G::STAGES) * G::STAGE_BYTES;
         wait<2 * G::STAGES - 1>();
         __syncwarp();                                   // the scales were copied by lanes 0 and 1
-        uint32_t sc[4];
-        load_words(sc, scales0 + (s % G::STAGES) * 16);
-        const bool bad[2] = {sc[0] == BAD_PAGE, sc[2] == BAD_PAGE};
-        const float kscale[2] = {__uint_as_float(sc[0]), __uint_as_float(sc[2])};
-        // both tiles' V scales relative to the larger, so that the weights keep fp16's range
-        float vs0 = bad[0] ? 0.0f : __uint_as_float(sc[1]), vs1 = bad[1] ? 0.0f : __uint_as_float(sc[3]);
-        float vtop = fmaxf(vs0, vs1);
+        float kscale[TILES], weight[TILES], vtop = 0.0f;
+        uint32_t bad = 0;                               // tiles whose page was not followed
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            uint32_t sc[2];
+            load_words(sc, scales0 + (s % G::STAGES) * G::SCALES + 8 * t);
+            bad |= (uint32_t)(sc[0] == BAD_PAGE) << t;
+            kscale[t] = __uint_as_float(sc[0]);
+            weight[t] = sc[0] == BAD_PAGE ? 0.0f : __uint_as_float(sc[1]);
+            vtop = fmaxf(vtop, weight[t]);
+        }
+        // the tiles' V scales relative to the largest, so that the weights keep fp16's range
         if (!(vtop > 0.0f && vtop < INFINITY)) vtop = 1.0f;
-        const float weight[2] = {vs0 == vtop ? 16384.0f : vs0 / vtop * 16384.0f, vs1 == vtop ? 16384.0f : vs1 / vtop * 16384.0f};
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) weight[t] = weight[t] == vtop ? 16384.0f : __fdividef(weight[t], vtop) * 16384.0f;
         const float back = vtop * (1.0f / 16384.0f);
 
         // ---- scores ----
-        float c[2][NQ][4];
+        float c[TILES][NQ][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < TILES; ++t) {
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -296,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
                 load_words(w1, at + (((2 * t + 1) * G::KC + h) * 32 + lane) * G::KB);
 #pragma unroll
                 for (int k = 0; k < KW; ++k) {
-                    const uint32_t a[4] = {halves(w0[k]), halves(w1[k]), halves(w0[k] >> 16), halves(w1[k] >> 16)};
+                    const uint32_t a[4] = {halves(w0[k]), halves(w1[k]), high_halves(w0[k]), high_halves(w1[k])};
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
                         mma(c[t][n], a, qh[n][h * KW + k][0], qh[n][h * KW + k][1]);
@@ -309,29 +358,31 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
         issue_k(s + G::STAGES);
 
         // ---- softmax ----
-        const bool edge = key0 < first_hi || key0 + KEYS - 1 > pos_lo || key0 + KEYS > stop || bad[0] || bad[1];
-        uint32_t ph[2][NQ][2], pl[2][SPLIT ? NQ : 1][2], vis[2][NQ][2];
+        const bool edge = key0 < first_hi || key0 + KEYS - 1 > pos_lo || key0 + KEYS > stop || bad;
+        uint32_t off[NQ];
         float alpha[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < TILES; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[t][n][e] = c[t][n][e] * factor[n][e & 1] * kscale[t];
-            uint32_t off = 0;                           // bit 4 t + e: this score's key is not seen by its row
+            off[n] = 0;                                 // bit 4 t + e: this score's key is not seen by its row
             if (edge) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < TILES; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int64_t key = key0 + 16 * t + g + 8 * (e >> 1);
-                        const bool on = !bad[t] && key >= seen.first[n][e & 1] && key <= seen.pos[n][e & 1] && key < stop;
-                        if (!on) off |= 1u << (4 * t + e), c[t][n][e] = -INFINITY;
+                        const bool on = !(bad >> t & 1) && key >= seen.first[n][e & 1] && key <= seen.pos[n][e & 1] && key < stop;
+                        if (!on) off[n] |= 1u << (4 * t + e), c[t][n][e] = -INFINITY;
                     }
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float top = fmaxf(fmaxf(c[0][n][e], c[0][n][e + 2]), fmaxf(c[1][n][e], c[1][n][e + 2]));
+                float top = fmaxf(c[0][n][e], c[0][n][e + 2]);
+#pragma unroll
+                for (int t = 1; t < TILES; ++t) top = fmaxf(top, fmaxf(c[t][n][e], c[t][n][e + 2]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -340,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
                 m[n][e] = now;
                 float sum = 0.0f;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < TILES; ++t)
 #pragma unroll
                     for (int x = e; x < 4; x += 2) {
                         const float w = ex2(c[t][n][x] - ref);
@@ -351,107 +402,95 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
             }
             if (edge) {                                 // a scale that is NaN reaches only the rows that see its keys
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < TILES; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (off >> (4 * t + e) & 1) c[t][n][e] = 0.0f;
-                    const uint32_t v = ~off >> (4 * t);
-                    vis[t][n][0] = transposed((v & 1 ? 0x3C00u : 0u) | (v & 2 ? 0x3C000000u : 0u));
-                    vis[t][n][1] = transposed((v & 4 ? 0x3C00u : 0u) | (v & 8 ? 0x3C000000u : 0u));
-                }
+                        if (off[n] >> (4 * t + e) & 1) c[t][n][e] = 0.0f;
             }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t hi = pack(c[t][n][2 * e], c[t][n][2 * e + 1]);
-                    ph[t][n][e] = transposed(hi);
-                    if constexpr (SPLIT) pl[t][n][e] = transposed(pack_rest(hi, c[t][n][2 * e], c[t][n][2 * e + 1]));
-                }
         }
 
         // ---- values ----
         wait<2 * G::STAGES - 1>();
-        uint32_t v[2][4][VW];
+        float acc[MT][NQ][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) load_words(v[t][r], at + G::KBYTES + ((4 * t + r) * 32 + lane) * G::VB);
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.0f;
         // A fragments of the m-tiles 2 w and 2 w + 1 (dimensions g VB + 4 w ... + 3) from a word of four keys
         auto fragments = [](uint32_t (&a)[2][4], uint32_t k0, uint32_t k1, uint32_t k8, uint32_t k9) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint32_t x = __byte_perm(k0, k1, i ? 0x7362 : 0x5140), y = __byte_perm(k8, k9, i ? 0x7362 : 0x5140);
-                a[i][0] = halves(x), a[i][1] = halves(x >> 16), a[i][2] = halves(y), a[i][3] = halves(y >> 16);
+                a[i][0] = halves(x), a[i][1] = high_halves(x), a[i][2] = halves(y), a[i][3] = high_halves(y);
             }
         };
-        bool special = false;
-        if (edge) {                                     // NaN codes: 0 * NaN must not reach a row that does not see the key
-            uint32_t any = 0;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < TILES; ++t) {
+            uint32_t v[4][VW], ph[NQ][2], pl[SPLIT ? NQ : 1][2];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) load_words(v[r], at + G::KBYTES + ((4 * t + r) * 32 + lane) * G::VB);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t hi = pack(c[t][n][2 * e], c[t][n][2 * e + 1]);
+                    ph[n][e] = transposed(hi);
+                    if constexpr (SPLIT) pl[n][e] = transposed(pack_rest(hi, c[t][n][2 * e], c[t][n][2 * e + 1]));
+                }
+            if (edge) {                                 // NaN codes: 0 * NaN must not reach a row that does not see the key
+                uint32_t any = 0;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) any |= nan_codes(v[t][r][w]);
-            special = __any_sync(0xffffffffu, any != 0);
-        }
-        if (special) {                                  // count the NaN that each row sees, then take the codes as zeros
-#pragma unroll 1
-            for (int w = 0; w < VW; ++w) {
-                uint32_t a[2][2][4];
+                    for (int w = 0; w < VW; ++w) any |= nan_codes(v[r][w]);
+                if (__any_sync(0xffffffffu, any != 0)) {    // count the NaN that each row sees, then take the codes as zeros
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    uint32_t one[4];
+                    for (int w = 0; w < VW; ++w) {
+                        uint32_t one[4], a[2][4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        uint32_t x = v[t][r][0];
+                        for (int r = 0; r < 4; ++r) {
+                            one[r] = (nan_codes(v[r][w]) >> 7) * 0x38u;    // e4m3's 1.0
+                            v[r][w] &= ~((nan_codes(v[r][w]) >> 7) * 0xFFu);
+                        }
+                        fragments(a, one[0], one[1], one[2], one[3]);
 #pragma unroll
-                        for (int y = 1; y < VW; ++y) x = w == y ? v[t][r][y] : x;
-                        one[r] = (nan_codes(x) >> 7) * 0x38u;              // e4m3's 1.0
+                        for (int n = 0; n < NQ; ++n) {
+                            const uint32_t seen_by = ~off[n] >> (4 * t);
+                            const uint32_t s0 = transposed((seen_by & 1 ? 0x3C00u : 0u) | (seen_by & 2 ? 0x3C000000u : 0u));
+                            const uint32_t s1 = transposed((seen_by & 4 ? 0x3C00u : 0u) | (seen_by & 8 ? 0x3C000000u : 0u));
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                float count[4] = {};
+                                mma(count, a[i], s0, s1);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (count[e] != 0.0f) o[2 * w + i][n][e] = __int_as_float(0x7FC00000);
+                            }
+                        }
                     }
-                    fragments(a[t], one[0], one[1], one[2], one[3]);
                 }
+            }
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                uint32_t a[2][4];
+                fragments(a, v[0][w], v[1][w], v[2][w], v[3][w]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        float count[4] = {};
-                        mma(count, a[0][i], vis[0][n][0], vis[0][n][1]);
-                        mma(count, a[1][i], vis[1][n][0], vis[1][n][1]);
-#pragma unroll
-                        for (int y = 0; y < VW; ++y)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (w == y && count[e] != 0.0f) o[2 * y + i][n][e] = __int_as_float(0x7FC00000);
+                        mma(acc[2 * w + i][n], a[i], ph[n][0], ph[n][1]);
+                        if constexpr (SPLIT) mma(acc[2 * w + i][n], a[i], pl[n][0], pl[n][1]);
                     }
             }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) v[t][r][w] &= ~((nan_codes(v[t][r][w]) >> 7) * 0xFFu);
         }
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-            uint32_t a[2][2][4];
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) fragments(a[t], v[t][0][w], v[t][1][w], v[t][2][w], v[t][3][w]);
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    float acc[4] = {};
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        mma(acc, a[t][i], ph[t][n][0], ph[t][n][1]);
-                        if constexpr (SPLIT) mma(acc, a[t][i], pl[t][n][0], pl[t][n][1]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[2 * w + i][n][e] = fmaf(o[2 * w + i][n][e], alpha[n][e & 1], acc[e] * back);
-                }
-        }
+                for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(o[i][n][e], alpha[n][e & 1], acc[i][n][e] * back);
         issue_v(s + G::STAGES);
     }
     wait<0>();
@@ -504,29 +543,57 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     }
 }
 
-// Joins the splits of the keys: a warp per row.
+// Joins the splits of the keys: a CTA per row, its warps a split in four each.
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS) kv_attention_join_kernel(const CachedParams p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t rows = p.tokens * p.q_heads, row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    float top = -INFINITY, total = 0.0f, sum[D / 32] = {};
-    for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[s * rows + row].x);
+    constexpr int E = D / 32;
+    extern __shared__ __align__(16) float factor[];     // [splits]; then [WARPS][D] sums
+    __shared__ float red[2][WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t rows = p.tokens * p.q_heads, row = blockIdx.x;
+    float *sums = factor + p.splits;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' results are there
+    float top = -INFINITY;
+    for (int s = threadIdx.x; s < p.splits; s += THREADS) top = fmaxf(top, p.part_ml[s * rows + row].x);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    for (int s = 0; s < p.splits; ++s) {
+    if (lane == 0) red[0][warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red[0][w]);
+    float total = 0.0f;
+    for (int s = threadIdx.x; s < p.splits; s += THREADS) {
         const float2 ml = p.part_ml[s * rows + row];
-        if (ml.y == 0.0f) continue;
-        const float f = ex2(ml.x - top);
-        total += ml.y * f;
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) sum[e] += p.part_o[(s * rows + row) * D + e * 32 + lane] * f;
+        const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - top);
+        factor[s] = f;
+        total += ml.y == 0.0f ? 0.0f : ml.y * f;
     }
-    const int64_t t = row / p.q_heads, h = row % p.q_heads;
-    T *out = reinterpret_cast<T *>(p.out) + t * p.sot + h * p.soh;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) out[e * 32 + lane] = from_float<T>(total == 0.0f ? 0.0f : sum[e] / total);
-    if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    if (lane == 0) red[1][warp] = total;
+    __syncthreads();
+    total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += red[1][w];
+    float sum[E] = {};
+#pragma unroll 8
+    for (int s = warp; s < p.splits; s += WARPS) {
+        const float f = factor[s];
+        const float *from = p.part_o + (s * rows + row) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] += f == 0.0f ? 0.0f : from[e] * f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[warp * D + lane * E + e] = sum[e];
+    __syncthreads();
+    const int64_t t = row / p.q_heads, h = row % p.q_heads;
+    if (threadIdx.x < D) {
+        float all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) all += sums[w * D + threadIdx.x];
+        reinterpret_cast<T *>(p.out)[t * p.sot + h * p.soh + threadIdx.x] = from_float<T>(total == 0.0f ? 0.0f : all / total);
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
 }
 
 // How a call is cut: NQ 8-row groups a tile, row tiles a (sequence, key head), splits of the keys.
@@ -544,15 +611,16 @@ Plan plan_of(const piton_kv_attention_args *a) {
     // keys that a row tile can see, as far as the host knows
     int64_t span = a->max_length ? a->max_length : a->table_width * a->page_size;
     span = span < a->table_width * a->page_size ? span : a->table_width * a->page_size;
-    if (a->window && a->window + most_new + KEYS < span) span = a->window + most_new + KEYS;
+    const int64_t keys = 16 * (256 / a->head_dim);      // of a stage
+    if (a->window && a->window + most_new + keys < span) span = a->window + most_new + keys;
     // enough CTAs for every SM's three (two) and no split below 256 keys
     const int64_t units = plan.row_tiles * a->kv_heads * a->batch, slots = (int64_t)num_sms() * (plan.nq == 1 ? 3 : 2);
     int64_t splits = units >= slots ? 1 : slots / units;
     const int64_t most = cdiv(span, 256);
     splits = splits < most ? splits : most;
     if (splits < 1) splits = 1;
-    plan.chunk = cdiv(cdiv(span, splits), KEYS * WARPS) * (KEYS * WARPS);
-    if (plan.chunk == 0) plan.chunk = KEYS * WARPS;
+    plan.chunk = cdiv(cdiv(span, splits), keys * WARPS) * (keys * WARPS);
+    if (plan.chunk == 0) plan.chunk = keys * WARPS;
     plan.splits = span > 0 ? cdiv(span, plan.chunk) : 1;
     return plan;
 }
@@ -570,7 +638,18 @@ template <typename T, int D, int NQ> int launch(const CachedParams &p, int64_t b
     const dim3 grid((unsigned)(p.row_tiles * p.splits), (unsigned)p.kv_heads, (unsigned)batch);
     kv_attention_kernel<T, D, NQ><<<grid, THREADS, G::SMEM, s>>>(p);
     if (p.splits == 1) return check_launch("kv_attention");
-    kv_attention_join_kernel<T, D><<<(unsigned)cdiv(p.tokens * p.q_heads, WARPS), THREADS, 0, s>>>(p);
+    // launched while the splits finish (programmatic dependent launch); it waits for them before it reads
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.tokens * p.q_heads));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = (size_t)(p.splits + WARPS * D) * sizeof(float);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    PITON_CUDA(cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<T, D>, p));
     return check_launch("kv_attention", 2);
 }
 
@@ -637,7 +716,7 @@ extern "C" int piton_b200_kv_attention(const piton_kv_attention_args *a, void *s
         return set_error(PITON_B200_EWORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes,
                          (unsigned long long)need);
     PITON_REQUIRE(a->workspace % 16 == 0 || !need, "workspace is not 16-byte aligned");
-    PITON_REQUIRE(plan.row_tiles * plan.splits < (1ll << 31) && cdiv(rows, WARPS) < (1ll << 31), "too many blocks");
+    PITON_REQUIRE(plan.row_tiles * plan.splits < (1ll << 31) && rows < (1ll << 31), "too many blocks");
     CachedParams p;
     p.q = reinterpret_cast<const void *>(a->q);
     p.out = reinterpret_cast<void *>(a->out);
