@@ -39,7 +39,7 @@ struct CachedParams {
     float *part_o;                       // [splits][tokens * q_heads][D], splits > 1 only
     float2 *part_ml;                     // [splits][tokens * q_heads]
     int64_t tokens, num_pages, table_stride, sqt, sqh, sot, soh, window, uniform, chunk;
-    int32_t q_heads, kv_heads, group, page_log2, table_width, row_tiles, splits;
+    int32_t q_heads, kv_heads, group, page_log2, table_width, row_tiles, splits, q_aligned;
     float scale;
 };
 
@@ -49,11 +49,11 @@ template <int D> struct Geometry {
     static constexpr int KB = D >= 64 ? 16 : D / 4;     // bytes of a key row in one copy of a lane
     static constexpr int KC = D / (4 * KB);             // such copies per row
     static constexpr int VB = D / 8;                    // bytes of a value row that a lane takes
-    static constexpr int TILES = 256 / D, KEYS = 16 * TILES;  // of a stage: 16-key tiles, each inside one page; 8 KB at every D
-    static constexpr int STAGES = 2, KBYTES = KEYS * D, STAGE_BYTES = 2 * KBYTES;
-    static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
+    static constexpr int TILES = D == 128 ? 2 : 4, KEYS = 16 * TILES;     // of a stage: 16-key tiles, each inside one page
+    // a warp's queue: two stages of keys and one of values, whose copies run while the scores are computed
+    static constexpr int BYTES = KEYS * D, QUEUE = 3 * BYTES, RING = WARPS * QUEUE;
     static constexpr int SCALES = 8 * TILES;            // bytes of a stage's K and V scales, tile by tile
-    static constexpr int SMEM = RING + WARPS * STAGES * SCALES;
+    static constexpr int SMEM = RING + WARPS * 2 * SCALES;
     static constexpr int RUN = 32 / TILES;              // stages whose page numbers the lanes hold at a time
 };
 
@@ -104,6 +104,11 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // c = a b
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -114,8 +119,24 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Four elements of a row, in one load where rows are aligned for it.
+template <typename T> __device__ __forceinline__ void load_four(float (&x)[4], const T *at, bool aligned) {
+    T v[4];
+    if (aligned) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(at);
+        else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(at);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = at[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = to_float(v[e]);
+}
 // NaN codes (7F and FF) of a word: a set high bit in each such byte.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// CTAs an SM holds: registers bound it. Sixteen-bit rows add their products straight into the output's registers.
+template <typename T> constexpr int ctas(int nq) { return (nq == 1 ? 4 : 3) - (sizeof(T) == 4 ? 1 : 0); }
 
 // The rows of a tile that a lane holds in its score and output fragments: columns 2 j and 2 j + 1 of each of the NQ
 // 8-row groups; the keys [first, pos] that each sees.
@@ -124,9 +145,10 @@ template <int NQ> struct Rows {
 };
 
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(const CachedParams p) {
+__global__ void __launch_bounds__(THREADS, NQ == 2 ? 2 : 3) kv_attention_kernel(const CachedParams p) {
     using G = Geometry<D>;
     constexpr bool SPLIT = sizeof(T) == 4;              // fp32 rows: queries and weights as pairs of halves
+    constexpr float LIFT = SPLIT ? 14.0f : 6.0f, SLACK = SPLIT ? 0.0f : 8.0f;
     constexpr int R = 8 * NQ, KW = G::KB / 4, VW = G::VB / 4, MT = D / 16, KT = D / 16, TILES = G::TILES, KEYS = G::KEYS;
     extern __shared__ __align__(16) uint8_t ring[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
@@ -134,19 +156,25 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     const int64_t b = blockIdx.z;
     const int kvh = blockIdx.y, tile = blockIdx.x % p.row_tiles, split = blockIdx.x / p.row_tiles;
     const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
-    const int64_t rows = sp.n * p.group;
-    const int64_t row0 = (int64_t)tile * R;
+    const uint32_t group = p.group, rows = (uint32_t)sp.n * group, row0 = (uint32_t)tile * R;   // below 2^31, as tokens * heads is
     if (row0 >= rows) return;
-    const int live = (int)min((int64_t)R, rows - row0);
+    const uint32_t live = min((uint32_t)R, rows - row0);
     // positions are below 2^31 (lengths are int32); a row past the tile's last repeats the last one
     const int32_t length = p.lengths[b];
+    const int32_t *table = p.table + b * p.table_stride;
+    const int64_t held = (int64_t)p.table_width << p.page_log2;
+    // Without a window the first keys do not depend on the length, so their page numbers are read along with it.
+    int32_t ahead = -1;
+    if (!p.window) {
+        const int64_t key = (int64_t)split * p.chunk + warp * KEYS + (int64_t)(lane / TILES) * (KEYS * WARPS) + 16 * (lane % TILES);
+        if (key < held) ahead = table[key >> p.page_log2];
+    }
     const int32_t before = length - (int32_t)sp.n;      // position of query token 0
-    auto pos_of = [&](int r) { return before + (int32_t)((row0 + min(r, live - 1)) / p.group); };
+    auto pos_of = [&](uint32_t r) { return before + (int32_t)((row0 + min(r, live - 1)) / group); };
     auto first_of = [&](int32_t pos) { return p.window ? (int32_t)max((int64_t)pos - p.window + 1, (int64_t)0) : 0; };
     const int32_t pos_lo = pos_of(0), pos_hi = pos_of(R - 1);
     const int32_t first_lo = first_of(pos_lo), first_hi = first_of(pos_hi);
     int64_t end = (int64_t)pos_hi + 1;                  // no row of the tile sees a key outside [first_lo, end)
-    const int64_t held = (int64_t)p.table_width << p.page_log2;
     if (end > held) {
         if (threadIdx.x == 0) record_status(STATUS_BAD_POSITION);
         end = held;
@@ -157,23 +185,23 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     const int stages = stop > mine ? (int)((stop - mine + KEYS * WARPS - 1) / (KEYS * WARPS)) : 0;
 
     // ---- this lane's copies ----
-    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * (G::STAGES * G::STAGE_BYTES);
-    const uint32_t scales0 = (uint32_t)__cvta_generic_to_shared(ring) + G::RING + warp * (G::STAGES * G::SCALES);
+    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * G::QUEUE;
+    const uint32_t scales0 = (uint32_t)__cvta_generic_to_shared(ring) + G::RING + warp * (2 * G::SCALES);
     const int32_t page_mask = (1 << p.page_log2) - 1;
-    const uint32_t k_slot = ring0 + lane * G::KB, v_slot = ring0 + G::KBYTES + lane * G::VB;
+    const uint32_t k_slot = ring0 + lane * G::KB, v_slot = ring0 + 2 * G::BYTES + lane * G::VB;
     const uint8_t *k_lane = p.kc + g * D + j * G::KB, *v_lane = p.vc + 2 * j * D + g * G::VB;
-    int32_t ids = -1, ids_next = -1;                    // pages of the 32 tiles of RUN stages, lane by lane
-    uint32_t off_run = 0;                               // which of them are not to be read
+    int32_t ids = -1, ids_next = -1, ids_v = -1;        // pages of the 32 tiles of RUN stages, lane by lane; the values' are a stage behind
+    uint32_t off_run = 0, off_run_v = 0;                // which of them are not to be read
     auto load_ids = [&](int s0) {                       // stages s0 .. s0 + RUN - 1
         const int64_t key = mine + (int64_t)(s0 + lane / TILES) * (KEYS * WARPS) + 16 * (lane % TILES);
         if (key >= stop || key + 15 < first_lo) return -1;
-        const int32_t id = p.table[b * p.table_stride + (key >> p.page_log2)];
+        const int32_t id = s0 == 0 && !p.window ? ahead : table[key >> p.page_log2];
         if (id >= 0 && id < p.num_pages) return id;
         record_status(STATUS_BAD_PAGE);
         return -1;
     };
-    auto whole = [&](int64_t key0, int s) {             // every key of the stage exists
-        return key0 >= first_lo && key0 + KEYS <= stop && !(off_run >> (TILES * (s % G::RUN)) & ((1u << TILES) - 1));
+    auto whole = [&](int64_t key0, int s, uint32_t off) {   // every key of the stage exists
+        return key0 >= first_lo && key0 + KEYS <= stop && !(off >> (TILES * (s % G::RUN)) & ((1u << TILES) - 1));
     };
     auto offset_of = [&](int32_t id, int64_t key) {     // of a key's row in either array of codes
         return (((int64_t)max(id, 0) * p.kv_heads + kvh << p.page_log2) + (key & page_mask)) * D;
@@ -186,8 +214,8 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
                 ids_next = load_ids(s + G::RUN);
             }
             const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
-            const uint32_t at = k_slot + (s % G::STAGES) * G::STAGE_BYTES;
-            const bool all = whole(key0, s);
+            const uint32_t at = k_slot + (s & 1) * G::BYTES;
+            const bool all = whole(key0, s, off_run);
             if (all) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
@@ -213,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
             // lane 2 t: tile t's K scale, lane 2 t + 1: its V scale
             const int32_t id = __shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + (lane >> 1) % TILES);
             if (lane < 2 * TILES) {
-                const uint32_t to = scales0 + (s % G::STAGES) * G::SCALES + lane * 4;
+                const uint32_t to = scales0 + (s & 1) * G::SCALES + lane * 4;
                 if (id >= 0) copy_async<4>(to, (lane & 1 ? p.vs : p.ks) + ((int64_t)id * p.kv_heads + kvh));
                 else asm volatile("st.shared.u32 [%0], %1;" ::"r"(to), "r"(BAD_PAGE) : "memory");
             }
@@ -222,13 +250,14 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     };
     auto issue_v = [&](int s) {
         if (s < stages) {
+            if (s % G::RUN == 0) ids_v = ids, off_run_v = off_run;     // the keys are at most one stage on
             const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
-            const uint32_t at = v_slot + (s % G::STAGES) * G::STAGE_BYTES;
-            const bool all = whole(key0, s);
+            const uint32_t at = v_slot;
+            const bool all = whole(key0, s, off_run_v);
             if (all) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
-                    const uint8_t *src = v_lane + offset_of(__shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t), key0 + 16 * t);
+                    const uint8_t *src = v_lane + offset_of(__shfl_sync(0xffffffffu, ids_v, TILES * (s % G::RUN) + t), key0 + 16 * t);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)             // rows 2 j + (r & 1) + 8 (r >> 1)
                         copy_async<G::VB>(at + (4 * t + r) * 32 * G::VB, src + ((r & 1) + 8 * (r >> 1)) * D);
@@ -236,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
             } else {
 #pragma unroll 1
                 for (int t = 0; t < TILES; ++t) {
-                    const int32_t id = __shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t);
+                    const int32_t id = __shfl_sync(0xffffffffu, ids_v, TILES * (s % G::RUN) + t);
                     const int64_t key = key0 + 16 * t;
                     const uint8_t *src = v_lane + offset_of(id, key);
 #pragma unroll
@@ -250,10 +279,9 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
         }
         commit();
     };
-    for (int s = 0; s < G::STAGES; ++s) {
-        issue_k(s);
-        issue_v(s);
-    }
+    issue_k(0);
+    issue_k(1);
+    issue_v(0);
 
     // ---- the queries: B fragments, scaled by a power of two per row ----
     uint32_t qh[NQ][KT][2], ql[SPLIT ? NQ : 1][KT][2];
@@ -261,18 +289,15 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     Rows<NQ> seen;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int64_t r = row0 + min(8 * n + g, live - 1);
-        const T *q = reinterpret_cast<const T *>(p.q) + (sp.t0 + r / p.group) * p.sqt + (kvh * p.group + r % p.group) * p.sqh;
+        const uint32_t r = row0 + min((uint32_t)(8 * n + g), live - 1);
+        const T *q = reinterpret_cast<const T *>(p.q) + (sp.t0 + r / group) * p.sqt + (kvh * group + r % group) * p.sqh;
         float x[KT][4], top = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const T *at = q + (k / KW) * 64 + j * G::KB + 4 * (k % KW);
+        for (int k = 0; k < KT; ++k) load_four(x[k], q + (k / KW) * 64 + j * G::KB + 4 * (k % KW), p.q_aligned);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[k][e] = to_float(at[e]);
-                top = fmaxf(top, isfinite(x[k][e]) ? fabsf(x[k][e]) : 0.0f);
-            }
-        }
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, isfinite(x[k][e]) ? fabsf(x[k][e]) : 0.0f);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // the row's largest magnitude in [2^14, 2^15)
@@ -306,38 +331,44 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.0f;
+    float vref = 0.0f;                                  // 16-bit rows: O is kept relative to the largest V scale so far
 
 #pragma unroll 1
     for (int s = 0; s < stages; ++s) {
         const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
-        const uint32_t at = ring0 + (s % G::STAGES) * G::STAGE_BYTES;
-        wait<2 * G::STAGES - 1>();
+        const uint32_t at = ring0 + (s & 1) * G::BYTES;
+        wait<2>();                                      // the next stage's keys and this one's values may be on their way
         __syncwarp();                                   // the scales were copied by lanes 0 and 1
         float kscale[TILES], weight[TILES], vtop = 0.0f;
         uint32_t bad = 0;                               // tiles whose page was not followed
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             uint32_t sc[2];
-            load_words(sc, scales0 + (s % G::STAGES) * G::SCALES + 8 * t);
+            load_words(sc, scales0 + (s & 1) * G::SCALES + 8 * t);
             bad |= (uint32_t)(sc[0] == BAD_PAGE) << t;
             kscale[t] = __uint_as_float(sc[0]);
             weight[t] = sc[0] == BAD_PAGE ? 0.0f : __uint_as_float(sc[1]);
             vtop = fmaxf(vtop, weight[t]);
         }
         // the tiles' V scales relative to the largest, so that the weights keep fp16's range
-        if (!(vtop > 0.0f && vtop < INFINITY)) vtop = 1.0f;
+        if (!(vtop > 0.0f && vtop < INFINITY)) vtop = vref > 0.0f ? vref : 1.0f;
+        float shrink = 1.0f;
+        if constexpr (!SPLIT) {
+            if (vtop > vref) shrink = vref / vtop, vref = vtop;
+            vtop = vref;
+        }
+        bool level = true;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) weight[t] = weight[t] == vtop ? 16384.0f : __fdividef(weight[t], vtop) * 16384.0f;
-        const float back = vtop * (1.0f / 16384.0f);
+        for (int t = 0; t < TILES; ++t) level = level && weight[t] == vtop;
+        if (!level) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) weight[t] = weight[t] == vtop ? 1.0f : weight[t] / vtop;
+        }
 
         // ---- scores ----
         float c[TILES][NQ][4];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) c[t][n][e] = 0.0f;
 #pragma unroll
             for (int h = 0; h < G::KC; ++h) {
                 uint32_t w0[KW], w1[KW];
@@ -348,14 +379,15 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
                     const uint32_t a[4] = {halves(w0[k]), halves(w1[k]), high_halves(w0[k]), high_halves(w1[k])};
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        mma(c[t][n], a, qh[n][h * KW + k][0], qh[n][h * KW + k][1]);
+                        if (h + k == 0) mma_first(c[t][n], a, qh[n][0][0], qh[n][0][1]);
+                        else mma(c[t][n], a, qh[n][h * KW + k][0], qh[n][h * KW + k][1]);
                         if constexpr (SPLIT) mma(c[t][n], a, ql[n][h * KW + k][0], ql[n][h * KW + k][1]);
                     }
                 }
             }
         }
         __syncwarp();
-        issue_k(s + G::STAGES);
+        issue_k(s + 2);
 
         // ---- softmax ----
         const bool edge = key0 < first_hi || key0 + KEYS - 1 > pos_lo || key0 + KEYS > stop || bad;
@@ -386,19 +418,27 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                const float now = fmaxf(m[n][e], top), ref = now == -INFINITY ? 0.0f : now;
-                alpha[n][e] = ex2(m[n][e] - ref);
+                // The reference of the exponents: the largest score so far; 16-bit rows let a score pass it by up to 2^SLACK, so
+                // that O is rarely rescaled, which LIFT leaves room for in the weights' fp16.
+                const float now = SPLIT ? fmaxf(m[n][e], top) : top > m[n][e] + SLACK ? top : m[n][e];
+                const float ref = (now == -INFINITY ? 0.0f : now) - LIFT;
+                alpha[n][e] = now == m[n][e] ? 1.0f : ex2(m[n][e] - now);
                 m[n][e] = now;
                 float sum = 0.0f;
 #pragma unroll
                 for (int t = 0; t < TILES; ++t)
 #pragma unroll
                     for (int x = e; x < 4; x += 2) {
-                        const float w = ex2(c[t][n][x] - ref);
-                        sum += w;
-                        c[t][n][x] = w * weight[t];
+                        c[t][n][x] = ex2(c[t][n][x] - ref);
+                        sum += c[t][n][x];
                     }
                 l[n][e] = l[n][e] * alpha[n][e] + sum;
+            }
+            if (!level) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[t][n][e] *= weight[t];
             }
             if (edge) {                                 // a scale that is NaN reaches only the rows that see its keys
 #pragma unroll
@@ -410,14 +450,21 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
         }
 
         // ---- values ----
-        wait<2 * G::STAGES - 1>();
-        float acc[MT][NQ][4];
+        wait<1>();                                      // the keys after the next may be on their way
+        float acc[SPLIT ? MT : 1][NQ][4];               // fp32 rows: a stage's sums, added to O in fp32
+        if constexpr (!SPLIT) {
+            bool moved = shrink != 1.0f;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+            for (int n = 0; n < NQ; ++n) moved = moved || alpha[n][0] != 1.0f || alpha[n][1] != 1.0f;
+            if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.0f;
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][n][e] *= alpha[n][e & 1] * shrink;
+            }
+        }
         // A fragments of the m-tiles 2 w and 2 w + 1 (dimensions g VB + 4 w ... + 3) from a word of four keys
         auto fragments = [](uint32_t (&a)[2][4], uint32_t k0, uint32_t k1, uint32_t k8, uint32_t k9) {
 #pragma unroll
@@ -430,7 +477,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
         for (int t = 0; t < TILES; ++t) {
             uint32_t v[4][VW], ph[NQ][2], pl[SPLIT ? NQ : 1][2];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) load_words(v[r], at + G::KBYTES + ((4 * t + r) * 32 + lane) * G::VB);
+            for (int r = 0; r < 4; ++r) load_words(v[r], v_slot + (4 * t + r) * 32 * G::VB);
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -480,18 +527,25 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        mma(acc[2 * w + i][n], a[i], ph[n][0], ph[n][1]);
-                        if constexpr (SPLIT) mma(acc[2 * w + i][n], a[i], pl[n][0], pl[n][1]);
+                        if constexpr (SPLIT) {
+                            if (t == 0) mma_first(acc[2 * w + i][n], a[i], ph[n][0], ph[n][1]);
+                            else mma(acc[2 * w + i][n], a[i], ph[n][0], ph[n][1]);
+                            mma(acc[2 * w + i][n], a[i], pl[n][0], pl[n][1]);
+                        } else {
+                            mma(o[2 * w + i][n], a[i], ph[n][0], ph[n][1]);
+                        }
                     }
             }
         }
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
+                for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(o[i][n][e], alpha[n][e & 1], acc[i][n][e] * back);
-        issue_v(s + G::STAGES);
+                    for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(o[i][n][e], alpha[n][e & 1], acc[i][n][e] * vtop);
+        }
+        issue_v(s + 1);
     }
     wait<0>();
 
@@ -500,6 +554,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+            m[n][e] -= LIFT;                            // l and O are 2^LIFT times what belongs to m
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
@@ -513,12 +568,13 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
         for (int e = 0; e < 2; ++e) {
             const int r = 8 * n + 2 * j + e;
             if (g == 0) sml[warp * R + r] = make_float2(m[n][e], l[n][e]);
+            const float back = SPLIT ? 1.0f : vref;
             float *to = so + (warp * R + r) * D + g * G::VB;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) *reinterpret_cast<float2 *>(to + 2 * i) = make_float2(o[i][n][e], o[i][n][e + 2]);
+            for (int i = 0; i < MT; ++i) *reinterpret_cast<float2 *>(to + 2 * i) = make_float2(o[i][n][e] * back, o[i][n][e + 2] * back);
         }
     __syncthreads();
-    for (int x = threadIdx.x; x < live * D; x += THREADS) {
+    for (int x = threadIdx.x; x < (int)live * D; x += THREADS) {
         const int r = x / D, d = x % D;
         float top = -INFINITY, total = 0.0f, sum = 0.0f;
 #pragma unroll
@@ -531,7 +587,7 @@ __global__ void __launch_bounds__(THREADS, NQ == 1 ? 3 : 2) kv_attention_kernel(
             total += ml.y * f;
             sum += so[(w * R + r) * D + d] * f;
         }
-        const int64_t t = sp.t0 + (row0 + r) / p.group, h = kvh * p.group + (row0 + r) % p.group;
+        const int64_t t = sp.t0 + (row0 + r) / group, h = kvh * group + (row0 + r) % group;
         if (p.splits == 1) {
             reinterpret_cast<T *>(p.out)[t * p.sot + h * p.soh + d] = from_float<T>(total == 0.0f ? 0.0f : sum / total);
             if (p.lse && d == 0) p.lse[t * p.q_heads + h] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
@@ -611,10 +667,10 @@ Plan plan_of(const piton_kv_attention_args *a) {
     // keys that a row tile can see, as far as the host knows
     int64_t span = a->max_length ? a->max_length : a->table_width * a->page_size;
     span = span < a->table_width * a->page_size ? span : a->table_width * a->page_size;
-    const int64_t keys = 16 * (256 / a->head_dim);      // of a stage
+    const int64_t keys = a->head_dim == 128 ? 32 : 64;  // of a stage
     if (a->window && a->window + most_new + keys < span) span = a->window + most_new + keys;
-    // enough CTAs for every SM's three (two) and no split below 256 keys
-    const int64_t units = plan.row_tiles * a->kv_heads * a->batch, slots = (int64_t)num_sms() * (plan.nq == 1 ? 3 : 2);
+    // enough CTAs for every SM and no split below 256 keys
+    const int64_t units = plan.row_tiles * a->kv_heads * a->batch, slots = (int64_t)num_sms() * (plan.nq == 2 ? 2 : plan.nq == 1 ? 3 : a->type == PITON_B200_TYPE_F32 ? ctas<float>(plan.nq) : ctas<__half>(plan.nq));
     int64_t splits = units >= slots ? 1 : slots / units;
     const int64_t most = cdiv(span, 256);
     splits = splits < most ? splits : most;
@@ -716,7 +772,7 @@ extern "C" int piton_b200_kv_attention(const piton_kv_attention_args *a, void *s
         return set_error(PITON_B200_EWORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes,
                          (unsigned long long)need);
     PITON_REQUIRE(a->workspace % 16 == 0 || !need, "workspace is not 16-byte aligned");
-    PITON_REQUIRE(plan.row_tiles * plan.splits < (1ll << 31) && rows < (1ll << 31), "too many blocks");
+    PITON_REQUIRE(plan.row_tiles * plan.splits < (1ll << 31) && rows < (1ll << 31), "tokens times heads too large");
     CachedParams p;
     p.q = reinterpret_cast<const void *>(a->q);
     p.out = reinterpret_cast<void *>(a->out);
@@ -737,6 +793,8 @@ extern "C" int piton_b200_kv_attention(const piton_kv_attention_args *a, void *s
     p.page_log2 = a->page_size == 16 ? 4 : a->page_size == 32 ? 5 : a->page_size == 64 ? 6 : 7;
     p.table_width = (int32_t)a->table_width; p.row_tiles = (int32_t)plan.row_tiles; p.splits = (int32_t)plan.splits;
     p.scale = (float)a->sm_scale;
+    const uint64_t size = a->type == PITON_B200_TYPE_F32 ? 4 : 2;
+    p.q_aligned = (a->q | (uint64_t)a->stride_qt * size | (uint64_t)a->stride_qh * size) % (4 * size) == 0;
     return with_type(a->type, [&](auto t) {
         using T = decltype(t);
         cudaStream_t s = as_stream(stream);
