@@ -6,6 +6,8 @@ Every ``csrc/*.cu`` file is compiled to an object under ``csrc/_build/`` with
 ``nvcc -gencode arch=compute_100a,code=sm_100a`` (in parallel), then linked
 into ``piton_b200/libpiton_b200.so``.  nvcc cross-compiles, so this runs on a
 machine without a GPU; the shared object travels with the source tree.
+``csrc/decode_calls.cpp``, the argument marshalling of ``piton_b200.decode``, is
+compiled against the installed torch into ``piton_b200/_decode_calls.so``.
 """
 
 from __future__ import annotations
@@ -23,6 +25,7 @@ REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(CSRC, "_build")
 LIB = os.path.join(PKG, "libpiton_b200.so")
+CALLS = os.path.join(PKG, "_decode_calls.so")
 INCLUDE = os.path.join(REPO, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -64,12 +67,40 @@ def _compile(src: str, deps: list, verbose: bool) -> str:
     return obj
 
 
+def _build_calls(verbose: bool) -> str:
+    """The extension module of piton_b200.decode: host code only, built by g++."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    src, stamp = os.path.join(CSRC, "decode_calls.cpp"), os.path.join(OBJ, "decode_calls.sha")
+    digest = _digest(src, [os.path.join(INCLUDE, "piton_b200.h")]) + torch.__version__
+    if os.path.exists(CALLS) and os.path.exists(stamp) and open(stamp).read() == digest:
+        return CALLS
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-shared", "-fPIC", "-fvisibility=hidden", src, "-o", CALLS,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + INCLUDE,
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+           *["-I" + p for p in include_paths()], *["-L" + p for p in library_paths()],
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {src}:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(digest)
+    return CALLS
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     sources = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     headers = sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h")))
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        calls = ex.submit(_build_calls, verbose)
         objs = list(ex.map(lambda s: _compile(s, headers, verbose), sources))
+        calls.result()
     newest = max(os.path.getmtime(o) for o in objs)
     if not os.path.exists(LIB) or os.path.getmtime(LIB) < newest:
         cmd = [nvcc()] + ARCH + ["-shared", "-o", LIB] + objs + ["-lcuda"]

@@ -23,8 +23,6 @@ reports 16 (page) or 17 (position).
 from __future__ import annotations
 
 import ctypes as C
-import math
-import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -54,42 +52,33 @@ class PagedKV(NamedTuple):
         return cls(*codes, *scales)
 
 
-# A decode step makes these calls every few microseconds, so the ordinary call evaluates one condition
-# over everything it needs and packs the C struct with one format; only where the condition fails are
-# the arguments looked at one by one (the _refuse_* functions), to say what is wrong.
-
-_LETTERS = {_lib.u64: "Q", _lib.i64: "q", _lib.i32: "i", _lib.u32: "I", _lib.f64: "d"}
+_ENTRIES = ("piton_b200_kv_append", "piton_b200_kv_attention", "piton_b200_kv_attention_workspace_size", "piton_b200_matvec_w4")
+_bound = None
 
 
-def _packer(struct_type):
-    """Packs the fields of a ctypes struct, in order, into bytes."""
-    s = struct.Struct("@" + "".join(_LETTERS[t] for _, t in struct_type._fields_))
-    assert s.size == C.sizeof(struct_type)
-    return s.pack
+def _calls():
+    """The extension module that checks and marshals the calls, bound to the loaded library."""
+    global _bound
+    if _bound is None:
+        try:
+            from . import _decode_calls
+        except ImportError as e:
+            raise ImportError(f"piton_b200/_decode_calls.so: {e}; build it with `python -m piton_b200.build`") from e
+        handle = lib()
+        _decode_calls.bind(*(C.cast(getattr(handle, name), C.c_void_p).value for name in _ENTRIES), torch.OutOfMemoryError)
+        _bound = _decode_calls
+    return _bound
 
 
-_pack_append, _pack_attention, _pack_matvec = map(_packer, (_lib.KvAppendArgs, _lib.KvAttentionArgs, _lib.MatvecW4Args))
-_ENTRY = {}
+def _failed(what: str, result, refuse, *args):
+    """Raises for a call that gave a status code, or None for an argument that `refuse` finds."""
+    if result is None:
+        refuse(*args)
+        raise ValueError(f"{what}: unsupported arguments")
+    check(result, what)
 
 
-def _entry(name: str, restype=C.c_int, *rest):
-    """The library's function taking a packed struct."""
-    f = lib()[name]
-    f.restype, f.argtypes = restype, [C.c_char_p, *rest]
-    _ENTRY[name] = f
-    return f
-
-
-def _call(name: str, packed: bytes, index: int) -> None:
-    f = _ENTRY.get(name) or _entry(name, C.c_int, C.c_void_p)
-    if torch.cuda.current_device() == index:
-        rc = f(packed, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = f(packed, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        check(rc, name[len("piton_b200_"):])
-
+# What is wrong with a call that was not made: the arguments one by one.
 
 def _need(ok: bool, message: str) -> None:
     if not ok:
@@ -117,6 +106,8 @@ def _refuse_rows(name: str, t, dtype, heads, dim: int, index: int) -> None:
 
 
 def _refuse_cache(cache, index: int) -> None:
+    if not isinstance(cache, tuple) or len(cache) != 4:
+        raise TypeError("cache: expected a PagedKV or a tuple (k, v, k_scale, v_scale)")
     k, v, ks, vs = cache
     for name, t, dtypes in (("k", k, _CODES), ("v", v, _CODES), ("k_scale", ks, (torch.float32,)),
                             ("v_scale", vs, (torch.float32,))):
@@ -135,18 +126,62 @@ def _refuse_indices(table, vectors, cu, batch: int, tokens: int, index: int) -> 
           f"{tokens} tokens are not the same number for each of {batch} sequences: pass cu")
 
 
-def _table(table, index: int):
-    """(batch, width, row stride) of a page table."""
-    if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.get_device() != index:
-        _refuse_tensor("table", table, (torch.int32,), index)
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table: expected [batch, width], rows contiguous")
-    batch, width = table.shape
-    return batch, width, table.stride(0)
+def _refuse_table(table, index: int) -> int:
+    _refuse_tensor("table", table, (torch.int32,), index)
+    _need(table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1), "table: expected [batch, width], rows contiguous")
+    return table.shape[0]
 
 
-def _same(t, dtype, index: int) -> bool:
-    return t.dtype is dtype and t.get_device() == index
+def _refuse_append(k, v, cache, table, starts, cu, cos, sin, interleaved, q) -> None:
+    _type_of("k", k)
+    index, dtype = k.get_device(), k.dtype
+    _refuse_cache(cache, index)
+    heads, dim = cache[0].shape[1], cache[0].shape[3]
+    _refuse_rows("k", k, dtype, heads, dim, index)
+    _refuse_rows("v", v, dtype, heads, dim, index)
+    tokens = k.shape[0]
+    _need(v.shape[0] == tokens, f"k has {tokens} tokens, v {v.shape[0]}")
+    batch = _refuse_table(table, index)
+    _refuse_indices(table, (("starts", starts, batch),), cu, batch, tokens, index)
+    if cos is not None or sin is not None:
+        _need(cos is not None and sin is not None, "pass both cos and sin, or neither")
+        _refuse_tensor("cos", cos, (torch.float32,), index)
+        _refuse_tensor("sin", sin, (torch.float32,), index)
+        _need(cos.dim() == 2 and cos.shape == sin.shape and 2 * cos.shape[1] <= dim and cos.is_contiguous() and
+              sin.is_contiguous(), f"cos, sin: expected two contiguous [positions, at most {dim // 2}], got {tuple(cos.shape)} and "
+              f"{tuple(sin.shape)}")
+    if q is not None:
+        _refuse_rows("q", q, dtype, None, dim, index)
+        _need(q.shape[0] == tokens, f"k has {tokens} tokens, q {q.shape[0]}")
+
+
+def _refuse_attention(q, cache, table, lengths, cu, scale, window, max_length, max_new, return_lse) -> None:
+    _type_of("q", q)
+    index = q.get_device()
+    _refuse_cache(cache, index)
+    _refuse_rows("q", q, q.dtype, None, cache[0].shape[3], index)
+    batch = _refuse_table(table, index)
+    _refuse_indices(table, (("lengths", lengths, batch),), cu, batch, q.shape[0], index)
+    _need(window >= 0 and max_length >= 0 and max_new >= 0, "window, max_length and max_new must not be negative")
+
+
+def _refuse_matvec(x, codes, scales, group, zeros, bias) -> None:
+    _type_of("x", x)
+    index = x.get_device()
+    if group not in (32, 64, 128):
+        raise NotImplementedError(f"group {group}: 32, 64 or 128")
+    _need(x.dim() in (1, 2), f"x: shape {tuple(x.shape)}, expected [rows, inner] or [inner]")
+    _refuse_tensor("codes", codes, (torch.uint8,), index)
+    _refuse_tensor("scales", scales, tuple(_TYPES), index)
+    if zeros is not None:
+        _refuse_tensor("zeros", zeros, (torch.uint8,), index)
+    if bias is not None:
+        _refuse_tensor("bias", bias, (x.dtype,), index)
+    outer, inner = codes.shape[0], x.shape[-1]
+    raise ValueError(f"x {tuple(x.shape)}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}, zeros "
+                     f"{None if zeros is None else tuple(zeros.shape)}, bias {None if bias is None else tuple(bias.shape)}: "
+                     f"expected codes [{outer}, {(inner + 1) // 2}], scales and zeros [{outer}, {-(-inner // group)}], bias "
+                     f"[{outer}], each with unit stride in its last dimension")
 
 
 def kv_append(k, v, cache, table, starts, *, cu=None, cos=None, sin=None, interleaved: bool = False, q=None):
@@ -163,60 +198,11 @@ def kv_append(k, v, cache, table, starts, *, cu=None, cos=None, sin=None, interl
     A block (page and head) has one scale: the least power of two that holds its values within e4m3's 448;
     when new values make it grow, the block's older codes are requantised.  Non-finite values are stored
     as NaN and do not move the scale."""
-    kind = _type_of("k", k)
-    index, dtype = k.get_device(), k.dtype
-    kc, vc, ks, vs = cache
-    shape = kc.shape
-    if len(shape) != 4:
-        _refuse_cache(cache, index)
-    pages, heads, page, dim = shape
-    batch, width, stride = _table(table, index)
-    tokens = k.shape[0]
-    if not (k.dim() == 3 and k.shape == v.shape and k.shape[1] == heads and k.shape[2] == dim and v.dtype is dtype and
-            v.get_device() == index and k.stride(2) == 1 and v.stride(2) == 1 and
-            kc.dtype in _CODES and vc.dtype in _CODES and vc.shape == shape and ks.shape == shape[:2] == vs.shape and
-            _same(ks, torch.float32, index) and _same(vs, torch.float32, index) and kc.get_device() == index and
-            vc.get_device() == index and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and
-            vs.is_contiguous() and _same(starts, torch.int32, index) and starts.shape == (batch,) and
-            starts.is_contiguous() and
-            ((batch and tokens % batch == 0) if cu is None else
-             _same(cu, torch.int32, index) and cu.shape == (batch + 1,) and cu.is_contiguous())):
-        _refuse_rows("k", k, dtype, heads, dim, index)
-        _refuse_rows("v", v, dtype, heads, dim, index)
-        _need(v.shape[0] == tokens, f"k has {tokens} tokens, v {v.shape[0]}")
-        _refuse_cache(cache, index)
-        _refuse_indices(table, (("starts", starts, batch),), cu, batch, tokens, index)
-    rot = rope_len = cos_at = sin_at = 0
-    if cos is not None or sin is not None:
-        _need(cos is not None and sin is not None, "pass both cos and sin, or neither")
-        if not (_same(cos, torch.float32, index) and _same(sin, torch.float32, index) and cos.dim() == 2 and
-                cos.shape == sin.shape and 2 * cos.shape[1] <= dim and cos.is_contiguous() and sin.is_contiguous()):
-            _refuse_tensor("cos", cos, (torch.float32,), index)
-            _refuse_tensor("sin", sin, (torch.float32,), index)
-            raise ValueError(f"cos, sin: expected two contiguous [positions, at most {dim // 2}], got {tuple(cos.shape)} and "
-                             f"{tuple(sin.shape)}")
-        rope_len, rot = cos.shape
-        rot *= 2
-        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
-    q_heads = q_at = out_at = sqt = sqh = 0
-    out = None
-    if q is not None:
-        if not (_same(q, dtype, index) and q.dim() == 3 and q.shape[2] == dim and q.shape[0] == tokens and q.stride(2) == 1):
-            _refuse_rows("q", q, dtype, None, dim, index)
-            raise ValueError(f"k has {tokens} tokens, q {q.shape[0]}")
-        q_heads = q.shape[1]
-        sqt, sqh, _ = q.stride()
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        q_at, out_at = q.data_ptr(), out.data_ptr()
-    lengths = torch.empty_like(starts)
-    skt, skh, _ = k.stride()
-    svt, svh, _ = v.stride()
-    _call("piton_b200_kv_append",
-          _pack_append(k.data_ptr(), v.data_ptr(), q_at, out_at, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-                       table.data_ptr(), starts.data_ptr(), 0 if cu is None else cu.data_ptr(), lengths.data_ptr(), cos_at,
-                       sin_at, batch, tokens, heads, q_heads, dim, page, pages, width, stride, skt, skh, svt, svh, sqt, sqh,
-                       q_heads * dim, dim, rot, rope_len, kind, 1 if interleaved else 0, 0, 0), index)
-    return out, lengths
+    args = (k, v, cache, table, starts, cu, cos, sin, interleaved, q)
+    result = (_bound or _calls()).kv_append(*args)
+    if result.__class__ is not tuple:
+        _failed("kv_append", result, _refuse_append, *args)
+    return result
 
 
 def kv_attention(q, cache, table, lengths, *, cu=None, scale: Optional[float] = None, window: int = 0,
@@ -230,42 +216,11 @@ def kv_attention(q, cache, table, lengths, *, cu=None, scale: Optional[float] = 
     lengths known to the host) and ``max_new`` (of the query tokens a sequence, with ``cu``) size the launch;
     by default the table's width and the number of tokens bound them.  With ``return_lse`` also the float32
     [tokens, heads] logarithms of the rows' sums of exponentials (-inf for rows that see no key)."""
-    kind = _type_of("q", q)
-    index = q.get_device()
-    kc, vc, ks, vs = cache
-    shape = kc.shape
-    if len(shape) != 4:
-        _refuse_cache(cache, index)
-    pages, kv_heads, page, dim = shape
-    batch, width, stride = _table(table, index)
-    if not (q.dim() == 3 and q.shape[2] == dim and q.stride(2) == 1 and
-            kc.dtype in _CODES and vc.dtype in _CODES and vc.shape == shape and ks.shape == shape[:2] == vs.shape and
-            _same(ks, torch.float32, index) and _same(vs, torch.float32, index) and kc.get_device() == index and
-            vc.get_device() == index and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and
-            vs.is_contiguous() and _same(lengths, torch.int32, index) and lengths.shape == (batch,) and
-            lengths.is_contiguous() and window >= 0 and max_length >= 0 and max_new >= 0 and
-            ((batch and q.shape[0] % batch == 0) if cu is None else
-             _same(cu, torch.int32, index) and cu.shape == (batch + 1,) and cu.is_contiguous())):
-        _refuse_rows("q", q, q.dtype, None, dim, index)
-        _refuse_cache(cache, index)
-        _refuse_indices(table, (("lengths", lengths, batch),), cu, batch, q.shape[0], index)
-        _need(window >= 0 and max_length >= 0 and max_new >= 0, "window, max_length and max_new must not be negative")
-    tokens, heads, _ = q.shape
-    sqt, sqh, _ = q.stride()
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    args = (q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(),
-            vs.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0 if cu is None else cu.data_ptr(),
-            dim ** -0.5 if scale is None else scale, batch, tokens, heads, kv_heads, dim, page, pages, width, stride, sqt, sqh,
-            heads * dim, dim, window, max_length, max_new)
-    packed = _pack_attention(*args, 0, 0, kind, 0)
-    need = (_ENTRY.get("piton_b200_kv_attention_workspace_size") or
-            _entry("piton_b200_kv_attention_workspace_size", C.c_size_t))(packed)
-    if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)   # of this call's stream, so calls never share it
-        packed = _pack_attention(*args, scratch.data_ptr(), need, kind, 0)
-    _call("piton_b200_kv_attention", packed, index)
-    return (out, lse) if return_lse else out
+    args = (q, cache, table, lengths, cu, scale, window, max_length, max_new, return_lse)
+    result = (_bound or _calls()).kv_attention(*args)
+    if result is None or result.__class__ is int:
+        _failed("kv_attention", result, _refuse_attention, *args)
+    return result
 
 
 def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
@@ -276,44 +231,10 @@ def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
     the same shape, the low four bits count; zero point 8 without) per group of 32, 64 or 128: W = scale * (code - zero).  ``bias``
     [outer] of x's type.  Rows of every operand may be strided.  Accumulates in 32 bits, returns x's type.
     Meant for few rows: the weights are read again for every 16."""
-    kind = _type_of("x", x)
-    index, dtype = x.get_device(), x.dtype
-    flat = x.dim() == 1
-    if x.dim() not in (1, 2):
-        raise ValueError(f"x: shape {tuple(x.shape)}, expected [rows, inner] or [inner]")
-    inner = x.shape[-1]
-    if group not in (32, 64, 128):
-        raise NotImplementedError(f"group {group}: 32, 64 or 128")
-    if not isinstance(codes, torch.Tensor) or codes.dim() != 2:
-        _refuse_tensor("codes", codes, (torch.uint8,), index)
-        raise ValueError(f"codes: shape {tuple(codes.shape)}, expected [outer, {(inner + 1) // 2}]")
-    outer, groups = codes.shape[0], -(-inner // group)
-    shape = (outer, groups)
-    if not (_same(codes, torch.uint8, index) and codes.shape[1] == (inner + 1) // 2 and
-            (codes.stride(1) == 1 or codes.shape[1] <= 1) and (x.stride(-1) == 1 or inner <= 1) and
-            scales.dtype in _TYPES and scales.get_device() == index and scales.shape == shape and
-            (groups <= 1 or scales.stride(1) == 1) and
-            (zeros is None or (_same(zeros, torch.uint8, index) and zeros.shape == shape and
-                               (groups <= 1 or zeros.stride(1) == 1))) and
-            (bias is None or (_same(bias, dtype, index) and bias.shape == (outer,) and (outer <= 1 or bias.stride(0) == 1)))):
-        _refuse_tensor("codes", codes, (torch.uint8,), index)
-        _refuse_tensor("scales", scales, tuple(_TYPES), index)
-        if zeros is not None:
-            _refuse_tensor("zeros", zeros, (torch.uint8,), index)
-        if bias is not None:
-            _refuse_tensor("bias", bias, (dtype,), index)
-        raise ValueError(f"x {tuple(x.shape)}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}, zeros "
-                         f"{None if zeros is None else tuple(zeros.shape)}, bias {None if bias is None else tuple(bias.shape)}: "
-                         f"expected codes [{outer}, {(inner + 1) // 2}], scales and zeros {list(shape)}, bias [{outer}], each with "
-                         f"unit stride in its last dimension")
-    rows = 1 if flat else x.shape[0]
-    y = x.new_empty(outer if flat else (rows, outer))
-    _call("piton_b200_matvec_w4",
-          _pack_matvec(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
-                       0 if bias is None else bias.data_ptr(), y.data_ptr(), rows, inner, outer, 0 if flat else x.stride(0),
-                       codes.stride(0), scales.stride(0), 0 if zeros is None else zeros.stride(0), outer, group, kind,
-                       _TYPES[scales.dtype], 0), index)
-    return y
+    result = (_bound or _calls()).matvec_w4(x, codes, scales, group, zeros, bias)
+    if result is None or result.__class__ is int:
+        _failed("matvec_w4", result, _refuse_matvec, x, codes, scales, group, zeros, bias)
+    return result
 
 
 def quantize_w4(weight, group: int = 128, zeros: bool = True, dtype=None):
