@@ -60,15 +60,16 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-// `count` bytes of the 16, one by one and at any alignment; the rest becomes 0.
-__device__ __forceinline__ void copy16_slow(uint32_t dst, const uint8_t *src, int count) {
-#pragma unroll 1
-    for (int w = 0; w < 4; ++w) {
-        uint32_t word = 0;
-        for (int i = 0; i < 4; ++i)
-            if (4 * w + i < count) word |= (uint32_t)src[4 * w + i] << (8 * i);
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 4 * w), "r"(word) : "memory");
-    }
+// The larger magnitude; NaN if one is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
+    return d;
+}
+// Byte `i` of four words.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
+    const uint32_t two = 0x40 + 0x11 * i;                               // byte i of the first, then of the second
+    return __byte_perm(__byte_perm(a, b, two), __byte_perm(c, d, two), 0x5410);
 }
 __device__ __forceinline__ uint4 load16(uint32_t at) {
     uint4 v;
@@ -149,14 +150,21 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                     if (R > 1 || r < rows) copy4(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src);
                     src += p.sc;
                 }
-            } else {                                                    // the last step, or rows that are not aligned
-                const int left = (p.inner + 1) / 2 - (step0 + own0 + issued * STRIDE) * LINE - 16 * (lane & 7);
-#pragma unroll 1
-                for (int r = lane >> 3; r < rows; r += 4) {
-                    const uint32_t dst = fill + 128 * r + ((lane & 7) ^ (r & 7)) * 16;
-                    const uint8_t *src = codes + r * p.sc + 16 * (lane & 7);
-                    if (p.codes_align == 16 && left >= 16) copy16(dst, src);
-                    else copy16_slow(dst, src, left);
+            } else {                                                    // the last step, or rows that are not aligned: word by word
+                const int left = (p.inner + 1) / 2 - (step0 + own0 + issued * STRIDE) * LINE - 4 * lane;
+                const uint8_t *src = codes + 4 * lane;
+#pragma unroll 4
+                for (int r = 0; r < rows; ++r) {
+                    const uint32_t dst = fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3);
+                    if (p.codes_align >= 4 && left >= 4) {
+                        copy4(dst, src);
+                    } else if (left > 0) {                              // (past the row's end x is 0, whatever the slot holds)
+                        uint32_t word = src[0];
+#pragma unroll
+                        for (int i = 1; i < 4; ++i) word |= (left > i ? (uint32_t)src[i] : 0u) << (8 * i);
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(word) : "memory");
+                    }
+                    src += p.sc;
                 }
             }
             codes += STRIDE * LINE;
@@ -226,28 +234,30 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
             }
             float f[8], top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                f[i] = to_float(v[i]);
-                top = fmaxf(top, isfinite(f[i]) ? fabsf(f[i]) : INFINITY);
-            }
+            for (int i = 0; i < 8; ++i) f[i] = to_float(v[i]), top = max_abs(top, f[i]);
 #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = 1; o < 16; o <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
             // the largest magnitude becomes 127 in the first digit and 0 in the others
             constexpr float LIMIT = DIGITS == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
             const bool finite = top < INFINITY;
             const float up = !finite ? 0.0f : fminf(LIMIT / fmaxf(top, 1e-37f), 8.5070592e37f), down = !finite ? __int_as_float(0x7FC00000) : 1.0f / up;
-            uint32_t digit[3][2] = {};
-            int32_t sum = 0;
+            // with 128 added to every digit but the first the digits are the bytes of the sum, those less 128 of them signed
+            uint32_t t[8], digit[3][2] = {};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                int32_t q = finite ? __float2int_rn(f[i] * up) : 0;
-                sum += q;
+                if constexpr (DIGITS == 3) t[i] = (uint32_t)(finite ? __float2int_rn(f[i] * up) + 0x8080 : 0x8080);
+                else t[i] = finite ? __float_as_uint(fmaf(f[i], up, 12582912.0f + 128.0f)) : 0x80u;
+            }
+            int32_t sum = 0;
 #pragma unroll
-                for (int d = DIGITS - 1; d >= 0; --d) {
-                    const int32_t low = d ? (int32_t)(int8_t)q : q;     // the remainder in -128 ... 127
-                    q = (q - low) >> 8;
-                    digit[d][i & 1] |= (uint32_t)(low & 255) << (8 * (i >> 1));
+            for (int d = 0; d < DIGITS; ++d) {
+                int32_t own = 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {                           // elements 0, 2, 4, 6 and 1, 3, 5, 7
+                    digit[d][h] = bytes_of(t[h], t[2 + h], t[4 + h], t[6 + h], DIGITS - 1 - d) ^ (d ? 0x80808080u : 0u);
+                    own = __dp4a((int)digit[d][h], 0x01010101, own);
                 }
+                sum = 256 * sum + own;
             }
 #pragma unroll
             for (int o = 1; o < 4 * WORDS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);    // a group's units: below 2^30
