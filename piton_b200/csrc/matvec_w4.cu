@@ -48,10 +48,14 @@ __device__ __forceinline__ float value_of(int32_t v) { return __int_as_float(v) 
 
 // d = a b + d, or a b + MAGIC.
 template <bool FIRST> __device__ __forceinline__ void mma(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    const int32_t c[4] = {FIRST ? MAGIC : d[0], FIRST ? MAGIC : d[1], FIRST ? MAGIC : d[2], FIRST ? MAGIC : d[3]};
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(MAGIC));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
@@ -94,7 +98,7 @@ template <typename T, int NT, int R, int GROUPS> struct Shape {
     static constexpr int SUMS = 8 * NT * 16 * R;                        // outputs of a warp's tile
     // x in shared memory, per row: 16 bytes for every 8 elements (their first two digits), 8 more for fp32 (the third), and per
     // block a scale and each group's sum; paddings put rows that are read together into different banks
-    static constexpr int META = 1 + GROUPS;                             // words of a block
+    static constexpr int META = 2 * GROUPS;                             // words of a block: 1 + GROUPS, in whole loads
     __host__ __device__ static constexpr int pitch(int steps) { return steps * 512 + 64; }
     __host__ __device__ static constexpr int pitch3(int steps) { return DIGITS == 3 ? steps * 256 + 32 : 0; }
     // shared memory: queues (in the end the warps' sums), x
@@ -272,14 +276,14 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     };
     // rows of x past the last read the last: a column of the product depends on its own row alone
     uint32_t x_at[NT], x3_at[NT];
-    const float *meta_at[NT][2];
+    uint32_t meta_at[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int m = min(8 * t + g, x_rows - 1);
         x_at[t] = (uint32_t)__cvta_generic_to_shared(xs) + m * S::pitch(p.phase) + 16 * j;
         x3_at[t] = (uint32_t)__cvta_generic_to_shared(x3) + m * S::pitch3(p.phase) + 8 * j;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) meta_at[t][e] = meta + min(8 * t + 2 * j + e, x_rows - 1) * (2 * p.phase * S::META);
+        for (int e = 0; e < 2; ++e) meta_at[t][e] = (uint32_t)__cvta_generic_to_shared(meta + min(8 * t + 2 * j + e, x_rows - 1) * (2 * p.phase * S::META));
     }
 
     float acc[R][NT][4];
@@ -321,19 +325,23 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
             __syncwarp();                                               // every lane's copies, and the slot that is filled next has been read
             issue();
             const int b0 = 2 * (own0 + turn * STRIDE - phase0);         // block of the phase
-            const uint32_t wat = slot + row * LINE;
+            const uint32_t wat = slot + row * LINE + (((WORDS * j >> 2) ^ (row & 7)) * 16) + (4 * WORDS * j & 15);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                float back[NT][2];
+                uint32_t about[NT][2][S::META];                         // the block's scale, then its groups' sums
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) back[t][e] = meta_at[t][e][(b0 + b) * S::META];
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t from = meta_at[t][e] + (b0 + b) * (4 * S::META);
+                        if constexpr (GROUPS == 1) load_words<2>(about[t][e], from);
+                        else load_words<4>(*reinterpret_cast<uint32_t(*)[4]>(about[t][e]), from);
+                        if constexpr (GROUPS == 4) load_words<1>(*reinterpret_cast<uint32_t(*)[1]>(about[t][e] + 4), from + 16);
+                    }
 #pragma unroll
                 for (int q = 0; q < GROUPS; ++q) {
                     uint4 x12[NT][WORDS];
                     uint2 x3v[NT][WORDS];
-                    float x_sum[NT][2];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -344,8 +352,6 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                                 asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x3v[t][i].x), "=r"(x3v[t][i].y)
                                              : "r"(x3_at[t] + (b0 + b) * 128 + (q * WORDS + i) * 32) : "memory");
                         }
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) x_sum[t][e] = meta_at[t][e][(b0 + b) * S::META + 1 + q];
                     }
                     constexpr int LAST = LOADS - 1;
                     const int load = GROUPS == 4 ? b & LAST : 0;
@@ -360,8 +366,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                             s2[h] = __uint_as_float(__shfl_sync(0xffffffffu, scale[load][2 * r + h], from));
                             z2[h] = value_of(MAGIC | (z >> (8 * r + 4 * h) & 15));
                             // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of row 16 r + row + 8 h
-                            const int piece = 4 * b + WORDS * q + (WORDS * j >> 2);
-                            load_words(w[h], wat + (16 * r + 8 * h) * LINE + ((piece ^ (row & 7)) * 16) + (4 * WORDS * j & 15));
+                            load_words(w[h], (wat ^ (64 * b + 16 * WORDS * q)) + (16 * r + 8 * h) * LINE);
                         }
                         int32_t sum[NT][DIGITS][4];
 #pragma unroll
@@ -385,8 +390,8 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                                 float v = value_of(sum[t][0][e]);
 #pragma unroll
                                 for (int d = 1; d < DIGITS; ++d) v = fmaf(v, 256.0f, value_of(sum[t][d][e]));
-                                v = fmaf(-z2[e >> 1], x_sum[t][e & 1], v);
-                                acc[r][t][e] = fmaf(v, back[t][e & 1] * s2[e >> 1], acc[r][t][e]);
+                                v = fmaf(-z2[e >> 1], __uint_as_float(about[t][e & 1][1 + q]), v);
+                                acc[r][t][e] = fmaf(v, __uint_as_float(about[t][e & 1][0]) * s2[e >> 1], acc[r][t][e]);
                             }
                     }
                 }
@@ -420,10 +425,10 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     // CTA `part` stores its share of the outputs
     const int outputs = TILES * x_rows * (16 * R), share = (outputs + parts - 1) / parts;
     for (int i = part * share + threadIdx.x; i < min((part + 1) * share, outputs); i += THREADS) {
-        const int n = i % (16 * R), m = i / (16 * R) % x_rows, w = i / (16 * R * x_rows);
-        const int64_t t = (int64_t)(blockIdx.x / parts) * TILES + w;
-        if (t * (16 * R) >= p.outer) continue;
-        const int64_t at = min(t * (16 * R), max(p.outer - 16 * R, (int64_t)0)) + n;
+        const uint32_t n = i % (16 * R), y = i / (16 * R), m = y % (uint32_t)x_rows, w = y / (uint32_t)x_rows;
+        const int64_t first_row = ((int64_t)(blockIdx.x / parts) * TILES + w) * (16 * R);
+        if (first_row >= p.outer) continue;
+        const int64_t at = min(first_row, max(p.outer - 16 * R, (int64_t)0)) + n;
         if (at >= p.outer) continue;
         float sum = 0.0f;
         float *from = sums + w * S::SUMS + m * (16 * R) + n;
@@ -476,7 +481,7 @@ template <typename T, int NT, int R, bool ALONG_K> int launch(const MatvecParams
 
 template <typename T, int NT> int launch(MatvecParams p, cudaStream_t s) {
     const int64_t tiles = cdiv(p.outer, 16), sms = num_sms(), steps = cdiv(p.inner, 2 * BLOCK);
-    const int64_t most = steps < MAX_PARTS ? steps : MAX_PARTS;
+    const int64_t most = steps < MAX_PARTS ? steps : MAX_PARTS;      // powers of two: clusters of 7 took longer than of 4
     // Warps along the rows from 2 x 148 tiles of 16 weight rows on, in as many parts of the inner dimension as two CTAs an SM
     // take in one wave (28000 x 8192, bf16, one row: 2 parts 29.4 us, 1 part 36.6, 4 parts 32.2; warps along the inner
     // dimension 40); below that along the inner dimension (4096 x 4096: 6.2 us, along the rows 6.2 to 9), split
@@ -484,8 +489,7 @@ template <typename T, int NT> int launch(MatvecParams p, cudaStream_t s) {
     int64_t parts = 1;
     if (tiles >= 2 * sms) {
         const int64_t groups = cdiv(tiles, 2 * WARPS);
-        parts = 2 * sms / groups;
-        parts = parts > most ? most : parts < 1 ? 1 : parts;
+        while (2 * parts <= most && groups * 2 * parts <= 2 * sms) parts *= 2;
         return launch<T, NT, 2, false>(p, (int)parts, s);
     }
     while (2 * parts <= most && tiles * 2 * parts <= 2 * sms && steps >= WARPS * 2 * parts) parts *= 2;
