@@ -423,9 +423,12 @@ typedef struct {
     uint64_t x, codes, scales, zeros, bias, y;
     int64_t rows, inner, outer;
     int64_t stride_x, stride_codes, stride_scales, stride_zeros, stride_y;
+    uint64_t workspace;         /* device scratch of piton_b200_matvec_w4_workspace_size() bytes (may be 0), 16-byte aligned */
+    uint64_t workspace_bytes;
     int32_t group, type, scale_type;
     uint32_t flags;             /* 0 */
 } piton_matvec_w4_args;
+PITON_B200_API size_t piton_b200_matvec_w4_workspace_size(const piton_matvec_w4_args *args);
 PITON_B200_API int piton_b200_matvec_w4(const piton_matvec_w4_args *args, void *stream);
 
 #ifdef __cplusplus

@@ -23,6 +23,7 @@ int (*append_entry)(const piton_kv_append_args *, void *);
 int (*attention_entry)(const piton_kv_attention_args *, void *);
 size_t (*attention_workspace)(const piton_kv_attention_args *);
 int (*matvec_entry)(const piton_matvec_w4_args *, void *);
+size_t (*matvec_workspace)(const piton_matvec_w4_args *);
 PyObject *out_of_memory;      // torch.OutOfMemoryError
 
 const at::Tensor *tensor(PyObject *o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -222,22 +223,27 @@ PyObject *matvec_w4(PyObject *, PyObject *const *o, Py_ssize_t n) {
         a.stride_x = flat ? 0 : x->stride(0), a.stride_codes = codes->stride(0), a.stride_scales = scales->stride(0);
         a.stride_zeros = zeros ? zeros->stride(0) : 0, a.stride_y = outer;
         a.group = (int32_t)group, a.type = type_of(*x), a.scale_type = type_of(*scales);
+        at::Tensor scratch;
+        if (const size_t need = matvec_workspace(&a)) {
+            scratch = empty({(int64_t)need}, at::kByte, *x);
+            a.workspace = address(scratch), a.workspace_bytes = need;
+        }
         if (const int rc = enter(matvec_entry, a, device)) return PyLong_FromLong(rc);
         return wrap(std::move(y));
     });
 }
 
-// bind(addresses of kv_append, kv_attention, kv_attention_workspace_size and matvec_w4 in the library that the package has
-// loaded, torch.OutOfMemoryError).
+// bind(addresses of the entry points in the library that the package has loaded, in the order below, torch.OutOfMemoryError).
 PyObject *bind(PyObject *, PyObject *args) {
-    unsigned long long f[4];
+    unsigned long long f[5];
     PyObject *oom;
-    if (!PyArg_ParseTuple(args, "KKKKO", &f[0], &f[1], &f[2], &f[3], &oom)) return nullptr;
+    if (!PyArg_ParseTuple(args, "KKKKKO", &f[0], &f[1], &f[2], &f[3], &f[4], &oom)) return nullptr;
     Py_XSETREF(out_of_memory, Py_NewRef(oom));
     append_entry = reinterpret_cast<decltype(append_entry)>(f[0]);
     attention_entry = reinterpret_cast<decltype(attention_entry)>(f[1]);
     attention_workspace = reinterpret_cast<decltype(attention_workspace)>(f[2]);
-    matvec_entry = reinterpret_cast<decltype(matvec_entry)>(f[3]);
+    matvec_workspace = reinterpret_cast<decltype(matvec_workspace)>(f[3]);
+    matvec_entry = reinterpret_cast<decltype(matvec_entry)>(f[4]);
     Py_RETURN_NONE;
 }
 

@@ -39,6 +39,7 @@ struct MatvecParams {
     void *y;
     int64_t rows, outer, sx, sc, ss, sz, sy;
     int32_t inner, group_log2, scale_type, codes_align, x_aligned;
+    uint8_t *digits;                        // x laid out in the workspace, or null: every CTA lays out what it needs
     int32_t span, phase;                    // steps of a CTA's part, and of what shared memory holds of x at a time
 };
 
@@ -107,6 +108,89 @@ template <typename T, int NT, int R, int GROUPS> struct Shape {
         return QUEUES + rows * (steps * (512 + (DIGITS == 3 ? 256 : 0) + 2 * META * 4) + 96);
     }
 };
+
+// Where x is laid out: rows of 512 bytes a step (two blocks) of the first two digits, of 256 of the third (fp32), and of META
+// words a block.
+struct Layout {
+    uint8_t *x, *x3;
+    float *meta;
+    int64_t pitch, pitch3, meta_pitch;
+};
+// Where the workspace holds all steps of all rows.
+template <typename S> __host__ __device__ Layout whole_layout(uint8_t *at, int64_t rows, int64_t steps) {
+    Layout l;
+    l.pitch = steps * 512, l.pitch3 = S::DIGITS == 3 ? steps * 256 : 0, l.meta_pitch = steps * 2 * S::META;
+    l.x = at, l.x3 = at + rows * l.pitch, l.meta = reinterpret_cast<float *>(l.x3 + rows * l.pitch3);
+    return l;
+}
+
+// Lays out `steps` steps from step0 on of the rows m0 ...: per row and block 16 units of 8 elements, unit 4 c + j for word c of lane
+// j (word w of group q: c = q WORDS + w), which faces elements 32 WORDS q + 8 WORDS j + 8 w ... of the block. A unit's bytes are
+// its elements 0, 2, 4, 6 (the low nibbles of the word) and 1, 3, 5, 7.
+template <typename T, typename S>
+__device__ __forceinline__ void lay_out(const MatvecParams &p, int64_t m0, int x_rows, int step0, int steps, const Layout &to) {
+    constexpr int WORDS = S::WORDS, DIGITS = S::DIGITS;
+    const int count = 2 * steps, units = x_rows * count * 16;
+            for (int u0 = 0; u0 < units; u0 += THREADS) {
+                const int u = u0 + threadIdx.x, unit = u & 15, c = unit >> 2, b = (u >> 4) % count, m = (u >> 4) / count;
+                const int k = (2 * step0 + b) * BLOCK + c / WORDS * (32 * WORDS) + 8 * WORDS * (unit & 3) + 8 * (c % WORDS);
+                const bool in = u < units;
+                const T *src = reinterpret_cast<const T *>(p.x) + (m0 + (in ? m : 0)) * p.sx + k;
+                T v[8];
+                if (in && k + 8 <= p.inner && p.x_aligned) {
+    #pragma unroll
+                    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(src)[i];
+                } else {
+    #pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = in && k + i < p.inner ? src[i] : from_float<T>(0.0f);
+                }
+                float f[8], top = 0.0f;
+    #pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = to_float(v[i]), top = max_abs(top, f[i]);
+    #pragma unroll
+                for (int o = 1; o < 16; o <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
+                // the largest magnitude becomes 127 in the first digit and 0 in the others
+                constexpr float LIMIT = DIGITS == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
+                const bool finite = top < INFINITY;
+                const float up = !finite ? 0.0f : fminf(LIMIT / fmaxf(top, 1e-37f), 8.5070592e37f), down = !finite ? __int_as_float(0x7FC00000) : 1.0f / up;
+                // with 128 added to every digit but the first the digits are the bytes of the sum, those less 128 of them signed
+                uint32_t t[8], digit[3][2] = {};
+    #pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if constexpr (DIGITS == 3) t[i] = (uint32_t)(finite ? __float2int_rn(f[i] * up) + 0x8080 : 0x8080);
+                    else t[i] = finite ? __float_as_uint(fmaf(f[i], up, 12582912.0f + 128.0f)) : 0x80u;
+                }
+                int32_t sum = 0;
+    #pragma unroll
+                for (int d = 0; d < DIGITS; ++d) {
+                    int32_t own = 0;
+    #pragma unroll
+                    for (int h = 0; h < 2; ++h) {                           // elements 0, 2, 4, 6 and 1, 3, 5, 7
+                        digit[d][h] = bytes_of(t[h], t[2 + h], t[4 + h], t[6 + h], DIGITS - 1 - d) ^ (d ? 0x80808080u : 0u);
+                        own = __dp4a((int)digit[d][h], 0x01010101, own);
+                    }
+                    sum = 256 * sum + own;
+                }
+    #pragma unroll
+                for (int o = 1; o < 4 * WORDS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);    // a group's units: below 2^30
+                if (in) {
+                    *reinterpret_cast<uint4 *>(to.x + m * to.pitch + (b * 16 + unit) * 16) = make_uint4(digit[0][0], digit[0][1], digit[1][0], digit[1][1]);
+                    if constexpr (DIGITS == 3) *reinterpret_cast<uint2 *>(to.x3 + m * to.pitch3 + (b * 16 + unit) * 8) = make_uint2(digit[2][0], digit[2][1]);
+                    float *about = to.meta + m * to.meta_pitch + b * S::META;
+                    if (unit == 0) about[0] = down;
+                    if (unit % (4 * WORDS) == 0) about[1 + unit / (4 * WORDS)] = (float)sum;
+                }
+            }
+}
+
+// x laid out once for all CTAs, which would otherwise repeat it for every 256 weight rows: a thread a unit.
+template <typename T, typename S> __global__ void __launch_bounds__(THREADS) matvec_w4_digits_kernel(const MatvecParams p, int all_steps) {
+    asm volatile("griddepcontrol.launch_dependents;");              // the product may start on its weights, and waits before it reads x
+    const int step = blockIdx.x * 8, m = blockIdx.y;
+    Layout to = whole_layout<S>(p.digits, p.rows, all_steps);
+    to.x += m * to.pitch + step * 512, to.x3 += m * to.pitch3 + step * 256, to.meta += m * to.meta_pitch + step * 2 * S::META;
+    lay_out<T, S>(p, m, 1, step, min(8, all_steps - step), to);
+}
 
 // ALONG_K: the CTA's warps share 16 R weight rows and split the inner dimension; otherwise each has rows of its own.
 template <typename T, int NT, int R, int GROUPS, bool ALONG_K>
@@ -218,62 +302,6 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     uint8_t *xs = queue + S::QUEUES;
     uint8_t *x3 = xs + x_rows * S::pitch(p.phase);
     float *meta = reinterpret_cast<float *>(x3 + x_rows * S::pitch3(p.phase));      // [x row][block of the phase][META]
-    // Lays out steps phase0 ... of the part: per row and block 16 units of 8 elements, unit 4 c + j for word c of lane j (word w
-    // of group q: c = q WORDS + w), which faces elements 32 WORDS q + 8 WORDS j + 8 w ... of the block. A unit's bytes
-    // are its elements 0, 2, 4, 6 (the low nibbles of the word) and 1, 3, 5, 7.
-    auto lay_out = [&](int phase0) {
-        const int count = 2 * min(p.phase, steps - phase0), units = x_rows * count * 16;
-        for (int u0 = 0; u0 < units; u0 += THREADS) {
-            const int u = u0 + threadIdx.x, unit = u & 15, c = unit >> 2, b = (u >> 4) % count, m = (u >> 4) / count;
-            const int k = (2 * (step0 + phase0) + b) * BLOCK + c / WORDS * (32 * WORDS) + 8 * WORDS * (unit & 3) + 8 * (c % WORDS);
-            const bool in = u < units;
-            const T *src = reinterpret_cast<const T *>(p.x) + (m0 + (in ? m : 0)) * p.sx + k;
-            T v[8];
-            if (in && k + 8 <= p.inner && p.x_aligned) {
-#pragma unroll
-                for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(src)[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = in && k + i < p.inner ? src[i] : from_float<T>(0.0f);
-            }
-            float f[8], top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = to_float(v[i]), top = max_abs(top, f[i]);
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
-            // the largest magnitude becomes 127 in the first digit and 0 in the others
-            constexpr float LIMIT = DIGITS == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
-            const bool finite = top < INFINITY;
-            const float up = !finite ? 0.0f : fminf(LIMIT / fmaxf(top, 1e-37f), 8.5070592e37f), down = !finite ? __int_as_float(0x7FC00000) : 1.0f / up;
-            // with 128 added to every digit but the first the digits are the bytes of the sum, those less 128 of them signed
-            uint32_t t[8], digit[3][2] = {};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (DIGITS == 3) t[i] = (uint32_t)(finite ? __float2int_rn(f[i] * up) + 0x8080 : 0x8080);
-                else t[i] = finite ? __float_as_uint(fmaf(f[i], up, 12582912.0f + 128.0f)) : 0x80u;
-            }
-            int32_t sum = 0;
-#pragma unroll
-            for (int d = 0; d < DIGITS; ++d) {
-                int32_t own = 0;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {                           // elements 0, 2, 4, 6 and 1, 3, 5, 7
-                    digit[d][h] = bytes_of(t[h], t[2 + h], t[4 + h], t[6 + h], DIGITS - 1 - d) ^ (d ? 0x80808080u : 0u);
-                    own = __dp4a((int)digit[d][h], 0x01010101, own);
-                }
-                sum = 256 * sum + own;
-            }
-#pragma unroll
-            for (int o = 1; o < 4 * WORDS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);    // a group's units: below 2^30
-            if (in) {
-                *reinterpret_cast<uint4 *>(xs + m * S::pitch(p.phase) + (b * 16 + unit) * 16) = make_uint4(digit[0][0], digit[0][1], digit[1][0], digit[1][1]);
-                if constexpr (DIGITS == 3) *reinterpret_cast<uint2 *>(x3 + m * S::pitch3(p.phase) + (b * 16 + unit) * 8) = make_uint2(digit[2][0], digit[2][1]);
-                float *to = meta + (m * 2 * p.phase + b) * S::META;
-                if (unit == 0) to[0] = down;
-                if (unit % (4 * WORDS) == 0) to[1 + unit / (4 * WORDS)] = (float)sum;
-            }
-        }
-    };
     // rows of x past the last read the last: a column of the product depends on its own row alone
     uint32_t x_at[NT], x3_at[NT];
     uint32_t meta_at[NT][2];
@@ -299,9 +327,26 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 #pragma unroll 1
     for (int phase0 = 0; phase0 < steps; phase0 += p.phase) {
         if (phase0) __syncthreads();                                    // the last phase's x has been read
-        lay_out(phase0);
+        const int count = min(p.phase, steps - phase0);
+        if (p.digits) {                                                 // 16 bytes at a time, as they lie in the workspace
+            const Layout from = whole_layout<S>(p.digits, p.rows, (p.inner + STEP - 1) / STEP);
+            if (phase0 == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+            auto copy = [&](uint8_t *to, int to_pitch, const uint8_t *src, int64_t src_pitch, int row_bytes) {
+                for (int m = warp; m < x_rows; m += WARPS)
+#pragma unroll 4
+                    for (int i = 16 * lane; i < row_bytes; i += 512) copy16((uint32_t)__cvta_generic_to_shared(to + m * to_pitch + i), src + (m0 + m) * src_pitch + i);
+            };
+            const int64_t at = step0 + phase0;
+            copy(xs, S::pitch(p.phase), from.x + at * 512, from.pitch, count * 512);
+            if constexpr (DIGITS == 3) copy(x3, S::pitch3(p.phase), from.x3 + at * 256, from.pitch3, count * 256);
+            copy(reinterpret_cast<uint8_t *>(meta), 8 * S::META * p.phase, reinterpret_cast<const uint8_t *>(from.meta + at * 2 * S::META), 4 * from.meta_pitch,
+                 count * 8 * S::META);
+            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+        } else {
+            lay_out<T, S>(p, m0, x_rows, step0 + phase0, count, {xs, x3, meta, S::pitch(p.phase), S::pitch3(p.phase), 2 * p.phase * S::META});
+        }
         __syncthreads();
-        const int phase_end = min(phase0 + p.phase, steps);
+        const int phase_end = phase0 + count;
 #pragma unroll 1
         for (; own0 + turn * STRIDE < phase_end; ++turn) {
             if (AHEAD == 1 || !(turn & 1)) {
@@ -444,66 +489,86 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     if (parts > 1) cluster.sync();                                      // shared memory stays until the others have read it
 }
 
-template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(MatvecParams p, int parts, cudaStream_t s) {
+// How a call is cut (made of the sizes alone, so that the workspace's size is known before).
+struct Plan {
+    bool along_k;
+    int parts;
+    size_t digits;                          // bytes of x laid out in the workspace, 0: in every CTA
+};
+
+template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(MatvecParams p, const Plan &plan, cudaStream_t s) {
     using S = Shape<T, NT, R, GROUPS>;
     const int64_t x_rows = p.rows < 8 * NT ? p.rows : 8 * NT;
-    p.span = (int32_t)cdiv(cdiv(p.inner, 2 * BLOCK), parts);
+    const int all_steps = (int)cdiv(p.inner, 2 * BLOCK);
+    p.span = (int32_t)cdiv(all_steps, plan.parts);
     // x whole, or as many of its steps as leave room for a second CTA
     p.phase = p.span > 0 ? p.span : 1;
     while (S::smem(x_rows, p.phase) > 113 * 1024 && p.phase > 1) p.phase = (p.phase + 1) / 2;
     static bool known[64];
-    int dev = 0;
+    int dev = 0, launches = 1;
     PITON_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !known[dev]) {
         PITON_CUDA(cudaFuncSetAttribute(matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
         if (dev >= 0 && dev < 64) known[dev] = true;
     }
+    if (plan.digits) {
+        matvec_w4_digits_kernel<T, S><<<dim3((unsigned)cdiv(all_steps, 8), (unsigned)p.rows), THREADS, 0, s>>>(p, all_steps);
+        launches = 2;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(cdiv(p.outer, ALONG_K ? 16 * R : 16 * R * WARPS) * parts), (unsigned)cdiv(p.rows, 8 * NT));
+    cfg.gridDim = dim3((unsigned)(cdiv(p.outer, ALONG_K ? 16 * R : 16 * R * WARPS) * plan.parts), (unsigned)cdiv(p.rows, 8 * NT));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = (size_t)S::smem(x_rows, p.phase);
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)parts;
+    at[0].val.clusterDim.x = (unsigned)plan.parts;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = plan.digits ? 2 : 1;
     PITON_CUDA(cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K>, p));
-    return check_launch("matvec_w4");
+    return check_launch("matvec_w4", launches);
 }
 
-template <typename T, int NT, int R, bool ALONG_K> int launch(const MatvecParams &p, int parts, cudaStream_t s) {
-    return p.group_log2 == 7 ? launch<T, NT, R, 1, ALONG_K>(p, parts, s)
-           : p.group_log2 == 6 ? launch<T, NT, R, 2, ALONG_K>(p, parts, s) : launch<T, NT, R, 4, ALONG_K>(p, parts, s);
+template <typename T, int NT, int R, bool ALONG_K> int launch(const MatvecParams &p, const Plan &plan, cudaStream_t s) {
+    return p.group_log2 == 7 ? launch<T, NT, R, 1, ALONG_K>(p, plan, s)
+           : p.group_log2 == 6 ? launch<T, NT, R, 2, ALONG_K>(p, plan, s) : launch<T, NT, R, 4, ALONG_K>(p, plan, s);
 }
 
-template <typename T, int NT> int launch(MatvecParams p, cudaStream_t s) {
-    const int64_t tiles = cdiv(p.outer, 16), sms = num_sms(), steps = cdiv(p.inner, 2 * BLOCK);
-    const int64_t most = steps < MAX_PARTS ? steps : MAX_PARTS;      // powers of two: clusters of 7 took longer than of 4
+template <typename T, int NT> int launch(const MatvecParams &p, const Plan &plan, cudaStream_t s) {
+    return plan.along_k ? launch<T, NT, 1, true>(p, plan, s) : launch<T, NT, 2, false>(p, plan, s);
+}
+
+Plan plan_of(const piton_matvec_w4_args *a) {
+    Plan plan = {true, 1, 0};
+    const int64_t tiles = cdiv(a->outer, 16), sms = num_sms(), steps = cdiv(a->inner, 2 * BLOCK);
+    const int64_t most = steps < MAX_PARTS ? steps : MAX_PARTS;
+    int64_t parts = 1;                      // a power of two: clusters of 7 took longer than of 4
     // Warps along the rows from 2 x 148 tiles of 16 weight rows on, in as many parts of the inner dimension as two CTAs an SM
     // take in one wave (28000 x 8192, bf16, one row: 2 parts 29.4 us, 1 part 36.6, 4 parts 32.2; warps along the inner
     // dimension 40); below that along the inner dimension (4096 x 4096: 6.2 us, along the rows 6.2 to 9), split
     // further only while SMs are idle and every warp keeps two steps (1024 x 8192: 4 parts 5.5 us, 1 part 7.8).
-    int64_t parts = 1;
     if (tiles >= 2 * sms) {
+        plan.along_k = false;
         const int64_t groups = cdiv(tiles, 2 * WARPS);
         while (2 * parts <= most && groups * 2 * parts <= 2 * sms) parts *= 2;
-        return launch<T, NT, 2, false>(p, (int)parts, s);
+    } else {
+        while (2 * parts <= most && tiles * 2 * parts <= 2 * sms && steps >= WARPS * 2 * parts) parts *= 2;
     }
-    while (2 * parts <= most && tiles * 2 * parts <= 2 * sms && steps >= WARPS * 2 * parts) parts *= 2;
-    return launch<T, NT, 1, true>(p, (int)parts, s);
+    plan.parts = (int)parts;
+    // More than 8192 elements of x a CTA are laid out once in the workspace by a kernel of their own
+    const int64_t x_rows = a->rows < 16 ? a->rows : 16;
+    if (x_rows * cdiv(steps, parts) * 2 * BLOCK > 8192) {
+        const int64_t fp32 = a->type == PITON_B200_TYPE_F32;
+        plan.digits = (size_t)(a->rows * steps) * (512 + (fp32 ? 256 : 0) + 2 * 4 * 2 * (128 / a->group));
+    }
+    return plan;
 }
 
-}  // namespace
-}  // namespace decode
-}  // namespace piton
-
-using namespace piton;
-using namespace piton::decode;
-
-extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream) {
+int check_matvec(const piton_matvec_w4_args *a) {
     PITON_REQUIRE(a != nullptr, "args is NULL");
     PITON_REQUIRE(a->flags == 0, "unknown flags 0x%x", a->flags);
     PITON_REQUIRE(a->type >= PITON_B200_TYPE_F32 && a->type <= PITON_B200_TYPE_BF16, "unknown element type %d", a->type);
@@ -513,9 +578,32 @@ extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream)
     PITON_REQUIRE(a->rows <= 65535 && a->outer < (1ll << 31) && a->inner <= (1ll << 30), "rows, inner or outer too large");
     if (a->group != 32 && a->group != 64 && a->group != 128)
         return set_error(PITON_B200_ENOTSUP, "group %d (32, 64, 128)", a->group);
+    return PITON_B200_OK;
+}
+
+}  // namespace
+}  // namespace decode
+}  // namespace piton
+
+using namespace piton;
+using namespace piton::decode;
+
+extern "C" size_t piton_b200_matvec_w4_workspace_size(const piton_matvec_w4_args *a) {
+    if (check_matvec(a) != PITON_B200_OK || a->rows == 0 || a->outer == 0) return 0;
+    return plan_of(a).digits;
+}
+
+extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream) {
+    if (int rc = check_matvec(a)) return rc;
     if (a->rows == 0 || a->outer == 0) return PITON_B200_OK;
     PITON_REQUIRE(a->y && (a->inner == 0 || (a->x && a->codes && a->scales)), "NULL pointer");
+    const Plan plan = plan_of(a);
+    if (plan.digits && (!a->workspace || a->workspace_bytes < plan.digits))
+        return set_error(PITON_B200_EWORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes,
+                         (unsigned long long)plan.digits);
+    PITON_REQUIRE(a->workspace % 16 == 0 || !plan.digits, "workspace is not 16-byte aligned");
     MatvecParams p;
+    p.digits = plan.digits ? reinterpret_cast<uint8_t *>(a->workspace) : nullptr;
     p.x = reinterpret_cast<const void *>(a->x);
     p.codes = reinterpret_cast<const uint8_t *>(a->codes);
     p.scales = reinterpret_cast<const void *>(a->scales);
@@ -531,6 +619,6 @@ extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream)
     return with_type(a->type, [&](auto t) {
         using T = decltype(t);
         cudaStream_t s = as_stream(stream);
-        return a->rows <= 8 ? launch<T, 1>(p, s) : launch<T, 2>(p, s);
+        return a->rows <= 8 ? launch<T, 1>(p, plan, s) : launch<T, 2>(p, plan, s);
     });
 }

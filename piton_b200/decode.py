@@ -52,7 +52,8 @@ class PagedKV(NamedTuple):
         return cls(*codes, *scales)
 
 
-_ENTRIES = ("piton_b200_kv_append", "piton_b200_kv_attention", "piton_b200_kv_attention_workspace_size", "piton_b200_matvec_w4")
+_ENTRIES = ("piton_b200_kv_append", "piton_b200_kv_attention", "piton_b200_kv_attention_workspace_size",
+            "piton_b200_matvec_w4_workspace_size", "piton_b200_matvec_w4")
 _bound = None
 
 

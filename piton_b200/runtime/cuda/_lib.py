@@ -125,8 +125,8 @@ class KvAttentionArgs(C.Structure):
 class MatvecW4Args(C.Structure):
     _fields_ = [("x", u64), ("codes", u64), ("scales", u64), ("zeros", u64), ("bias", u64), ("y", u64),
                 ("rows", i64), ("inner", i64), ("outer", i64), ("stride_x", i64), ("stride_codes", i64),
-                ("stride_scales", i64), ("stride_zeros", i64), ("stride_y", i64), ("group", i32), ("type", i32),
-                ("scale_type", i32), ("flags", u32)]
+                ("stride_scales", i64), ("stride_zeros", i64), ("stride_y", i64), ("workspace", u64),
+                ("workspace_bytes", u64), ("group", i32), ("type", i32), ("scale_type", i32), ("flags", u32)]
 
 
 # name -> (restype, argtypes); every function include/piton_b200.h declares
@@ -177,6 +177,7 @@ PROTOTYPES = {
     "piton_b200_kv_append": (C.c_int, [C.POINTER(KvAppendArgs), C.c_void_p]),
     "piton_b200_kv_attention_workspace_size": (C.c_size_t, [C.POINTER(KvAttentionArgs)]),
     "piton_b200_kv_attention": (C.c_int, [C.POINTER(KvAttentionArgs), C.c_void_p]),
+    "piton_b200_matvec_w4_workspace_size": (C.c_size_t, [C.POINTER(MatvecW4Args)]),
     "piton_b200_matvec_w4": (C.c_int, [C.POINTER(MatvecW4Args), C.c_void_p]),
 }
 
