@@ -90,6 +90,34 @@ template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WO
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
 
+// Two floats in one 64-bit register, and the instructions that take two at a time: half as many to issue.
+typedef unsigned long long pair;
+__device__ __forceinline__ pair both(float a, float b) {
+    pair d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ pair add2(pair a, pair b) {
+    pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ pair mul2(pair a, pair b) {
+    pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
+    pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// Two sums that were started at MAGIC.
+__device__ __forceinline__ pair values_of(int32_t a, int32_t b) {
+    return add2(both(__int_as_float(a), __int_as_float(b)), both(-12582912.0f, -12582912.0f));
+}
+
 // NT tiles of 8 rows of x, R tiles of 16 weight rows a warp, GROUPS = 128 / group scales of a weight row in a block.
 template <typename T, int NT, int R, int GROUPS> struct Shape {
     // Of each group's 32 WORDS elements in a block lane j takes the 8 WORDS from 8 WORDS j on: WORDS words of codes.
@@ -105,7 +133,7 @@ template <typename T, int NT, int R, int GROUPS> struct Shape {
     // shared memory: queues (in the end the warps' sums), x
     static_assert(WARPS * SUMS * 4 <= QUEUES, "the sums fit");
     static int64_t smem(int64_t rows, int64_t steps) {
-        return QUEUES + rows * (steps * (512 + (DIGITS == 3 ? 256 : 0) + 2 * META * 4) + 96);
+        return QUEUES + rows * (steps * (512 + (DIGITS == 3 ? 256 : 0)) + 96) + (rows + 1) / 2 * steps * (16 * META);
     }
 };
 
@@ -119,7 +147,7 @@ struct Layout {
 // Where the workspace holds all steps of all rows.
 template <typename S> __host__ __device__ Layout whole_layout(uint8_t *at, int64_t rows, int64_t steps) {
     Layout l;
-    l.pitch = steps * 512, l.pitch3 = S::DIGITS == 3 ? steps * 256 : 0, l.meta_pitch = steps * 2 * S::META;
+    l.pitch = steps * 512, l.pitch3 = S::DIGITS == 3 ? steps * 256 : 0, l.meta_pitch = steps * 4 * S::META;
     l.x = at, l.x3 = at + rows * l.pitch, l.meta = reinterpret_cast<float *>(l.x3 + rows * l.pitch3);
     return l;
 }
@@ -176,9 +204,9 @@ __device__ __forceinline__ void lay_out(const MatvecParams &p, int64_t m0, int x
                 if (in) {
                     *reinterpret_cast<uint4 *>(to.x + m * to.pitch + (b * 16 + unit) * 16) = make_uint4(digit[0][0], digit[0][1], digit[1][0], digit[1][1]);
                     if constexpr (DIGITS == 3) *reinterpret_cast<uint2 *>(to.x3 + m * to.pitch3 + (b * 16 + unit) * 8) = make_uint2(digit[2][0], digit[2][1]);
-                    float *about = to.meta + m * to.meta_pitch + b * S::META;
+                    float *about = to.meta + (m >> 1) * to.meta_pitch + b * (2 * S::META) + ((m0 + m) & 1);
                     if (unit == 0) about[0] = down;
-                    if (unit % (4 * WORDS) == 0) about[1 + unit / (4 * WORDS)] = (float)sum;
+                    if (unit % (4 * WORDS) == 0) about[2 + 2 * (unit / (4 * WORDS))] = (float)sum;
                 }
             }
 }
@@ -188,7 +216,7 @@ template <typename T, typename S> __global__ void __launch_bounds__(THREADS) mat
     asm volatile("griddepcontrol.launch_dependents;");              // the product may start on its weights, and waits before it reads x
     const int step = blockIdx.x * 8, m = blockIdx.y;
     Layout to = whole_layout<S>(p.digits, p.rows, all_steps);
-    to.x += m * to.pitch + step * 512, to.x3 += m * to.pitch3 + step * 256, to.meta += m * to.meta_pitch + step * 2 * S::META;
+    to.x += m * to.pitch + step * 512, to.x3 += m * to.pitch3 + step * 256, to.meta += (m >> 1) * to.meta_pitch + step * 4 * S::META;
     lay_out<T, S>(p, m, 1, step, min(8, all_steps - step), to);
 }
 
@@ -304,23 +332,22 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     float *meta = reinterpret_cast<float *>(x3 + x_rows * S::pitch3(p.phase));      // [x row][block of the phase][META]
     // rows of x past the last read the last: a column of the product depends on its own row alone
     uint32_t x_at[NT], x3_at[NT];
-    uint32_t meta_at[NT][2];
+    uint32_t meta_at[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int m = min(8 * t + g, x_rows - 1);
         x_at[t] = (uint32_t)__cvta_generic_to_shared(xs) + m * S::pitch(p.phase) + 16 * j;
         x3_at[t] = (uint32_t)__cvta_generic_to_shared(x3) + m * S::pitch3(p.phase) + 8 * j;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) meta_at[t][e] = (uint32_t)__cvta_generic_to_shared(meta + min(8 * t + 2 * j + e, x_rows - 1) * (2 * p.phase * S::META));
+        meta_at[t] = (uint32_t)__cvta_generic_to_shared(meta + min(4 * t + j, (x_rows - 1) >> 1) * (4 * p.phase * S::META));
     }
 
-    float acc[R][NT][4];
+    pair acc[R][NT][2];                                                 // weight rows row + 8 h, rows 2 j and 2 j + 1 of x
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[r][t][e] = 0.0f;
+            for (int h = 0; h < 2; ++h) acc[r][t][h] = 0;
 
     uint32_t slot = at0;
     int turn = 0;
@@ -331,19 +358,20 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
         if (p.digits) {                                                 // 16 bytes at a time, as they lie in the workspace
             const Layout from = whole_layout<S>(p.digits, p.rows, (p.inner + STEP - 1) / STEP);
             if (phase0 == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-            auto copy = [&](uint8_t *to, int to_pitch, const uint8_t *src, int64_t src_pitch, int row_bytes) {
-                for (int m = warp; m < x_rows; m += WARPS)
+            auto copy = [&](uint8_t *to, int to_pitch, const uint8_t *src, int64_t src_pitch, int row_bytes, int rows_of) {
+                for (int m = warp; m < rows_of; m += WARPS)
 #pragma unroll 4
-                    for (int i = 16 * lane; i < row_bytes; i += 512) copy16((uint32_t)__cvta_generic_to_shared(to + m * to_pitch + i), src + (m0 + m) * src_pitch + i);
+                    for (int i = 16 * lane; i < row_bytes; i += 512) copy16((uint32_t)__cvta_generic_to_shared(to + m * to_pitch + i), src + m * src_pitch + i);
             };
             const int64_t at = step0 + phase0;
-            copy(xs, S::pitch(p.phase), from.x + at * 512, from.pitch, count * 512);
-            if constexpr (DIGITS == 3) copy(x3, S::pitch3(p.phase), from.x3 + at * 256, from.pitch3, count * 256);
-            copy(reinterpret_cast<uint8_t *>(meta), 8 * S::META * p.phase, reinterpret_cast<const uint8_t *>(from.meta + at * 2 * S::META), 4 * from.meta_pitch,
-                 count * 8 * S::META);
+            copy(xs, S::pitch(p.phase), from.x + m0 * from.pitch + at * 512, from.pitch, count * 512, x_rows);
+            if constexpr (DIGITS == 3) copy(x3, S::pitch3(p.phase), from.x3 + m0 * from.pitch3 + at * 256, from.pitch3, count * 256, x_rows);
+            copy(reinterpret_cast<uint8_t *>(meta), 16 * S::META * p.phase,
+                 reinterpret_cast<const uint8_t *>(from.meta + m0 / 2 * from.meta_pitch + at * 4 * S::META), 4 * from.meta_pitch, count * 16 * S::META,
+                 (x_rows + 1) / 2);
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
         } else {
-            lay_out<T, S>(p, m0, x_rows, step0 + phase0, count, {xs, x3, meta, S::pitch(p.phase), S::pitch3(p.phase), 2 * p.phase * S::META});
+            lay_out<T, S>(p, m0, x_rows, step0 + phase0, count, {xs, x3, meta, S::pitch(p.phase), S::pitch3(p.phase), 4 * p.phase * S::META});
         }
         __syncthreads();
         const int phase_end = phase0 + count;
@@ -373,15 +401,14 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
             const uint32_t wat = slot + row * LINE + (((WORDS * j >> 2) ^ (row & 7)) * 16) + (4 * WORDS * j & 15);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                uint32_t about[NT][2][S::META];                         // the block's scale, then its groups' sums
+                pair about[NT][S::META];                                // the block's scales, then its groups' sums
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t from = meta_at[t][e] + (b0 + b) * (4 * S::META);
-                        if constexpr (GROUPS == 1) load_words<2>(about[t][e], from);
-                        else load_words<4>(*reinterpret_cast<uint32_t(*)[4]>(about[t][e]), from);
-                        if constexpr (GROUPS == 4) load_words<1>(*reinterpret_cast<uint32_t(*)[1]>(about[t][e] + 4), from + 16);
+                    for (int i = 0; i <= GROUPS; i += 2) {
+                        const uint32_t from = meta_at[t] + (b0 + b) * (8 * S::META) + 8 * i;
+                        if (i < GROUPS) asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(about[t][i]), "=l"(about[t][i + 1]) : "r"(from) : "memory");
+                        else asm volatile("ld.shared.u64 %0, [%1];" : "=l"(about[t][i]) : "r"(from) : "memory");
                     }
 #pragma unroll
                 for (int q = 0; q < GROUPS; ++q) {
@@ -404,12 +431,13 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                     const uint32_t z = __shfl_sync(0xffffffffu, zeros[load], from);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        float s2[2], z2[2];
+                        pair s2[2], z2[2];                              // scales and zero points, the latter negative
                         uint32_t w[2][WORDS];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            s2[h] = __uint_as_float(__shfl_sync(0xffffffffu, scale[load][2 * r + h], from));
-                            z2[h] = value_of(MAGIC | (z >> (8 * r + 4 * h) & 15));
+                            const float s = __uint_as_float(__shfl_sync(0xffffffffu, scale[load][2 * r + h], from));
+                            const float minus = -value_of(MAGIC | (z >> (8 * r + 4 * h) & 15));
+                            s2[h] = both(s, s), z2[h] = both(minus, minus);
                             // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of row 16 r + row + 8 h
                             load_words(w[h], (wat ^ (64 * b + 16 * WORDS * q)) + (16 * r + 8 * h) * LINE);
                         }
@@ -431,12 +459,12 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float v = value_of(sum[t][0][e]);
+                            for (int h = 0; h < 2; ++h) {
+                                pair v = values_of(sum[t][0][2 * h], sum[t][0][2 * h + 1]);
 #pragma unroll
-                                for (int d = 1; d < DIGITS; ++d) v = fmaf(v, 256.0f, value_of(sum[t][d][e]));
-                                v = fmaf(-z2[e >> 1], __uint_as_float(about[t][e & 1][1 + q]), v);
-                                acc[r][t][e] = fmaf(v, __uint_as_float(about[t][e & 1][0]) * s2[e >> 1], acc[r][t][e]);
+                                for (int d = 1; d < DIGITS; ++d) v = fma2(v, both(256.0f, 256.0f), values_of(sum[t][d][2 * h], sum[t][d][2 * h + 1]));
+                                v = fma2(z2[h], about[t][1 + q], v);
+                                acc[r][t][h] = fma2(v, mul2(about[t][0], s2[h]), acc[r][t][h]);
                             }
                     }
                 }
@@ -454,8 +482,10 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                sums[warp * S::SUMS + (8 * t + 2 * j + (e & 1)) * (16 * R) + 16 * r + row + 8 * (e >> 1)] = acc[r][t][e];
+            for (int h = 0; h < 2; ++h) {
+                float *to = sums + warp * S::SUMS + (8 * t + 2 * j) * (16 * R) + 16 * r + row + 8 * h;
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(to[0]), "=f"(to[16 * R]) : "l"(acc[r][t][h]));
+            }
     __syncthreads();
     constexpr int ADD = ALONG_K ? WARPS : 1, TILES = WARPS / ADD;       // warps that share a tile, tiles of the CTA
     if (ALONG_K && parts > 1) {
@@ -563,7 +593,7 @@ Plan plan_of(const piton_matvec_w4_args *a) {
     const int64_t x_rows = a->rows < 16 ? a->rows : 16;
     if (x_rows * cdiv(steps, parts) * 2 * BLOCK > 8192) {
         const int64_t fp32 = a->type == PITON_B200_TYPE_F32;
-        plan.digits = (size_t)(a->rows * steps) * (512 + (fp32 ? 256 : 0) + 2 * 4 * 2 * (128 / a->group));
+        plan.digits = (size_t)(a->rows * steps) * (512 + (fp32 ? 256 : 0)) + (size_t)((a->rows + 1) / 2 * steps) * (32 * (128 / a->group));
     }
     return plan;
 }
