@@ -212,12 +212,13 @@ __device__ __forceinline__ void lay_out(const MatvecParams &p, int64_t m0, int x
 }
 
 // x laid out once for all CTAs, which would otherwise repeat it for every 256 weight rows: a thread a unit.
-template <typename T, typename S> __global__ void __launch_bounds__(THREADS) matvec_w4_digits_kernel(const MatvecParams p, int all_steps) {
-    asm volatile("griddepcontrol.launch_dependents;");              // the product may start on its weights, and waits before it reads x
+template <typename T, typename S> __global__ void __launch_bounds__(THREADS) matvec_w4_digits_kernel(const MatvecParams p, int all_steps, bool early) {
+    if (early) asm volatile("griddepcontrol.launch_dependents;");   // the product may start on its weights, and waits before it reads x
     const int step = blockIdx.x * 8, m = blockIdx.y;
     Layout to = whole_layout<S>(p.digits, p.rows, all_steps);
     to.x += m * to.pitch + step * 512, to.x3 += m * to.pitch3 + step * 256, to.meta += (m >> 1) * to.meta_pitch + step * 4 * S::META;
     lay_out<T, S>(p, m, 1, step, min(8, all_steps - step), to);
+    if (!early) asm volatile("griddepcontrol.launch_dependents;");
 }
 
 // ALONG_K: the CTA's warps share 16 R weight rows and split the inner dimension; otherwise each has rows of its own.
@@ -541,12 +542,17 @@ template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(Matvec
         PITON_CUDA(cudaFuncSetAttribute(matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
         if (dev >= 0 && dev < 64) known[dev] = true;
     }
+    const dim3 grid((unsigned)(cdiv(p.outer, ALONG_K ? 16 * R : 16 * R * WARPS) * plan.parts), (unsigned)cdiv(p.rows, 8 * NT));
     if (plan.digits) {
-        matvec_w4_digits_kernel<T, S><<<dim3((unsigned)cdiv(all_steps, 8), (unsigned)p.rows), THREADS, 0, s>>>(p, all_steps);
+        const dim3 laying((unsigned)cdiv(all_steps, 8), (unsigned)p.rows);
+        // The product starts while x is laid out, unless its clusters would then not all find room at once: 4096 x 4096, one
+        // row, 256 + 2 CTAs: 5.8 us, after it 6.4; 8192 x 8192, 5 rows, bf16, 32 clusters + 20 CTAs: 17.5 us, after it 12.9.
+        const bool early = plan.parts == 1 || (int64_t)grid.x * grid.y + (int64_t)laying.x * laying.y <= 272;
+        matvec_w4_digits_kernel<T, S><<<laying, THREADS, 0, s>>>(p, all_steps, early);
         launches = 2;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(cdiv(p.outer, ALONG_K ? 16 * R : 16 * R * WARPS) * plan.parts), (unsigned)cdiv(p.rows, 8 * NT));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = (size_t)S::smem(x_rows, p.phase);
     cfg.stream = s;
@@ -589,9 +595,11 @@ Plan plan_of(const piton_matvec_w4_args *a) {
         while (2 * parts <= most && tiles * 2 * parts <= 2 * sms && steps >= WARPS * 2 * parts) parts *= 2;
     }
     plan.parts = (int)parts;
-    // More than 8192 elements of x a CTA are laid out once in the workspace by a kernel of their own
+    // More than 2048 elements of x a CTA are laid out once in the workspace, by a kernel of their own (bf16, 8192 elements, 4 rows
+    // by 2048 x 2048: 4.6 us, in every CTA 6.0; 2048 elements, 8 rows by 8192 x 2048: 7.1 and 6.7; 65536 elements, 16 rows by
+    // 4096 x 4096: 10.4 and 28).
     const int64_t x_rows = a->rows < 16 ? a->rows : 16;
-    if (x_rows * cdiv(steps, parts) * 2 * BLOCK > 8192) {
+    if (x_rows * cdiv(steps, parts) * 2 * BLOCK > 2048) {
         const int64_t fp32 = a->type == PITON_B200_TYPE_F32;
         plan.digits = (size_t)(a->rows * steps) * (512 + (fp32 ? 256 : 0)) + (size_t)((a->rows + 1) / 2 * steps) * (32 * (128 / a->group));
     }
