@@ -135,8 +135,9 @@ template <typename T> __device__ __forceinline__ void load_four(float (&x)[4], c
 // NaN codes (7F and FF) of a word: a set high bit in each such byte.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
-// CTAs an SM holds: registers bound it. Sixteen-bit rows add their products straight into the output's registers.
-template <typename T> constexpr int ctas(int nq) { return (nq == 1 ? 4 : 3) - (sizeof(T) == 4 ? 1 : 0); }
+// CTAs an SM holds: registers bound it. Three of 16 rows a tile would spill at 128 dimensions or in fp32 (24 sequences, 4 new
+// tokens, window 2048, fp32: 2 CTAs 40.5 us, 3 CTAs 55; 16 bits, 64 dimensions, 2000 keys: 28.1 and 26.0).
+constexpr int ctas(int nq, int dim, bool fp32) { return nq == 1 || (dim <= 64 && !fp32) ? 3 : 2; }
 
 // The rows of a tile that a lane holds in its score and output fragments: columns 2 j and 2 j + 1 of each of the NQ
 // 8-row groups; the keys [first, pos] that each sees.
@@ -145,7 +146,7 @@ template <int NQ> struct Rows {
 };
 
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(THREADS, NQ == 2 ? 2 : 3) kv_attention_kernel(const CachedParams p) {
+__global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_attention_kernel(const CachedParams p) {
     using G = Geometry<D>;
     constexpr bool SPLIT = sizeof(T) == 4;              // fp32 rows: queries and weights as pairs of halves
     constexpr float LIFT = SPLIT ? 14.0f : 6.0f, SLACK = SPLIT ? 0.0f : 8.0f;
@@ -607,7 +608,53 @@ __global__ void __launch_bounds__(THREADS, NQ == 2 ? 2 : 3) kv_attention_kernel(
     }
 }
 
-// Joins the splits of the keys: a CTA per row, its warps a split in four each.
+// Joins a few (up to 32) splits of the keys: a warp per row, lane s holds split s's maximum and sum.
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS) kv_attention_join_few_kernel(const CachedParams p) {
+    constexpr int E = D / 32, HELD = 8;                 // elements of a lane, splits that are on their way at a time
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = p.tokens * p.q_heads, row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' results are there
+    const float2 ml = lane < p.splits ? p.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
+    const float *from = p.part_o + row * D + lane * E;
+    float held[HELD][E];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            if (s0 + i >= p.splits) break;
+            const float *at = from + (s0 + i) * rows * D;
+            if constexpr (E == 4) *reinterpret_cast<float4 *>(held[i]) = *reinterpret_cast<const float4 *>(at);
+            else if constexpr (E == 2) *reinterpret_cast<float2 *>(held[i]) = *reinterpret_cast<const float2 *>(at);
+            else held[i][0] = *at;
+        }
+    };
+    load(0);
+    float top = ml.x;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float factor = ml.y == 0.0f ? 0.0f : ex2(ml.x - top);
+    float total = ml.y == 0.0f ? 0.0f : ml.y * factor, sum[E] = {};
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    for (int s0 = 0; s0 < p.splits; s0 += HELD) {
+        if (s0) load(s0);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            if (s0 + i >= p.splits) break;
+            const float f = __shfl_sync(0xffffffffu, factor, s0 + i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[e] += f == 0.0f ? 0.0f : held[i][e] * f;
+        }
+    }
+    const int64_t t = row / p.q_heads, h = row % p.q_heads;
+    T *out = reinterpret_cast<T *>(p.out) + t * p.sot + h * p.soh + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = from_float<T>(total == 0.0f ? 0.0f : sum[e] / total);
+    if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
+}
+
+// Joins more of them: a CTA per row, its warps a split in four each.
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS) kv_attention_join_kernel(const CachedParams p) {
     constexpr int E = D / 32;
@@ -693,7 +740,7 @@ Plan plan_of(const piton_kv_attention_args *a) {
     const int64_t keys = a->head_dim == 128 ? 32 : 64;  // of a stage
     if (a->window && a->window + most_new + keys < span) span = a->window + most_new + keys;
     // enough CTAs for every SM and no split below 256 keys
-    const int64_t units = plan.row_tiles * a->kv_heads * a->batch, slots = (int64_t)num_sms() * (plan.nq == 2 ? 2 : plan.nq == 1 ? 3 : a->type == PITON_B200_TYPE_F32 ? ctas<float>(plan.nq) : ctas<__half>(plan.nq));
+    const int64_t units = plan.row_tiles * a->kv_heads * a->batch, slots = (int64_t)num_sms() * ctas(plan.nq, (int)a->head_dim, a->type == PITON_B200_TYPE_F32);
     int64_t splits = units >= slots ? 1 : slots / units;
     const int64_t most = cdiv(span, 256);
     splits = splits < most ? splits : most;
@@ -719,16 +766,20 @@ template <typename T, int D, int NQ> int launch(const CachedParams &p, int64_t b
     if (p.splits == 1) return check_launch("kv_attention");
     // launched while the splits finish (programmatic dependent launch); it waits for them before it reads
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.tokens * p.q_heads));
+    const int64_t rows = p.tokens * p.q_heads;
+    // a warp a row for few splits (2 splits of 1920 rows: 32.3 us a call, a CTA a row 40.6), a CTA a row for more (16 splits of 32
+    // rows: 9.9 us, a warp a row 10.3), unless there are many rows (13 splits of 128 rows: a warp a row 16.4, a CTA 17.2)
+    const bool few = p.splits <= (rows < 128 ? 8 : 16);
+    cfg.gridDim = dim3((unsigned)(few ? cdiv(rows, WARPS) : rows));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = (size_t)(p.splits + WARPS * D) * sizeof(float);
+    cfg.dynamicSmemBytes = few ? 0 : (size_t)(p.splits + WARPS * D) * sizeof(float);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    PITON_CUDA(cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<T, D>, p));
+    PITON_CUDA(cudaLaunchKernelEx(&cfg, few ? kv_attention_join_few_kernel<T, D> : kv_attention_join_kernel<T, D>, p));
     return check_launch("kv_attention", 2);
 }
 
