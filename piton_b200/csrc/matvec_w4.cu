@@ -4,18 +4,25 @@
 // arranged around streaming them with few instructions a byte.  A warp takes 16 R weight rows in steps of 256 inner
 // elements (128 bytes of a row), copied with cp.async into a queue of its own, so no warp waits for another while it
 // streams.  The sums over a group are taken exactly in integers: a nibble is a byte after one mask, and the rows of x
-// are laid out once per CTA in shared memory as fixed-point numbers of their block's largest magnitude, two signed
-// 8-bit digits for 16-bit types (error below 2^-16 of that magnitude, where the types' own roundings are 2^-9 and
-// 2^-12 of each element) and three for fp32 (2^-24).  Codes are the 16-row side of the integer mma.m16n8k32
+// are laid out as fixed-point numbers of the largest magnitude in their block of 128, two signed 8-bit digits for
+// 16-bit types (half a step is 2^-16 of that magnitude; the types' own half steps are larger from 2^-5 of it on for fp16, from
+// 2^-8 for bf16) and three for fp32 (2^-24).  x is laid out by a small kernel into a
+// workspace, from where a CTA copies its share into shared memory, or by every CTA itself where that share is small.  Codes are the 16-row side of the integer mma.m16n8k32
 // and the digits of x its 8-column side; what the accumulators hold is less than 2^22, so started at the bits of
 // 1.5 2^23 they are read back as floats by one subtraction.  The zero point's share, zero * sum(x), and the group's
-// scale are applied in fp32.  Against products with fp16 or bf16 weights (built first) this takes 3 instead of 9 or 11
+// scale are applied in fp32, two outputs an instruction.  Against products with fp16 or bf16 weights (built first) this takes 3 instead of 9 or 11
 // instructions per 8 codes, and instruction issue is what bounds the kernel.  A block of x with a non-finite element
 // makes its row of y NaN.
 //
 // A matrix with many rows gives every warp rows of its own (warps along the rows); one with few splits each
 // CTA's inner dimension over its eight warps (warps along the inner dimension).  Either way a cluster of CTAs
 // may split the inner dimension further, and adds its parts through distributed shared memory in a fixed order.
+//
+// Measured: 28000 x 8192, bf16, groups of 128: 1 row 28.7 us (4.1 TB/s), 8 rows 32.5, groups of 32 with zero points 70;
+// 4096 x 4096, bf16: 1 row 5.8 us, 16 rows 10.2; 32768 x 8192, bf16, 16 rows 60 us (2.4 TB/s). A call has 4 to 5 us that do
+// not depend on the matrix (launches, x, the cluster's sums); the rest waits for its own chain of loads, integer products
+// and fp32 sums with 16 warps an SM: instructions issue in 43 % of the cycles at 16 rows, DRAM is at 27 to 63 %. A third stage
+// of the queue of 32 rows was slower (28000 x 8192: 30.0 us).
 #include <cooperative_groups.h>
 
 #include <type_traits>

@@ -117,6 +117,15 @@ def test_append_many_heads(cuda, dtype, kv_heads, heads, n):
     check_append([0, 127, 300], [n, 0, 1], page=64, dim=64, kv_heads=kv_heads, heads=heads, dtype=dtype, seed=n, rot=48)
 
 
+@pytest.mark.parametrize("batch,n,kv_heads,page,dim,dtype", [(30, 40, 8, 16, 128, torch.float32), (9, 300, 12, 32, 128, torch.bfloat16),
+                                                             (40, 33, 7, 16, 128, torch.float16), (3, 1000, 33, 64, 32, torch.float32)])
+def test_append_blocks_that_walk_many_heads(cuda, batch, n, kv_heads, page, dim, dtype):
+    check_append([(11 * b) % 40 for b in range(batch)], [n] * batch, page=page, dim=dim, kv_heads=kv_heads, heads=kv_heads, uniform=True,
+                 dtype=dtype, rot=dim // 2, interleaved=batch % 2 == 0)
+    check_append([(11 * b) % 40 for b in range(batch)], [n - b % 5 for b in range(batch)], page=page, dim=dim, kv_heads=kv_heads, heads=2,
+                 dtype=dtype, with_q=False)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim,page", [(32, 16), (64, 128), (128, 16), (128, 64)])
 def test_attention_scales_far_apart(cuda, dtype, dim, page):
