@@ -3,7 +3,7 @@
 The reference runs dense attention (examples/attention.py:75-113) and dense layers
 (examples/nn_kernels.py:23-74) on whole fp32 operands; a decoder that serves many or long
 sequences keeps its keys and values in pages and its weights in few bits.  Three operators make
-one step of such a decoder, each one launch of libpiton_b200 on the current torch stream,
+one step of such a decoder, each one or two launches of libpiton_b200 on the current torch stream,
 asynchronous, on CUDA tensors of float32, float16 or bfloat16:
 
 * :func:`kv_append` rotates new keys (and queries) by their positions and stores keys and values
@@ -231,7 +231,11 @@ def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
     the low half.  ``scales`` [outer, ceil(inner / group)] (float32, float16 or bfloat16) and ``zeros`` (uint8 of
     the same shape, the low four bits count; zero point 8 without) per group of 32, 64 or 128: W = scale * (code - zero).  ``bias``
     [outer] of x's type.  Rows of every operand may be strided.  Accumulates in 32 bits, returns x's type.
-    Meant for few rows: the weights are read again for every 16."""
+    Meant for few rows: the weights are read again for every 16.
+
+    Sums over a group are exact products of the codes with x in fixed point: of the largest magnitude in each
+    block of 128 elements of a row, 2^-16 is half a step for the 16-bit types and 2^-24 for float32.  A
+    row whose x has a non-finite element is NaN throughout."""
     result = (_bound or _calls()).matvec_w4(x, codes, scales, group, zeros, bias)
     if result is None or result.__class__ is int:
         _failed("matvec_w4", result, _refuse_matvec, x, codes, scales, group, zeros, bias)
