@@ -195,7 +195,13 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
     const int64_t begin = (int64_t)(first_lo & ~(KEYS - 1)) + (int64_t)split * p.chunk;
     const int64_t stop = split == p.splits - 1 ? end : min(end, begin + p.chunk);
     const int64_t mine = begin + warp * KEYS;
-    const int stages = stop > mine ? (int)((stop - mine + KEYS * WARPS - 1) / (KEYS * WARPS)) : 0;
+    // From here on keys are counted from `mine`, in 32 bits: [0, span) is this warp's range, its stage s the KEYS from s STRIDE on.
+    // What lies far before it is as good as just before.
+    constexpr int32_t STRIDE = KEYS * WARPS;
+    const int32_t span = (int32_t)max(stop - mine, (int64_t)0), mine32 = (int32_t)mine;
+    const int32_t stages = span / STRIDE + (span % STRIDE != 0);
+    auto from_mine = [&](int32_t pos) { return (int32_t)max((int64_t)pos - mine, (int64_t)-1); };
+    const int32_t lo = from_mine(first_lo), lo_all = from_mine(first_hi), hi_all = from_mine(pos_lo);    // every row sees [lo_all, hi_all]
 
     // ---- this lane's copies ----
     const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * G::QUEUE;
@@ -210,22 +216,24 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
     const uint32_t k_read[2] = {ring0 + (G::KC == 2 ? g * D + (j + 4 * (g & 1)) * 16 : lane * G::KB),
                                 ring0 + (G::KC == 2 ? g * D + (j + 4 * (~g & 1)) * 16 : lane * G::KB)};
     const uint32_t v_slot = ring0 + 2 * G::BYTES + lane * G::VB;
-    const uint8_t *k_lane = p.kc + k_row * D + (G::KC == 2 ? (lane & 7) * 16 : j * G::KB), *v_lane = p.vc + 2 * j * D + g * G::VB;
+    const uint32_t head_bytes = (uint32_t)D << p.page_log2, page_bytes = head_bytes * p.kv_heads;     // below 2^31 (heads are below 2^16)
+    const uint8_t *k_lane = p.kc + (int64_t)kvh * head_bytes + k_row * D + (G::KC == 2 ? (lane & 7) * 16 : j * G::KB);
+    const uint8_t *v_lane = p.vc + (int64_t)kvh * head_bytes + 2 * j * D + g * G::VB;
     int32_t ids = -1, ids_next = -1, ids_v = -1;        // pages of the 32 tiles of RUN stages, lane by lane; the values' are a stage behind
     uint32_t off_run = 0, off_run_v = 0;                // which of them are not to be read
     auto load_ids = [&](int s0) {                       // stages s0 .. s0 + RUN - 1
-        const int64_t key = mine + (int64_t)(s0 + lane / TILES) * (KEYS * WARPS) + 16 * (lane % TILES);
-        if (key >= stop || key + 15 < first_lo) return -1;
-        const int32_t id = s0 == 0 && !p.window ? ahead : table[key >> p.page_log2];
+        const uint32_t at = (uint32_t)(s0 + lane / TILES) * STRIDE + 16 * (lane % TILES);       // may pass 2^31
+        if (at >= (uint32_t)span || (int32_t)at < lo - 15) return -1;
+        const int32_t id = s0 == 0 && !p.window ? ahead : table[(mine32 + (int32_t)at) >> p.page_log2];
         if (id >= 0 && id < p.num_pages) return id;
         record_status(STATUS_BAD_PAGE);
         return -1;
     };
-    auto whole = [&](int64_t key0, int s, uint32_t off) {   // every key of the stage exists
-        return key0 >= first_lo && key0 + KEYS <= stop && !(off >> (TILES * (s % G::RUN)) & ((1u << TILES) - 1));
+    auto whole = [&](int32_t at, int s, uint32_t off) { // every key of the stage exists
+        return at >= lo && span - at >= KEYS && !(off >> (TILES * (s % G::RUN)) & ((1u << TILES) - 1));
     };
-    auto offset_of = [&](int32_t id, int64_t key) {     // of a key's row in either array of codes
-        return (((int64_t)max(id, 0) * p.kv_heads + kvh << p.page_log2) + (key & page_mask)) * D;
+    auto row_of = [&](const uint8_t *lane_at, int32_t id, int32_t at) {     // of a lane's first key in a tile
+        return lane_at + (uint64_t)(uint32_t)max(id, 0) * page_bytes + (uint32_t)((mine32 + at & page_mask) * D);
     };
     auto issue_k = [&](int s) {
         if (s < stages) {
@@ -234,13 +242,13 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
                 off_run = __ballot_sync(0xffffffffu, ids < 0);
                 ids_next = load_ids(s + G::RUN);
             }
-            const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
+            const int32_t key0 = s * STRIDE;
             const uint32_t at = k_slot + (s & 1) * G::BYTES;
             const bool all = whole(key0, s, off_run);
             if (all) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
-                    const uint8_t *src = k_lane + offset_of(__shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t), key0 + 16 * t);
+                    const uint8_t *src = row_of(k_lane, __shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t), key0 + 16 * t);
 #pragma unroll
                     for (int i = 0; i < 2 * G::KC; ++i)
                         copy_async<G::KB>(at + (2 * t * G::KC + i) * 32 * G::KB, src + i * K_STEP * D);
@@ -249,12 +257,12 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
 #pragma unroll 1
                 for (int t = 0; t < TILES; ++t) {
                     const int32_t id = __shfl_sync(0xffffffffu, ids, TILES * (s % G::RUN) + t);
-                    const int64_t key = key0 + 16 * t;
-                    const uint8_t *src = k_lane + offset_of(id, key);
+                    const int32_t key = key0 + 16 * t;
+                    const uint8_t *src = row_of(k_lane, id, key);
 #pragma unroll
                     for (int i = 0; i < 2 * G::KC; ++i) {
                         const int row = k_row + i * K_STEP;
-                        const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
+                        const bool on = id >= 0 && key + row >= lo && key < span - row;
                         copy_async<G::KB>(at + (2 * t * G::KC + i) * 32 * G::KB, on ? src + i * K_STEP * D : p.kc, on);
                     }
                 }
@@ -272,13 +280,13 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
     auto issue_v = [&](int s) {
         if (s < stages) {
             if (s % G::RUN == 0) ids_v = ids, off_run_v = off_run;     // the keys are at most one stage on
-            const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
+            const int32_t key0 = s * STRIDE;
             const uint32_t at = v_slot;
             const bool all = whole(key0, s, off_run_v);
             if (all) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t) {
-                    const uint8_t *src = v_lane + offset_of(__shfl_sync(0xffffffffu, ids_v, TILES * (s % G::RUN) + t), key0 + 16 * t);
+                    const uint8_t *src = row_of(v_lane, __shfl_sync(0xffffffffu, ids_v, TILES * (s % G::RUN) + t), key0 + 16 * t);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)             // rows 2 j + (r & 1) + 8 (r >> 1)
                         copy_async<G::VB>(at + (4 * t + r) * 32 * G::VB, src + ((r & 1) + 8 * (r >> 1)) * D);
@@ -287,12 +295,12 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
 #pragma unroll 1
                 for (int t = 0; t < TILES; ++t) {
                     const int32_t id = __shfl_sync(0xffffffffu, ids_v, TILES * (s % G::RUN) + t);
-                    const int64_t key = key0 + 16 * t;
-                    const uint8_t *src = v_lane + offset_of(id, key);
+                    const int32_t key = key0 + 16 * t;
+                    const uint8_t *src = row_of(v_lane, id, key);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int row = 2 * j + (r & 1) + 8 * (r >> 1);
-                        const bool on = id >= 0 && key + row >= first_lo && key + row < stop;
+                        const bool on = id >= 0 && key + row >= lo && key < span - row;
                         copy_async<G::VB>(at + (4 * t + r) * 32 * G::VB, on ? src + ((r & 1) + 8 * (r >> 1)) * D : p.vc, on);
                     }
                 }
@@ -356,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
 
 #pragma unroll 1
     for (int s = 0; s < stages; ++s) {
-        const int64_t key0 = mine + (int64_t)s * (KEYS * WARPS);
+        const int32_t key0 = s * STRIDE;
         const uint32_t at = (s & 1) * G::BYTES;
         wait<2>();                                      // the next stage's keys and this one's values may be on their way
         __syncwarp();                                   // copies of other lanes
@@ -411,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
         issue_k(s + 2);
 
         // ---- softmax ----
-        const bool edge = key0 < first_hi || key0 + KEYS - 1 > pos_lo || key0 + KEYS > stop || bad;
+        const bool edge = key0 < lo_all || key0 > hi_all - (KEYS - 1) || span - key0 < KEYS || bad;
         uint32_t off[NQ];
         float alpha[NQ][2];
 #pragma unroll
@@ -426,8 +434,8 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
                 for (int t = 0; t < TILES; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int64_t key = key0 + 16 * t + g + 8 * (e >> 1);
-                        const bool on = !(bad >> t & 1) && key >= seen.first[n][e & 1] && key <= seen.pos[n][e & 1] && key < stop;
+                        const int32_t in = 16 * t + g + 8 * (e >> 1), key = (int32_t)((uint32_t)(mine32 + key0) + in);     // (past 2^31: off)
+                        const bool on = !(bad >> t & 1) && key0 < span - in && key >= seen.first[n][e & 1] && key <= seen.pos[n][e & 1];
                         if (!on) off[n] |= 1u << (4 * t + e), c[t][n][e] = -INFINITY;
                     }
             }
