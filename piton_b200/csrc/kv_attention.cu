@@ -24,10 +24,10 @@
 // fill one wave, and a second kernel, launched while the first finishes, joins them in a fixed order. More splits than one wave were slower
 // (24 sequences, 4 new tokens, window 2048: 240 CTAs 32.4 us, 360 CTAs 44.8).
 //
-// Measured: 268 MB of codes, one sequence, bf16: 63 us (4.2 TB/s); 32 sequences, fp32, 538 MB: 112 us (4.8 TB/s); 64
-// sequences of 2000 keys, fp16: 60 us (3.4 TB/s); one of 1000 keys: 9.3 us, of 100 keys and 4 heads: 5.2. Up to 8 rows a tile the copies bound it once a
+// Measured: 268 MB of codes, one sequence, bf16: 63 us (4.2 TB/s); 32 sequences, fp32, 538 MB: 109 us (4.9 TB/s); 64
+// sequences of 2000 keys, fp16: 59 us (3.4 TB/s); one of 1000 keys: 9.0 us, of 100 keys and 4 heads: 4.7. Up to 8 rows a tile the copies bound it once a
 // warp has several stages; with 16 rows the chain of products, softmax and products of 8 warps an SM does (instructions issue in
-// 30 % of the cycles: 32.4 us where the bytes take 9.8).
+// 30 % of the cycles: 32.1 us where the bytes take 9.8).
 #include "decode.cuh"
 
 namespace piton {

@@ -19,10 +19,10 @@
 // may split the inner dimension further, and adds its parts through distributed shared memory in a fixed order.
 //
 // Measured: 28000 x 8192, bf16, groups of 128: 1 row 28.7 us (4.1 TB/s), 8 rows 32.5, groups of 32 with zero points 70;
-// 4096 x 4096, bf16: 1 row 5.8 us, 16 rows 10.2; 32768 x 8192, bf16, 16 rows 60 us (2.4 TB/s). A call has 4 to 5 us that do
+// 4096 x 4096, bf16: 1 row 5.8 us, 16 rows 9.3; 32768 x 8192, bf16, 16 rows 60 us (2.4 TB/s). A call has 4 to 5 us that do
 // not depend on the matrix (launches, x, the cluster's sums); the rest waits for its own chain of loads, integer products
-// and fp32 sums with 16 warps an SM: instructions issue in 43 % of the cycles at 16 rows, DRAM is at 27 to 63 %. A third stage
-// of the queue of 32 rows was slower (28000 x 8192: 30.0 us).
+// and fp32 sums with 16 warps an SM: instructions issue in 43 % of the cycles at 16 rows, DRAM is at 27 to 63 %.
+// A second buffer of x, filled while the first is used, was slower for 16 rows (62 us).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -129,7 +129,9 @@ __device__ __forceinline__ pair values_of(int32_t a, int32_t b) {
 template <typename T, int NT, int R, int GROUPS> struct Shape {
     // Of each group's 32 WORDS elements in a block lane j takes the 8 WORDS from 8 WORDS j on: WORDS words of codes.
     static constexpr int WORDS = 4 / GROUPS;
-    static constexpr int SLOT = 16 * R * LINE, STAGES = R == 1 ? 4 : 2, QUEUES = WARPS * STAGES * SLOT;
+    // Two stages of 32 weight rows (three: 28000 x 8192 30.0 us, two 28.6); of 16, three with one tile of x and two with two, whose x
+    // takes the room (4096 x 4096, fp32: 8 rows with 4 / 3 / 2 stages 9.7 / 7.9 / 8.1 us, 16 rows with 4 / 2 18.1 / 13.1)
+    static constexpr int SLOT = 16 * R * LINE, STAGES = R == 1 && NT == 1 ? 3 : 2, QUEUES = WARPS * STAGES * SLOT;
     static constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;               // of x; the first holds the most
     static constexpr int SUMS = 8 * NT * 16 * R;                        // outputs of a warp's tile
     // x in shared memory, per row: 16 bytes for every 8 elements (their first two digits), 8 more for fp32 (the third), and per
@@ -604,7 +606,7 @@ Plan plan_of(const piton_matvec_w4_args *a) {
     plan.parts = (int)parts;
     // More than 2048 elements of x a CTA are laid out once in the workspace, by a kernel of their own (bf16, 8192 elements, 4 rows
     // by 2048 x 2048: 4.6 us, in every CTA 6.0; 2048 elements, 8 rows by 8192 x 2048: 7.1 and 6.7; 65536 elements, 16 rows by
-    // 4096 x 4096: 10.4 and 28).
+    // 4096 x 4096: 9.3 and 28).
     const int64_t x_rows = a->rows < 16 ? a->rows : 16;
     if (x_rows * cdiv(steps, parts) * 2 * BLOCK > 2048) {
         const int64_t fp32 = a->type == PITON_B200_TYPE_F32;
