@@ -131,7 +131,7 @@ template <typename T, int NT, int R, int GROUPS> struct Shape {
     static constexpr int WORDS = 4 / GROUPS;
     // Two stages of 32 weight rows (three: 28000 x 8192 30.0 us, two 28.6); of 16, three with one tile of x and two with two, whose x
     // takes the room (4096 x 4096, fp32: 8 rows with 4 / 3 / 2 stages 9.7 / 7.9 / 8.1 us, 16 rows with 4 / 2 18.1 / 13.1)
-    static constexpr int SLOT = 16 * R * LINE, STAGES = R == 1 && NT == 1 ? 3 : 2, QUEUES = WARPS * STAGES * SLOT;
+    static constexpr int SLOT = 16 * R * LINE + 128, STAGES = R == 1 && NT == 1 ? 3 : 2, QUEUES = WARPS * STAGES * SLOT;
     static constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;               // of x; the first holds the most
     static constexpr int SUMS = 8 * NT * 16 * R;                        // outputs of a warp's tile
     // x in shared memory, per row: 16 bytes for every 8 elements (their first two digits), 8 more for fp32 (the third), and per
@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     // the weight row (and that + 8) of a tile that fragment row g is: rows that are read together lie in different banks
     const int row = WORDS == 4 ? (g & 1) << 2 | g >> 1 : WORDS == 2 ? (g & 3) << 1 | g >> 2 : g;
 
-    // ---- the queue: in a slot, row r's 128 bytes lie at 128 r, its 16-byte pieces exchanged by r % 8 ----
+    // ---- the queue: in a slot, row r's 128 bytes lie at 128 r, its 16-byte pieces exchanged by r % 8. Rows that do not start on 4
+    // bytes are copied from the word before on, and put right as they are read; their last words follow the rows ----
     const uint32_t at0 = (uint32_t)__cvta_generic_to_shared(queue) + warp * (STAGES * S::SLOT);
     const uint8_t *codes = p.codes + n0 * p.sc + (int64_t)(step0 + own0) * LINE;
     const uint32_t copy_at = (lane >> 3) * LINE + ((lane & 7) ^ (lane >> 3)) * 16;
@@ -276,22 +277,18 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                     if (R > 1 || r < rows) copy4(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src);
                     src += p.sc;
                 }
-            } else {                                                    // the last step, or rows that are not aligned: word by word
-                const int left = (p.inner + 1) / 2 - (step0 + own0 + issued * STRIDE) * LINE - 4 * lane;
-                const uint8_t *src = codes + 4 * lane;
+            } else {                                                    // the last step, or rows that are not aligned: words that hold a byte of the row
+                const uint8_t *src = codes;
+                const int64_t left = (p.inner + 1) / 2 - (int64_t)(step0 + own0 + issued * STRIDE) * LINE;
 #pragma unroll 4
                 for (int r = 0; r < rows; ++r) {
-                    const uint32_t dst = fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3);
-                    if (p.codes_align >= 4 && left >= 4) {
-                        copy4(dst, src);
-                    } else if (left > 0) {                              // (past the row's end x is 0, whatever the slot holds)
-                        uint32_t word = src[0];
-#pragma unroll
-                        for (int i = 1; i < 4; ++i) word |= (left > i ? (uint32_t)src[i] : 0u) << (8 * i);
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(word) : "memory");
-                    }
+                    const int before = (int)(reinterpret_cast<uintptr_t>(src) & 3);
+                    if (4 * lane - before < left) copy4(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src - before + 4 * lane);
                     src += p.sc;
                 }
+                src = codes + lane * p.sc;
+                const int before = (int)(reinterpret_cast<uintptr_t>(src) & 3);
+                if (before && lane < rows && LINE - before < left) copy4(fill + 16 * R * LINE + 4 * lane, src - before + LINE);
             }
             codes += STRIDE * LINE;
             ++issued;
@@ -359,6 +356,9 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 #pragma unroll
             for (int h = 0; h < 2; ++h) acc[r][t][h] = 0;
 
+    uint32_t before = 0;                                                // a byte each: the bits before rows row, row + 8, ... in their first words
+#pragma unroll
+    for (int h = 0; h < 2 * R; ++h) before |= (uint32_t)(reinterpret_cast<uintptr_t>(p.codes + (n0 + row + 8 * h) * p.sc) & 3) << (8 * h + 3);
     uint32_t slot = at0;
     int turn = 0;
 #pragma unroll 1
@@ -450,6 +450,14 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                             s2[h] = both(s, s), z2[h] = both(minus, minus);
                             // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of row 16 r + row + 8 h
                             load_words(w[h], (wat ^ (64 * b + 16 * WORDS * q)) + (16 * r + 8 * h) * LINE);
+                            if (p.codes_align == 1) {
+                                const int next = 16 * b + 4 * WORDS * q + WORDS * j + WORDS;    // the word after them
+                                uint32_t v[1];
+                                load_words(v, next == LINE / 4 ? slot + 16 * R * LINE + 4 * (16 * r + row + 8 * h)
+                                                               : slot + (16 * r + row + 8 * h) * LINE + ((next >> 2) ^ (row & 7)) * 16 + 4 * (next & 3));
+#pragma unroll
+                                for (int i = 0; i < WORDS; ++i) w[h][i] = __funnelshift_r(w[h][i], i + 1 < WORDS ? w[h][i + 1] : v[0], before >> (8 * (2 * r + h)));
+                            }
                         }
                         int32_t sum[NT][DIGITS][4];
 #pragma unroll
