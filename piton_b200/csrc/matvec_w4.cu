@@ -231,7 +231,7 @@ template <typename T, typename S> __global__ void __launch_bounds__(THREADS) mat
 }
 
 // ALONG_K: the CTA's warps share 16 R weight rows and split the inner dimension; otherwise each has rows of its own.
-template <typename T, int NT, int R, int GROUPS, bool ALONG_K>
+template <typename T, int NT, int R, int GROUPS, bool ALONG_K, bool BYTES>
 __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParams p) {
     using S = Shape<T, NT, R, GROUPS>;
     constexpr int WORDS = S::WORDS, STAGES = S::STAGES, STRIDE = ALONG_K ? WARPS : 1, DIGITS = S::DIGITS, STEP = 2 * BLOCK;
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                             s2[h] = both(s, s), z2[h] = both(minus, minus);
                             // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of row 16 r + row + 8 h
                             load_words(w[h], (wat ^ (64 * b + 16 * WORDS * q)) + (16 * r + 8 * h) * LINE);
-                            if (p.codes_align == 1) {
+                            if constexpr (BYTES) {
                                 const int next = 16 * b + 4 * WORDS * q + WORDS * j + WORDS;    // the word after them
                                 uint32_t v[1];
                                 load_words(v, next == LINE / 4 ? slot + 16 * R * LINE + 4 * (16 * r + row + 8 * h)
@@ -544,7 +544,7 @@ struct Plan {
     size_t digits;                          // bytes of x laid out in the workspace, 0: in every CTA
 };
 
-template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(MatvecParams p, const Plan &plan, cudaStream_t s) {
+template <typename T, int NT, int R, int GROUPS, bool ALONG_K, bool BYTES> int launch(MatvecParams p, const Plan &plan, cudaStream_t s) {
     using S = Shape<T, NT, R, GROUPS>;
     const int64_t x_rows = p.rows < 8 * NT ? p.rows : 8 * NT;
     const int all_steps = (int)cdiv(p.inner, 2 * BLOCK);
@@ -556,7 +556,7 @@ template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(Matvec
     int dev = 0, launches = 1;
     PITON_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !known[dev]) {
-        PITON_CUDA(cudaFuncSetAttribute(matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
+        PITON_CUDA(cudaFuncSetAttribute(matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K, BYTES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024));
         if (dev >= 0 && dev < 64) known[dev] = true;
     }
     const dim3 grid((unsigned)(cdiv(p.outer, ALONG_K ? 16 * R : 16 * R * WARPS) * plan.parts), (unsigned)cdiv(p.rows, 8 * NT));
@@ -582,8 +582,12 @@ template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(Matvec
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = plan.digits ? 2 : 1;
-    PITON_CUDA(cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K>, p));
+    PITON_CUDA(cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K, BYTES>, p));
     return check_launch("matvec_w4", launches);
+}
+
+template <typename T, int NT, int R, int GROUPS, bool ALONG_K> int launch(const MatvecParams &p, const Plan &plan, cudaStream_t s) {
+    return p.codes_align == 1 ? launch<T, NT, R, GROUPS, ALONG_K, true>(p, plan, s) : launch<T, NT, R, GROUPS, ALONG_K, false>(p, plan, s);
 }
 
 template <typename T, int NT, int R, bool ALONG_K> int launch(const MatvecParams &p, const Plan &plan, cudaStream_t s) {
