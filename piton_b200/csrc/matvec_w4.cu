@@ -18,8 +18,9 @@
 // CTA's inner dimension over its eight warps (warps along the inner dimension).  Either way a cluster of CTAs
 // may split the inner dimension further, and adds its parts through distributed shared memory in a fixed order.
 //
-// Measured: 28000 x 8192, bf16, groups of 128: 1 row 28.7 us (4.1 TB/s), 8 rows 32.5, groups of 32 with zero points 70;
-// 4096 x 4096, bf16: 1 row 5.8 us, 16 rows 9.3; 32768 x 8192, bf16, 16 rows 60 us (2.4 TB/s). A call has 4 to 5 us that do
+// Measured: 28000 x 8192, bf16, groups of 128: 1 row 28.0 us (4.2 TB/s), 8 rows 32, groups of 32 with zero points 69;
+// 4096 x 4096, bf16: 1 row 5.6 us, 16 rows 9.4; 32768 x 8192, bf16, 16 rows 59 us (2.4 TB/s). Rows of codes on 4 bytes: 8192 x 8200, 1 row
+// 15.4 us; on any byte: 4096 x 4098 8.2 us, 28000 x 8194 60 us, copies of 4 bytes a lane where whole rows take 16. A call has 4 to 5 us that do
 // not depend on the matrix (launches, x, the cluster's sums); the rest waits for its own chain of loads, integer products
 // and fp32 sums with 16 warps an SM: instructions issue in 43 % of the cycles at 16 rows, DRAM is at 27 to 63 %.
 // A second buffer of x, filled while the first is used, was slower for 16 rows (62 us).
@@ -129,7 +130,7 @@ __device__ __forceinline__ pair values_of(int32_t a, int32_t b) {
 template <typename T, int NT, int R, int GROUPS> struct Shape {
     // Of each group's 32 WORDS elements in a block lane j takes the 8 WORDS from 8 WORDS j on: WORDS words of codes.
     static constexpr int WORDS = 4 / GROUPS;
-    // Two stages of 32 weight rows (three: 28000 x 8192 30.0 us, two 28.6); of 16, three with one tile of x and two with two, whose x
+    // Two stages of 32 weight rows (three: 28000 x 8192 30.0 us, two 28.6 at the time); of 16, three with one tile of x and two with two, whose x
     // takes the room (4096 x 4096, fp32: 8 rows with 4 / 3 / 2 stages 9.7 / 7.9 / 8.1 us, 16 rows with 4 / 2 18.1 / 13.1)
     static constexpr int SLOT = 16 * R * LINE + 128, STAGES = R == 1 && NT == 1 ? 3 : 2, QUEUES = WARPS * STAGES * SLOT;
     static constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;               // of x; the first holds the most

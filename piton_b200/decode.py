@@ -245,7 +245,8 @@ def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
 def quantize_w4(weight, group: int = 128, zeros: bool = True, dtype=None):
     """Codes, scales and zero points (None if not ``zeros``) of a weight matrix [outer, inner], for
     :func:`matvec_w4`: each group of ``group`` elements spans its own range in 16 steps.  Plain torch, done
-    once when weights are loaded; scales are of ``dtype`` (the weight's by default)."""
+    once when weights are loaded; scales are of ``dtype`` (the weight's by default).  Rows of codes start on
+    16 bytes, which :func:`matvec_w4` reads fastest."""
     if group not in (32, 64, 128):
         raise NotImplementedError(f"group {group}: 32, 64 or 128")
     outer, inner = weight.shape
@@ -263,5 +264,7 @@ def quantize_w4(weight, group: int = 128, zeros: bool = True, dtype=None):
     inverse = torch.where(step > 0, 1.0 / step, 0.0)
     zero = (-lo * inverse).round().clamp(0, 15) if zeros else torch.full_like(step, 8.0)
     codes = (w * inverse[..., None] + zero[..., None]).round().clamp(0, 15).to(torch.uint8).view(outer, -1)
-    packed = codes[:, 0::2] | codes[:, 1::2] << 4
-    return packed[:, :(inner + 1) // 2].contiguous(), scales, zero.to(torch.uint8) if zeros else None
+    bytes_ = (inner + 1) // 2
+    packed = torch.zeros((outer, bytes_ + -bytes_ % 16), dtype=torch.uint8, device=weight.device)
+    packed[:, :bytes_] = (codes[:, 0::2] | codes[:, 1::2] << 4)[:, :bytes_]
+    return packed[:, :bytes_], scales, zero.to(torch.uint8) if zeros else None
