@@ -6,6 +6,7 @@ fixed-point numbers of the block's largest magnitude: an element is off by at mo
 ``test_matvec_outliers`` allows times the sum of |w| over the block.
 """
 
+import ctypes as C
 import math
 
 import pytest
@@ -13,6 +14,7 @@ import torch
 
 import decode_ref as ref
 from piton_b200 import decode
+from piton_b200.runtime.cuda import _lib
 from test_gpu_decode import (EPS, ROUND, TYPES, bound, check_append, check_attention, check_matvec, gen,
                               offsets, page_table, random_cache, status)
 
@@ -163,3 +165,31 @@ def test_attention_many_splits(cuda, dtype, dim, group, new):
 def test_attention_window_of_several_row_tiles(cuda, dtype, window, news):
     check_attention([5000, 1200], news, page=16, dim=128, kv_heads=2, group=8, dtype=dtype, window=window, uniform=len(set(news)) == 1)
     check_attention([5000, 1200], news, page=16, dim=128, kv_heads=2, group=8, dtype=dtype, window=window, max_length=5000, max_new=9)
+
+
+def test_matvec_workspace_is_asked_for(cuda):
+    g = gen(0)
+    handle = _lib.lib()
+    for rows, inner, needs in ((1, 2048, False), (9, 4096, True)):
+        x = torch.randn((rows, inner), generator=g, device="cuda")
+        codes = torch.randint(0, 256, (32, inner // 2), generator=g, device="cuda", dtype=torch.uint8)
+        scales = torch.rand((32, inner // 128), generator=g, device="cuda")
+        want = decode.matvec_w4(x, codes, scales)
+        y = torch.zeros_like(want)
+        args = _lib.MatvecW4Args(x=x.data_ptr(), codes=codes.data_ptr(), scales=scales.data_ptr(), y=y.data_ptr(), rows=rows,
+                                 inner=inner, outer=32, stride_x=inner, stride_codes=inner // 2, stride_scales=inner // 128, stride_y=32,
+                                 group=128, type=_lib.TYPE_F32, scale_type=_lib.TYPE_F32)
+        size = handle.piton_b200_matvec_w4_workspace_size(C.byref(args))
+        assert (size > 0) == needs
+        stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        if needs:
+            scratch = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+            for at, bytes_ in ((0, 0), (scratch.data_ptr(), size - 1)):
+                args.workspace, args.workspace_bytes = at, bytes_
+                assert handle.piton_b200_matvec_w4(C.byref(args), stream) == -6
+            args.workspace, args.workspace_bytes = scratch.data_ptr() + 8, size
+            assert handle.piton_b200_matvec_w4(C.byref(args), stream) == -1
+            assert not bool(y.any())
+            args.workspace = scratch.data_ptr()
+        assert handle.piton_b200_matvec_w4(C.byref(args), stream) == 0
+        assert torch.equal(y, want)
