@@ -418,7 +418,7 @@ PITON_B200_API int piton_b200_kv_attention(const piton_kv_attention_args *args, 
 
 /* y[rows, outer] = x[rows, inner] W^T (+ bias), W[n, k] = scales[n, k / group] * (code[n, k] - zero[n, k / group]).
    Codes are 4 bits, two per byte along k (even k in the low half), rows stride_codes bytes apart; group 32,
-   64 or 128; zeros uint8 (their low four bits count), or 0 for zero point 8.  x, bias and y are of `type`, scales of `scale_type`. */
+   64 or 128; zeros uint8 (any value), or 0 for zero point 8.  x, bias and y are of `type`, scales of `scale_type`. */
 typedef struct {
     uint64_t x, codes, scales, zeros, bias, y;
     int64_t rows, inner, outer;

@@ -302,11 +302,11 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 
     // ---- scales and zero points, a load ahead: lane (g, j) holds those of its 2 R weight rows for one group in four: with
     // group 128 the four groups of two steps, with 64 those of a step, with 32 those of a block (two loads a step); zero points
-    // of the rows share a word, four bits each ----
+    // of the rows share a word, a byte each ----
     constexpr int LOADS = GROUPS == 4 ? 2 : 1, AHEAD = GROUPS == 1 ? 2 : 1;    // loads in a step, steps of a load
     uint32_t scale[LOADS][2 * R], scale_next[LOADS][2 * R], zeros[LOADS], zeros_next[LOADS];
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) zeros[l] = zeros_next[l] = 0x88888888u;
+    for (int l = 0; l < LOADS; ++l) zeros[l] = zeros_next[l] = 0x08080808u;
     const int groups = (p.inner + (1 << p.group_log2) - 1) >> p.group_log2;
     const int64_t scale_row = (n0 + row) * p.ss, zero_row = (n0 + row) * p.sz;
     auto fetch = [&](int turn) {
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                 const uint8_t *at = p.zeros + zero_row + group;
                 zeros_next[l] = 0;
 #pragma unroll
-                for (int h = 0; h < 2 * R; ++h) zeros_next[l] |= (in && row + 8 * h < rows ? at[8 * h * p.sz] & 15u : 0u) << (4 * h);
+                for (int h = 0; h < 2 * R; ++h) zeros_next[l] |= (in && row + 8 * h < rows ? (uint32_t)at[8 * h * p.sz] : 0u) << (8 * h);
             }
         }
     };
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float s = __uint_as_float(__shfl_sync(0xffffffffu, scale[load][2 * r + h], from));
-                            const float minus = -value_of(MAGIC | (z >> (8 * r + 4 * h) & 15));
+                            const float minus = -value_of(MAGIC | (z >> (16 * r + 8 * h) & 255));
                             s2[h] = both(s, s), z2[h] = both(minus, minus);
                             // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of row 16 r + row + 8 h
                             load_words(w[h], (wat ^ (64 * b + 16 * WORDS * q)) + (16 * r + 8 * h) * LINE);

@@ -229,7 +229,7 @@ def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
 
     ``codes`` uint8 [outer, ceil(inner / 2)]: two codes per byte along the inner dimension, the even one in
     the low half.  ``scales`` [outer, ceil(inner / group)] (float32, float16 or bfloat16) and ``zeros`` (uint8 of
-    the same shape, the low four bits count; zero point 8 without) per group of 32, 64 or 128: W = scale * (code - zero).  ``bias``
+    the same shape, any value; zero point 8 without) per group of 32, 64 or 128: W = scale * (code - zero).  ``bias``
     [outer] of x's type.  Rows of every operand may be strided.  Accumulates in 32 bits, returns x's type.
     Meant for few rows: the weights are read again for every 16.
 
