@@ -3,27 +3,24 @@
 // The codes are read once (N K / 2 bytes) and bound the product up to about 16 rows, so everything is
 // arranged around streaming them with few instructions a byte.  A warp takes 16 R weight rows in steps of 256 inner
 // elements (128 bytes of a row), copied with cp.async into a queue of its own, so no warp waits for another while it
-// streams.  The sums over a group are taken exactly in integers: a nibble is a byte after one mask, and the rows of x
-// are laid out as fixed-point numbers of the largest magnitude in their block of 128, two signed 8-bit digits for
-// 16-bit types (half a step is 2^-16 of that magnitude; the types' own half steps are larger from 2^-5 of it on for fp16, from
-// 2^-8 for bf16) and three for fp32 (2^-24).  x is laid out by a small kernel into a
-// workspace, from where a CTA copies its share into shared memory, or by every CTA itself where that share is small.  Codes are the 16-row side of the integer mma.m16n8k32
-// and the digits of x its 8-column side; what the accumulators hold is less than 2^22, so started at the bits of
-// 1.5 2^23 they are read back as floats by one subtraction.  The zero point's share, zero * sum(x), and the group's
-// scale are applied in fp32, two outputs an instruction.  Against products with fp16 or bf16 weights (built first) this takes 3 instead of 9 or 11
-// instructions per 8 codes, and instruction issue is what bounds the kernel.  A block of x with a non-finite element
-// makes its row of y NaN.
+// streams.  Codes less their zero points are the 16-row side of mma.m16n8k16 and the rows of x its 8-column side.  Both are
+// exact: codes become 16-bit floats by a mask and one subtraction for two of them (9 instructions per 8 codes in fp16, 11 in bf16), x stays as
+// it is, and fp32 is the sum of three bf16 elements of 8 bits of significand each.  So only the fp32 sums are rounded, and something large
+// in x that meets weights of zero costs the rest nothing.  (Sums in integers over x in fixed point take 3 instructions per 8
+// codes and 28.0 us for one row of 28000 x 8192 where this takes 38, but lose what a row's small elements have below 2^-16 of a large one;
+// taking zero * sum(x) off the sum of code * x loses what the two have in common.)  The group's scale is applied in fp32, two outputs an
+// instruction.  x is put into the order of the fragments by every CTA, or once by a small kernel into a workspace, from where a
+// CTA copies its share.
 //
 // A matrix with many rows gives every warp rows of its own (warps along the rows); one with few splits each
 // CTA's inner dimension over its eight warps (warps along the inner dimension).  Either way a cluster of CTAs
 // may split the inner dimension further, and adds its parts through distributed shared memory in a fixed order.
 //
-// Measured: 28000 x 8192, bf16, groups of 128: 1 row 28.0 us (4.2 TB/s), 8 rows 32, groups of 32 with zero points 69;
-// 4096 x 4096, bf16: 1 row 5.6 us, 16 rows 9.4; 32768 x 8192, bf16, 16 rows 59 us (2.4 TB/s). Rows of codes on 4 bytes: 8192 x 8200, 1 row
-// 15.4 us; on any byte: 4096 x 4098 8.2 us, 28000 x 8194 60 us, copies of 4 bytes a lane where whole rows take 16. A call has 4 to 5 us that do
-// not depend on the matrix (launches, x, the cluster's sums); the rest waits for its own chain of loads, integer products
-// and fp32 sums with 16 warps an SM: instructions issue in 43 % of the cycles at 16 rows, DRAM is at 27 to 63 %.
-// A second buffer of x, filled while the first is used, was slower for 16 rows (62 us).
+// Measured: 28000 x 8192, groups of 128: 1 row, bf16 38 us (3.1 TB/s), fp16 35.5; 8 rows of bf16, groups of 32 with zero points 70;
+// 16 rows of fp32, groups of 64 with zero points 112. 4096 x 4096: 1 row, bf16 6.0 us, 16 rows 9.9; fp32, 8 rows 12.3, 16 rows 20.5; 32768 x
+// 8192, bf16, 16 rows 57 us (2.5 TB/s). Rows of codes on any byte: 4096 x 4098 9.0 us, copies of 4 bytes a lane where whole rows take
+// 16. A call has 4 to 5 us that do not depend on the matrix (launches, x, the cluster's sums); one row is bound by the instructions that SMs with two
+// CTAs issue (28000 x 8192 fills 220 of 296 places: 53 % of the issue slots over the SMs, DRAM at 37 %), 16 rows by the legacy tensor path besides.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -37,7 +34,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
-constexpr int BLOCK = 128;                  // inner elements that share a scale of x
+constexpr int BLOCK = 128;                  // inner elements: 64 bytes of a weight row
 constexpr int LINE = 128;                   // bytes of a weight row in a step: two blocks
 constexpr int MAX_PARTS = 8;
 
@@ -47,42 +44,87 @@ struct MatvecParams {
     void *y;
     int64_t rows, outer, sx, sc, ss, sz, sy;
     int32_t inner, group_log2, scale_type, codes_align, x_aligned;
-    uint8_t *digits;                        // x laid out in the workspace, or null: every CTA lays out what it needs
+    uint8_t *laid;                          // x laid out in the workspace, or null: every CTA lays out what it needs
     int32_t span, phase;                    // steps of a CTA's part, and of what shared memory holds of x at a time
 };
 
-// An integer v below 2^22 in magnitude, kept as MAGIC + v, read as a float is 1.5 2^23 + v.
-constexpr int32_t MAGIC = 0x4B400000;
-__device__ __forceinline__ float value_of(int32_t v) { return __int_as_float(v) - 12582912.0f; }
-
-// d = a b + d, or a b + MAGIC.
-template <bool FIRST> __device__ __forceinline__ void mma(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (FIRST)
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(MAGIC));
-    else
-        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c = a b + c, or a b: fp16 operands for rows of fp16, bf16 operands for the other types.
+template <typename T, bool FIRST> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>) {
+        if constexpr (FIRST)
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+        else
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        if constexpr (FIRST)
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+        else
+            asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
 }
+
+// (w & mask) | bits.
+template <uint32_t MASK, uint32_t BITS> __device__ __forceinline__ uint32_t masked(uint32_t w) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "n"(MASK), "r"(BITS));
+    return d;
+}
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
+// A weight row's zero point, made ready for its codes, and eight codes less the zero point: pairs of elements 0 and 4, 1 and 5,
+// 2 and 6, 3 and 7 of a word. A masked code is the low end of the significand of 1024 (fp16, where the codes four bits up
+// count 16) or of 128 (bf16); taking 1024 + zero or 128 + zero from it is exact. In bf16 that holds for zero points up to 127;
+// what larger ones are more than their low seven bits is taken off afterwards.
+template <typename T> struct Zero {
+    uint32_t low;                                                       // -(128 + zero), twice
+    // byte i of a word of zero points below 128
+    __device__ __forceinline__ Zero(uint32_t z, int i) { low = __byte_perm(z, 0xC3, 0x4040 | 0x101 * i); }
+    __device__ __forceinline__ void less(uint32_t (&a)[4], uint32_t w) const {
+        constexpr uint32_t ONE = 0x3F803F80u;
+        a[0] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w), ONE, low);
+        a[1] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 4), ONE, low);
+        a[2] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 8), ONE, low);
+        a[3] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 12), ONE, low);
+    }
+};
+template <> struct Zero<__half> {
+    uint32_t low, low16;                                                // 1024 + zero; -(64 + zero), twice
+    __device__ __forceinline__ Zero(uint32_t z, int i) {
+        low = __byte_perm(z, 0x64, 0x4040 | 0x101 * i);
+        low16 = sub_f16x2(0x63806380u, low);                            // 960 - (1024 + zero)
+    }
+    __device__ __forceinline__ void less(uint32_t (&a)[4], uint32_t w) const {
+        constexpr uint32_t SIXTEENTH = 0x2C002C00u;
+        a[0] = sub_f16x2(masked<0x000F000Fu, 0x64006400u>(w), low);
+        a[1] = fma_f16x2(masked<0x00F000F0u, 0x64006400u>(w), SIXTEENTH, low16);
+        a[2] = sub_f16x2(masked<0x000F000Fu, 0x64006400u>(w >> 8), low);
+        a[3] = fma_f16x2(masked<0x00F000F0u, 0x64006400u>(w >> 8), SIXTEENTH, low16);
+    }
+};
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-// The larger magnitude; NaN if one is.
-__device__ __forceinline__ float max_abs(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(fabsf(b)));
-    return d;
-}
-// Byte `i` of four words.
-__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
-    const uint32_t two = 0x40 + 0x11 * i;                               // byte i of the first, then of the second
-    return __byte_perm(__byte_perm(a, b, two), __byte_perm(c, d, two), 0x5410);
 }
 __device__ __forceinline__ uint4 load16(uint32_t at) {
     uint4 v;
@@ -105,25 +147,10 @@ __device__ __forceinline__ pair both(float a, float b) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
     return d;
 }
-__device__ __forceinline__ pair add2(pair a, pair b) {
-    pair d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ pair mul2(pair a, pair b) {
-    pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 __device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
     pair d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
-}
-
-// Two sums that were started at MAGIC.
-__device__ __forceinline__ pair values_of(int32_t a, int32_t b) {
-    return add2(both(__int_as_float(a), __int_as_float(b)), both(-12582912.0f, -12582912.0f));
 }
 
 // NT tiles of 8 rows of x, R tiles of 16 weight rows a warp, GROUPS = 128 / group scales of a weight row in a block.
@@ -133,109 +160,81 @@ template <typename T, int NT, int R, int GROUPS> struct Shape {
     // Two stages of 32 weight rows (three: 28000 x 8192 30.0 us, two 28.6 at the time); of 16, three with one tile of x and two with two, whose x
     // takes the room (4096 x 4096, fp32: 8 rows with 4 / 3 / 2 stages 9.7 / 7.9 / 8.1 us, 16 rows with 4 / 2 18.1 / 13.1)
     static constexpr int SLOT = 16 * R * LINE + 128, STAGES = R == 1 && NT == 1 ? 3 : 2, QUEUES = WARPS * STAGES * SLOT;
-    static constexpr int DIGITS = sizeof(T) == 4 ? 3 : 2;               // of x; the first holds the most
+    static constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;               // of x
     static constexpr int SUMS = 8 * NT * 16 * R;                        // outputs of a warp's tile
-    // x in shared memory, per row: 16 bytes for every 8 elements (their first two digits), 8 more for fp32 (the third), and per
-    // block a scale and each group's sum; paddings put rows that are read together into different banks
-    static constexpr int META = 2 * GROUPS;                             // words of a block: 1 + GROUPS, in whole loads
-    __host__ __device__ static constexpr int pitch(int steps) { return steps * 512 + 64; }
-    __host__ __device__ static constexpr int pitch3(int steps) { return DIGITS == 3 ? steps * 256 + 32 : 0; }
+    // x in shared memory, per row: 16 bytes for every 8 elements of a piece; the padding puts rows that are read together into
+    // different banks
+    static constexpr int STEP_BYTES = 512 * PIECES;                     // a row's part of a step
+    __host__ __device__ static constexpr int pitch(int steps) { return steps * STEP_BYTES + 64; }
     // shared memory: queues (in the end the warps' sums), x
     static_assert(WARPS * SUMS * 4 <= QUEUES, "the sums fit");
-    static int64_t smem(int64_t rows, int64_t steps) {
-        return QUEUES + rows * (steps * (512 + (DIGITS == 3 ? 256 : 0)) + 96) + (rows + 1) / 2 * steps * (16 * META);
-    }
+    static int64_t smem(int64_t rows, int64_t steps) { return QUEUES + rows * pitch((int)steps); }
 };
-
-// Where x is laid out: rows of 512 bytes a step (two blocks) of the first two digits, of 256 of the third (fp32), and of META
-// words a block.
-struct Layout {
-    uint8_t *x, *x3;
-    float *meta;
-    int64_t pitch, pitch3, meta_pitch;
-};
-// Where the workspace holds all steps of all rows.
-template <typename S> __host__ __device__ Layout whole_layout(uint8_t *at, int64_t rows, int64_t steps) {
-    Layout l;
-    l.pitch = steps * 512, l.pitch3 = S::DIGITS == 3 ? steps * 256 : 0, l.meta_pitch = steps * 4 * S::META;
-    l.x = at, l.x3 = at + rows * l.pitch, l.meta = reinterpret_cast<float *>(l.x3 + rows * l.pitch3);
-    return l;
-}
 
 // Lays out `steps` steps from step0 on of the rows m0 ...: per row and block 16 units of 8 elements, unit 4 c + j for word c of lane
-// j (word w of group q: c = q WORDS + w), which faces elements 32 WORDS q + 8 WORDS j + 8 w ... of the block. A unit's bytes are
-// its elements 0, 2, 4, 6 (the low nibbles of the word) and 1, 3, 5, 7.
-template <typename T, typename S>
-__device__ __forceinline__ void lay_out(const MatvecParams &p, int64_t m0, int x_rows, int step0, int steps, const Layout &to) {
-    constexpr int WORDS = S::WORDS, DIGITS = S::DIGITS;
+// j (word w of group q: c = q WORDS + w), which faces elements 32 WORDS q + 8 WORDS j + 8 w ... of the block. A unit's elements lie as the
+// codes of a word come out: 0, 4, 1, 5, 2, 6, 3, 7. An fp32 element is the sum of three bf16 ones, its upper, middle and lower 8 bits of
+// significand, exactly; they lie in 16 bytes a piece.
+template <typename T, int WORDS>
+__device__ __forceinline__ void lay_out(const MatvecParams &p, int64_t m0, int x_rows, int step0, int steps, uint8_t *to, int64_t pitch) {
+    constexpr int PIECES = sizeof(T) == 4 ? 3 : 1, AT_ONCE = PIECES == 1 ? 4 : 2;    // units that a thread has on their way
     const int count = 2 * steps, units = x_rows * count * 16;
-            for (int u0 = 0; u0 < units; u0 += THREADS) {
-                const int u = u0 + threadIdx.x, unit = u & 15, c = unit >> 2, b = (u >> 4) % count, m = (u >> 4) / count;
-                const int k = (2 * step0 + b) * BLOCK + c / WORDS * (32 * WORDS) + 8 * WORDS * (unit & 3) + 8 * (c % WORDS);
-                const bool in = u < units;
-                const T *src = reinterpret_cast<const T *>(p.x) + (m0 + (in ? m : 0)) * p.sx + k;
-                T v[8];
-                if (in && k + 8 <= p.inner && p.x_aligned) {
-    #pragma unroll
-                    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(v)[i] = reinterpret_cast<const uint4 *>(src)[i];
-                } else {
-    #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = in && k + i < p.inner ? src[i] : from_float<T>(0.0f);
-                }
-                float f[8], top = 0.0f;
-    #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = to_float(v[i]), top = max_abs(top, f[i]);
-    #pragma unroll
-                for (int o = 1; o < 16; o <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
-                // the largest magnitude becomes 127 in the first digit and 0 in the others
-                constexpr float LIMIT = DIGITS == 3 ? 127.0f * 65536.0f : 127.0f * 256.0f;
-                const bool finite = top < INFINITY;
-                const float up = !finite ? 0.0f : fminf(LIMIT / fmaxf(top, 1e-37f), 8.5070592e37f), down = !finite ? __int_as_float(0x7FC00000) : 1.0f / up;
-                // with 128 added to every digit but the first the digits are the bytes of the sum, those less 128 of them signed
-                uint32_t t[8], digit[3][2] = {};
-    #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if constexpr (DIGITS == 3) t[i] = (uint32_t)(finite ? __float2int_rn(f[i] * up) + 0x8080 : 0x8080);
-                    else t[i] = finite ? __float_as_uint(fmaf(f[i], up, 12582912.0f + 128.0f)) : 0x80u;
-                }
-                int32_t sum = 0;
-    #pragma unroll
-                for (int d = 0; d < DIGITS; ++d) {
-                    int32_t own = 0;
-    #pragma unroll
-                    for (int h = 0; h < 2; ++h) {                           // elements 0, 2, 4, 6 and 1, 3, 5, 7
-                        digit[d][h] = bytes_of(t[h], t[2 + h], t[4 + h], t[6 + h], DIGITS - 1 - d) ^ (d ? 0x80808080u : 0u);
-                        own = __dp4a((int)digit[d][h], 0x01010101, own);
-                    }
-                    sum = 256 * sum + own;
-                }
-    #pragma unroll
-                for (int o = 1; o < 4 * WORDS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);    // a group's units: below 2^30
-                if (in) {
-                    *reinterpret_cast<uint4 *>(to.x + m * to.pitch + (b * 16 + unit) * 16) = make_uint4(digit[0][0], digit[0][1], digit[1][0], digit[1][1]);
-                    if constexpr (DIGITS == 3) *reinterpret_cast<uint2 *>(to.x3 + m * to.pitch3 + (b * 16 + unit) * 8) = make_uint2(digit[2][0], digit[2][1]);
-                    float *about = to.meta + (m >> 1) * to.meta_pitch + b * (2 * S::META) + ((m0 + m) & 1);
-                    if (unit == 0) about[0] = down;
-                    if (unit % (4 * WORDS) == 0) about[2 + 2 * (unit / (4 * WORDS))] = (float)sum;
+    for (int u0 = threadIdx.x; u0 < units; u0 += AT_ONCE * THREADS) {
+        T v[AT_ONCE][8];
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) {
+            const int u = u0 + n * THREADS, unit = u & 15, c = unit >> 2, b = (u >> 4) % count, m = (u >> 4) / count;
+            const int k = (2 * step0 + b) * BLOCK + c / WORDS * (32 * WORDS) + 8 * WORDS * (unit & 3) + 8 * (c % WORDS);
+            const bool in = u < units;
+            const T *src = reinterpret_cast<const T *>(p.x) + (m0 + (in ? m : 0)) * p.sx + k;
+            if (in && k + 8 <= p.inner && p.x_aligned) {
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(v[n])[i] = reinterpret_cast<const uint4 *>(src)[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[n][i] = in && k + i < p.inner ? src[i] : from_float<T>(0.0f);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) {
+            const int u = u0 + n * THREADS, unit = u & 15, b = (u >> 4) % count, m = (u >> 4) / count;
+            if (u >= units) break;
+            uint4 *at = reinterpret_cast<uint4 *>(to + m * pitch + (b * 16 + unit) * (16 * PIECES));
+            if constexpr (PIECES == 1) {
+                const uint4 r = *reinterpret_cast<const uint4 *>(v[n]);
+                at[0] = make_uint4(__byte_perm(r.x, r.z, 0x5410), __byte_perm(r.x, r.z, 0x7632), __byte_perm(r.y, r.w, 0x5410), __byte_perm(r.y, r.w, 0x7632));
+            } else {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = to_float(v[n][i]);
+#pragma unroll
+                for (int piece = 0; piece < PIECES; ++piece) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = __byte_perm(__float_as_uint(f[i]), __float_as_uint(f[4 + i]), 0x7632);     // the upper halves
+                    at[piece] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)                          // an infinity has no rest, of a NaN a NaN is left
+                        f[i] = fabsf(f[i]) == INFINITY ? 0.0f : f[i] - __uint_as_float(__float_as_uint(f[i]) & 0xFFFF0000u);
                 }
             }
+        }
+    }
 }
 
-// x laid out once for all CTAs, which would otherwise repeat it for every 256 weight rows: a thread a unit.
-template <typename T, typename S> __global__ void __launch_bounds__(THREADS) matvec_w4_digits_kernel(const MatvecParams p, int all_steps, bool early) {
-    if (early) asm volatile("griddepcontrol.launch_dependents;");   // the product may start on its weights, and waits before it reads x
+// Rows of fp32 laid out once for all CTAs, which would otherwise split them again for every 16 or 256 weight rows: a thread a unit.
+template <typename T, int WORDS> __global__ void __launch_bounds__(THREADS) matvec_w4_layout_kernel(const MatvecParams p, int all_steps) {
     const int step = blockIdx.x * 8, m = blockIdx.y;
-    Layout to = whole_layout<S>(p.digits, p.rows, all_steps);
-    to.x += m * to.pitch + step * 512, to.x3 += m * to.pitch3 + step * 256, to.meta += (m >> 1) * to.meta_pitch + step * 4 * S::META;
-    lay_out<T, S>(p, m, 1, step, min(8, all_steps - step), to);
-    if (!early) asm volatile("griddepcontrol.launch_dependents;");
+    const int64_t pitch = all_steps * (512 * (sizeof(T) == 4 ? 3 : 1));
+    lay_out<T, WORDS>(p, m, 1, step, min(8, all_steps - step), p.laid + m * pitch + step * (pitch / all_steps), pitch);
+    asm volatile("griddepcontrol.launch_dependents;");
 }
 
 // ALONG_K: the CTA's warps share 16 R weight rows and split the inner dimension; otherwise each has rows of its own.
 template <typename T, int NT, int R, int GROUPS, bool ALONG_K, bool BYTES>
 __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParams p) {
     using S = Shape<T, NT, R, GROUPS>;
-    constexpr int WORDS = S::WORDS, STAGES = S::STAGES, STRIDE = ALONG_K ? WARPS : 1, DIGITS = S::DIGITS, STEP = 2 * BLOCK;
+    constexpr int WORDS = S::WORDS, STAGES = S::STAGES, STRIDE = ALONG_K ? WARPS : 1, PIECES = S::PIECES, STEP = 2 * BLOCK;
     extern __shared__ __align__(128) uint8_t queue[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
     const cg::cluster_group cluster = cg::this_cluster();
@@ -334,20 +333,12 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     };
     fetch(0);
 
-    // ---- x in shared memory ----
+    // ---- x in shared memory; rows of x past the last read the last: a column of the product depends on its own row alone ----
     uint8_t *xs = queue + S::QUEUES;
-    uint8_t *x3 = xs + x_rows * S::pitch(p.phase);
-    float *meta = reinterpret_cast<float *>(x3 + x_rows * S::pitch3(p.phase));      // [x row][block of the phase][META]
-    // rows of x past the last read the last: a column of the product depends on its own row alone
-    uint32_t x_at[NT], x3_at[NT];
-    uint32_t meta_at[NT];
+    uint32_t x_at[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int m = min(8 * t + g, x_rows - 1);
-        x_at[t] = (uint32_t)__cvta_generic_to_shared(xs) + m * S::pitch(p.phase) + 16 * j;
-        x3_at[t] = (uint32_t)__cvta_generic_to_shared(x3) + m * S::pitch3(p.phase) + 8 * j;
-        meta_at[t] = (uint32_t)__cvta_generic_to_shared(meta + min(4 * t + j, (x_rows - 1) >> 1) * (4 * p.phase * S::META));
-    }
+    for (int t = 0; t < NT; ++t)
+        x_at[t] = (uint32_t)__cvta_generic_to_shared(xs) + min(8 * t + g, x_rows - 1) * S::pitch(p.phase) + 16 * PIECES * j;
 
     pair acc[R][NT][2];                                                 // weight rows row + 8 h, rows 2 j and 2 j + 1 of x
 #pragma unroll
@@ -366,23 +357,17 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
     for (int phase0 = 0; phase0 < steps; phase0 += p.phase) {
         if (phase0) __syncthreads();                                    // the last phase's x has been read
         const int count = min(p.phase, steps - phase0);
-        if (p.digits) {                                                 // 16 bytes at a time, as they lie in the workspace
-            const Layout from = whole_layout<S>(p.digits, p.rows, (p.inner + STEP - 1) / STEP);
+        if (p.laid) {                                                   // 16 bytes at a time, as they lie in the workspace
+            const int64_t pitch = (int64_t)((p.inner + STEP - 1) / STEP) * S::STEP_BYTES;
             if (phase0 == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-            auto copy = [&](uint8_t *to, int to_pitch, const uint8_t *src, int64_t src_pitch, int row_bytes, int rows_of) {
-                for (int m = warp; m < rows_of; m += WARPS)
+            const uint8_t *src = p.laid + m0 * pitch + (int64_t)(step0 + phase0) * S::STEP_BYTES;
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(xs);
+            for (int m = warp; m < x_rows; m += WARPS)
 #pragma unroll 4
-                    for (int i = 16 * lane; i < row_bytes; i += 512) copy16((uint32_t)__cvta_generic_to_shared(to + m * to_pitch + i), src + m * src_pitch + i);
-            };
-            const int64_t at = step0 + phase0;
-            copy(xs, S::pitch(p.phase), from.x + m0 * from.pitch + at * 512, from.pitch, count * 512, x_rows);
-            if constexpr (DIGITS == 3) copy(x3, S::pitch3(p.phase), from.x3 + m0 * from.pitch3 + at * 256, from.pitch3, count * 256, x_rows);
-            copy(reinterpret_cast<uint8_t *>(meta), 16 * S::META * p.phase,
-                 reinterpret_cast<const uint8_t *>(from.meta + m0 / 2 * from.meta_pitch + at * 4 * S::META), 4 * from.meta_pitch, count * 16 * S::META,
-                 (x_rows + 1) / 2);
+                for (int i = 16 * lane; i < count * S::STEP_BYTES; i += 512) copy16(to + m * S::pitch(p.phase) + i, src + m * pitch + i);
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
         } else {
-            lay_out<T, S>(p, m0, x_rows, step0 + phase0, count, {xs, x3, meta, S::pitch(p.phase), S::pitch3(p.phase), 4 * p.phase * S::META});
+            lay_out<T, WORDS>(p, m0, x_rows, step0 + phase0, count, xs, S::pitch(p.phase));
         }
         __syncthreads();
         const int phase_end = phase0 + count;
@@ -412,80 +397,92 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
             const uint32_t wat = slot + row * LINE + (((WORDS * j >> 2) ^ (row & 7)) * 16) + (4 * WORDS * j & 15);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                pair about[NT][S::META];                                // the block's scales, then its groups' sums
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int i = 0; i <= GROUPS; i += 2) {
-                        const uint32_t from = meta_at[t] + (b0 + b) * (8 * S::META) + 8 * i;
-                        if (i < GROUPS) asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(about[t][i]), "=l"(about[t][i + 1]) : "r"(from) : "memory");
-                        else asm volatile("ld.shared.u64 %0, [%1];" : "=l"(about[t][i]) : "r"(from) : "memory");
-                    }
 #pragma unroll
                 for (int q = 0; q < GROUPS; ++q) {
-                    uint4 x12[NT][WORDS];
-                    uint2 x3v[NT][WORDS];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                        for (int i = 0; i < WORDS; ++i) {
-                            x12[t][i] = load16(x_at[t] + (b0 + b) * 256 + (q * WORDS + i) * 64);
-                            x3v[t][i] = make_uint2(0, 0);
-                            if constexpr (DIGITS == 3)
-                                asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x3v[t][i].x), "=r"(x3v[t][i].y)
-                                             : "r"(x3_at[t] + (b0 + b) * 128 + (q * WORDS + i) * 32) : "memory");
-                        }
-                    }
                     constexpr int LAST = LOADS - 1;
                     const int load = GROUPS == 4 ? b & LAST : 0;
                     const int from = (lane & ~3) | (GROUPS == 1 ? (turn & 1) * 2 + b : GROUPS == 2 ? 2 * b + q : q);
                     const uint32_t z = __shfl_sync(0xffffffffu, zeros[load], from);
+                    // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of the rows 16 r + row + 8 h
+                    uint32_t w[R][2][WORDS];
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        pair s2[2], z2[2];                              // scales and zero points, the latter negative
-                        uint32_t w[2][WORDS];
+                    for (int r = 0; r < R; ++r)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float s = __uint_as_float(__shfl_sync(0xffffffffu, scale[load][2 * r + h], from));
-                            const float minus = -value_of(MAGIC | (z >> (16 * r + 8 * h) & 255));
-                            s2[h] = both(s, s), z2[h] = both(minus, minus);
-                            // WORDS words of codes from byte 64 b + 16 WORDS q + 4 WORDS j of row 16 r + row + 8 h
-                            load_words(w[h], (wat ^ (64 * b + 16 * WORDS * q)) + (16 * r + 8 * h) * LINE);
+                            load_words(w[r][h], (wat ^ (64 * b + 16 * WORDS * q)) + (16 * r + 8 * h) * LINE);
                             if constexpr (BYTES) {
                                 const int next = 16 * b + 4 * WORDS * q + WORDS * j + WORDS;    // the word after them
                                 uint32_t v[1];
                                 load_words(v, next == LINE / 4 ? slot + 16 * R * LINE + 4 * (16 * r + row + 8 * h)
                                                                : slot + (16 * r + row + 8 * h) * LINE + ((next >> 2) ^ (row & 7)) * 16 + 4 * (next & 3));
 #pragma unroll
-                                for (int i = 0; i < WORDS; ++i) w[h][i] = __funnelshift_r(w[h][i], i + 1 < WORDS ? w[h][i + 1] : v[0], before >> (8 * (2 * r + h)));
+                                for (int i = 0; i < WORDS; ++i) w[r][h][i] = __funnelshift_r(w[r][h][i], i + 1 < WORDS ? w[r][h][i + 1] : v[0], before >> (8 * (2 * r + h)));
                             }
                         }
-                        int32_t sum[NT][DIGITS][4];
+                    const uint32_t z7 = std::is_same_v<T, __half> ? z : z & 0x7F7F7F7Fu;
+                    const Zero<T> zero[4] = {{z7, 0}, {z7, 1}, {z7, 2}, {z7, 3}};
+                    // the first piece of x, and the smaller ones by themselves, whose sums would be rounded to the first's
+                    float sum[R][NT][4], small[PIECES > 1 ? R : 1][NT][4];
 #pragma unroll
-                        for (int i = 0; i < WORDS; ++i) {
-                            constexpr uint32_t LOW = 0x0F0F0F0Fu;
-                            const uint32_t a[4] = {w[0][i] & LOW, w[1][i] & LOW, w[0][i] >> 4 & LOW, w[1][i] >> 4 & LOW};
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                const uint32_t x[6] = {x12[t][i].x, x12[t][i].y, x12[t][i].z, x12[t][i].w, x3v[t][i].x, x3v[t][i].y};
-#pragma unroll
-                                for (int d = 0; d < DIGITS; ++d) {
-                                    if (i == 0) mma<true>(sum[t][d], a, x[2 * d], x[2 * d + 1]);
-                                    else mma<false>(sum[t][d], a, x[2 * d], x[2 * d + 1]);
-                                }
-                            }
-                        }
+                    for (int i = 0; i < WORDS; ++i) {
+                        uint4 x[NT][PIECES];
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                pair v = values_of(sum[t][0][2 * h], sum[t][0][2 * h + 1]);
+                            for (int piece = 0; piece < PIECES; ++piece)
+                                x[t][piece] = load16(x_at[t] + (b0 + b) * (256 * PIECES) + (q * WORDS + i) * (64 * PIECES) + 16 * piece);
 #pragma unroll
-                                for (int d = 1; d < DIGITS; ++d) v = fma2(v, both(256.0f, 256.0f), values_of(sum[t][d][2 * h], sum[t][d][2 * h + 1]));
-                                v = fma2(z2[h], about[t][1 + q], v);
-                                acc[r][t][h] = fma2(v, mul2(about[t][0], s2[h]), acc[r][t][h]);
+                        for (int r = 0; r < R; ++r) {
+                            uint32_t a0[4], a1[4];
+                            zero[2 * r].less(a0, w[r][0][i]);
+                            zero[2 * r + 1].less(a1, w[r][1][i]);
+                            const uint32_t low[4] = {a0[0], a1[0], a0[1], a1[1]}, high[4] = {a0[2], a1[2], a0[3], a1[3]};
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                if (i == 0) mma<T, true>(sum[r][t], low, x[t][0].x, x[t][0].y);
+                                else mma<T, false>(sum[r][t], low, x[t][0].x, x[t][0].y);
+                                mma<T, false>(sum[r][t], high, x[t][0].z, x[t][0].w);
+                                if constexpr (PIECES > 1) {
+                                    if (i == 0) mma<T, true>(small[r][t], low, x[t][2].x, x[t][2].y);
+                                    else mma<T, false>(small[r][t], low, x[t][2].x, x[t][2].y);
+                                    mma<T, false>(small[r][t], high, x[t][2].z, x[t][2].w);
+                                    mma<T, false>(small[r][t], low, x[t][1].x, x[t][1].y);
+                                    mma<T, false>(small[r][t], high, x[t][1].z, x[t][1].w);
+                                }
                             }
+                        }
                     }
+                    if constexpr (!std::is_same_v<T, __half>) {
+                        if (__any_sync(0xffffffffu, z & 0x80808080u)) {  // zero points from 128 on: what they are more than their low seven bits
+#pragma unroll
+                            for (int i = 0; i < WORDS; ++i)
+#pragma unroll
+                                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                                    for (int piece = 0; piece < PIECES; ++piece) {
+                                        const uint4 x = load16(x_at[t] + (b0 + b) * (256 * PIECES) + (q * WORDS + i) * (64 * PIECES) + 16 * piece);
+#pragma unroll
+                                        for (int r = 0; r < R; ++r) {
+                                            const uint32_t d0 = z >> (16 * r + 7) & 1 ? 0xC300C300u : 0u, d1 = z >> (16 * r + 15) & 1 ? 0xC300C300u : 0u;
+                                            const uint32_t a[4] = {d0, d1, d0, d1};                     // -128 or 0
+                                            mma<T, false>(piece ? small[r][t] : sum[r][t], a, x.x, x.y);
+                                            mma<T, false>(piece ? small[r][t] : sum[r][t], a, x.z, x.w);
+                                        }
+                                    }
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float s = __uint_as_float(__shfl_sync(0xffffffffu, scale[load][2 * r + h], from));
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                float lo = sum[r][t][2 * h], hi = sum[r][t][2 * h + 1];
+                                if constexpr (PIECES > 1) lo += small[r][t][2 * h], hi += small[r][t][2 * h + 1];
+                                acc[r][t][h] = fma2(both(lo, hi), both(s, s), acc[r][t][h]);
+                            }
+                        }
                 }
             }
             slot = slot == at0 + (STAGES - 1) * S::SLOT ? at0 : slot + S::SLOT;
@@ -542,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 struct Plan {
     bool along_k;
     int parts;
-    size_t digits;                          // bytes of x laid out in the workspace, 0: in every CTA
+    size_t laid;                            // bytes of x laid out in the workspace, 0: in every CTA
 };
 
 template <typename T, int NT, int R, int GROUPS, bool ALONG_K, bool BYTES> int launch(MatvecParams p, const Plan &plan, cudaStream_t s) {
@@ -561,12 +558,9 @@ template <typename T, int NT, int R, int GROUPS, bool ALONG_K, bool BYTES> int l
         if (dev >= 0 && dev < 64) known[dev] = true;
     }
     const dim3 grid((unsigned)(cdiv(p.outer, ALONG_K ? 16 * R : 16 * R * WARPS) * plan.parts), (unsigned)cdiv(p.rows, 8 * NT));
-    if (plan.digits) {
+    if (plan.laid) {
         const dim3 laying((unsigned)cdiv(all_steps, 8), (unsigned)p.rows);
-        // The product starts while x is laid out, unless its clusters would then not all find room at once: 4096 x 4096, one
-        // row, 256 + 2 CTAs: 5.8 us, after it 6.4; 8192 x 8192, 5 rows, bf16, 32 clusters + 20 CTAs: 17.5 us, after it 12.9.
-        const bool early = plan.parts == 1 || (int64_t)grid.x * grid.y + (int64_t)laying.x * laying.y <= 272;
-        matvec_w4_digits_kernel<T, S><<<laying, THREADS, 0, s>>>(p, all_steps, early);
+        matvec_w4_layout_kernel<T, S::WORDS><<<laying, THREADS, 0, s>>>(p, all_steps);
         launches = 2;
     }
     cudaLaunchConfig_t cfg = {};
@@ -582,7 +576,7 @@ template <typename T, int NT, int R, int GROUPS, bool ALONG_K, bool BYTES> int l
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = plan.digits ? 2 : 1;
+    cfg.numAttrs = plan.laid ? 2 : 1;
     PITON_CUDA(cudaLaunchKernelEx(&cfg, matvec_w4_kernel<T, NT, R, GROUPS, ALONG_K, BYTES>, p));
     return check_launch("matvec_w4", launches);
 }
@@ -617,14 +611,11 @@ Plan plan_of(const piton_matvec_w4_args *a) {
         while (2 * parts <= most && tiles * 2 * parts <= 2 * sms && steps >= WARPS * 2 * parts) parts *= 2;
     }
     plan.parts = (int)parts;
-    // More than 2048 elements of x a CTA are laid out once in the workspace, by a kernel of their own (bf16, 8192 elements, 4 rows
-    // by 2048 x 2048: 4.6 us, in every CTA 6.0; 2048 elements, 8 rows by 8192 x 2048: 7.1 and 6.7; 65536 elements, 16 rows by
-    // 4096 x 4096: 9.3 and 28).
-    const int64_t x_rows = a->rows < 16 ? a->rows : 16;
-    if (x_rows * cdiv(steps, parts) * 2 * BLOCK > 2048) {
-        const int64_t fp32 = a->type == PITON_B200_TYPE_F32;
-        plan.digits = (size_t)(a->rows * steps) * (512 + (fp32 ? 256 : 0)) + (size_t)((a->rows + 1) / 2 * steps) * (32 * (128 / a->group));
-    }
+    // More than 8192 elements of x a CTA are laid out once, in the workspace, by a kernel of their own (bf16, 16 rows by 4096 x 4096: 9.9 us,
+    // in every CTA 11.8; fewer do not repay its launch), and more than 2048 of fp32, whose split into pieces is ten times the work.
+    const bool fp32 = a->type == PITON_B200_TYPE_F32;
+    const int64_t together = fp32 ? 8 : 16, x_rows = a->rows < together ? a->rows : together;
+    if (x_rows * cdiv(steps, parts) * 2 * BLOCK > (fp32 ? 2048 : 8192)) plan.laid = (size_t)(a->rows * steps) * (fp32 ? 1536 : 512);
     return plan;
 }
 
@@ -650,7 +641,7 @@ using namespace piton::decode;
 
 extern "C" size_t piton_b200_matvec_w4_workspace_size(const piton_matvec_w4_args *a) {
     if (check_matvec(a) != PITON_B200_OK || a->rows == 0 || a->outer == 0) return 0;
-    return plan_of(a).digits;
+    return plan_of(a).laid;
 }
 
 extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream) {
@@ -658,12 +649,12 @@ extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream)
     if (a->rows == 0 || a->outer == 0) return PITON_B200_OK;
     PITON_REQUIRE(a->y && (a->inner == 0 || (a->x && a->codes && a->scales)), "NULL pointer");
     const Plan plan = plan_of(a);
-    if (plan.digits && (!a->workspace || a->workspace_bytes < plan.digits))
+    if (plan.laid && (!a->workspace || a->workspace_bytes < plan.laid))
         return set_error(PITON_B200_EWORKSPACE, "workspace of %llu bytes, %llu needed", (unsigned long long)a->workspace_bytes,
-                         (unsigned long long)plan.digits);
-    PITON_REQUIRE(a->workspace % 16 == 0 || !plan.digits, "workspace is not 16-byte aligned");
+                         (unsigned long long)plan.laid);
+    PITON_REQUIRE(a->workspace % 16 == 0 || !plan.laid, "workspace is not 16-byte aligned");
     MatvecParams p;
-    p.digits = plan.digits ? reinterpret_cast<uint8_t *>(a->workspace) : nullptr;
+    p.laid = plan.laid ? reinterpret_cast<uint8_t *>(a->workspace) : nullptr;
     p.x = reinterpret_cast<const void *>(a->x);
     p.codes = reinterpret_cast<const uint8_t *>(a->codes);
     p.scales = reinterpret_cast<const void *>(a->scales);
@@ -679,6 +670,7 @@ extern "C" int piton_b200_matvec_w4(const piton_matvec_w4_args *a, void *stream)
     return with_type(a->type, [&](auto t) {
         using T = decltype(t);
         cudaStream_t s = as_stream(stream);
-        return a->rows <= 8 ? launch<T, 1>(p, plan, s) : launch<T, 2>(p, plan, s);
+        if constexpr (sizeof(T) == 4) return launch<T, 1>(p, plan, s);  // (three pieces of 16 rows would leave no room for steps)
+        else return a->rows <= 8 ? launch<T, 1>(p, plan, s) : launch<T, 2>(p, plan, s);
     });
 }

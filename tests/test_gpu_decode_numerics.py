@@ -30,3 +30,89 @@ def test_matvec_zero_points_of_any_byte(cuda, dtype, rows, inner, outer, group):
         want, size = ref.matvec_w4(x, codes, scales, zeros, None, group)
         tol = (inner / 16 + 32) * 2 * EPS * size + ROUND[dtype] * want.abs() + 1e-7 * (dtype == torch.float16)
         assert ((y.cpu().double() - want).abs() <= tol).all()
+
+
+# A product's operands are exact (4-bit codes less their zero points, and x, fp32 in three pieces), so what is left are the fp32 sums
+# of test_gpu_decode.py's bound, (n / 16 + 32) 2 eps of sum |x w|: something large that faces a weight of zero adds nothing to it.
+
+def product_bound(dtype, inner, want, size):
+    return (inner / 16 + 32) * 2 * EPS * size + ROUND[dtype] * want.abs() + 1e-7 * (dtype == torch.float16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,inner,outer", [(1, 256, 40), (3, 4096, 64), (9, 2304, 72), (2, 1280, 4800)])
+@pytest.mark.parametrize("times", [1e3, 5e3, 1e9])
+def test_matvec_channels_that_face_zero_weights(cuda, dtype, rows, inner, outer, times):
+    # one channel of every 128 is `times` the others and its weights sit at the zero point
+    if dtype == torch.float16 and times > 1e4:
+        pytest.skip("past the type's range")
+    g = gen(rows)
+    x = torch.randn((rows, inner), generator=g, device="cuda")
+    x[:, 4::128] = times * (1 + torch.rand((rows, inner // 128), generator=g, device="cuda"))
+    x = x.to(dtype)
+    codes = torch.randint(0, 256, (outer, inner // 2), generator=g, device="cuda", dtype=torch.uint8)
+    codes[:, 2::64] = codes[:, 2::64] & 0xF0 | 8
+    scales = (torch.rand((outer, inner // 64), generator=g, device="cuda") * 0.1).to(dtype)
+    y = decode.matvec_w4(x, codes, scales, group=64)
+    want, size = ref.matvec_w4(x, codes, scales, None, None, 64)
+    assert float(size.max()) < 1e5
+    assert ((y.cpu().double() - want).abs() <= product_bound(dtype, inner, want, size)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,inner,outer", [(1, 128, 24), (5, 1280, 48), (16, 4096, 33), (2, 1280, 4800)])
+def test_matvec_codes_around_the_zero_point(cuda, dtype, group, rows, inner, outer):
+    # x of one sign; groups whose codes all equal the zero point give exactly 0, others lie one step to either side of it
+    g = gen(inner + group)
+    x = (0.8 + 0.2 * torch.rand((rows, inner), generator=g, device="cuda")).to(dtype)
+    scales = (0.5 + torch.rand((outer, inner // group), generator=g, device="cuda")).to(dtype)
+    zeros = torch.randint(1, 15, (outer, inner // group), generator=g, device="cuda", dtype=torch.uint8)
+    for spread in (0, 1):
+        off = torch.randint(-spread, spread + 1, (outer, inner), generator=g, device="cuda")
+        off[::3] = 0
+        code = zeros.repeat_interleave(group, 1).int() + off
+        codes = (code[:, 0::2] | code[:, 1::2] << 4).to(torch.uint8)
+        y = decode.matvec_w4(x, codes, scales, group=group, zeros=zeros)
+        want, size = ref.matvec_w4(x, codes, scales, zeros, None, group)
+        assert bool((y.cpu()[:, ::3] == 0).all()) and bool((size[:, ::3] == 0).all())
+        assert ((y.cpu().double() - want).abs() <= product_bound(dtype, inner, want, size)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,inner,outer", [(4, 256, 40), (8, 4096, 64), (8, 1280, 4800)])
+def test_matvec_keeps_every_bit_of_an_element(cuda, dtype, rows, inner, outer):
+    # each row of x has one element of its type's full significand, from 2^-100 to 2^100 (fp16: 2^-8 to 2^8), beside larger ones that face
+    # weights of zero.  The product is then one term: its pieces' sum and the scale are rounded, 8 eps at most
+    g = gen(inner)
+    top = 8 if dtype == torch.float16 else 100
+    lone = torch.ldexp(1 + torch.rand(rows, generator=g, device="cuda"), torch.randint(-top, top, (rows,), generator=g, device="cuda"))
+    x = torch.zeros((rows, inner), device="cuda")
+    x[:, 0::2] = torch.ldexp(torch.ones_like(x[:, 0::2]), torch.tensor(min(top + 6, 100), device="cuda"))
+    at = 2 * torch.randint(0, inner // 2, (rows,), generator=g, device="cuda") + 1
+    x[torch.arange(rows, device="cuda"), at] = lone
+    x = x.to(dtype)
+    codes = torch.randint(0, 16, (outer, inner // 2), generator=g, device="cuda", dtype=torch.uint8) << 4 | 8     # even elements: zero
+    scales = torch.rand((outer, inner // 128), generator=g, device="cuda")
+    y = decode.matvec_w4(x, codes, scales)
+    want, _ = ref.matvec_w4(x, codes, scales, None, None, 128)
+    want = want.clamp(-65504.0, 65504.0) if dtype == torch.float16 else want
+    round_ = 0.0 if dtype == torch.float32 else ROUND[dtype]
+    small = 2.0 ** -24 if dtype == torch.float16 else 0.0
+    assert ((y.cpu().double() - want).abs() <= (8 * EPS + round_) * want.abs() + small).all()
+
+
+def test_matvec_infinite_elements(cuda):
+    # infinity times a weight: of the weight's sign, NaN where the weight is zero; the other rows are as without it
+    g = gen(0)
+    codes = torch.randint(0, 256, (60, 256), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.rand((60, 4), generator=g, device="cuda") + 0.1
+    weight = (codes[:, 100] >> 4).double().cpu() - 8              # of element 201
+    for dtype in TYPES:
+        x = torch.randn((3, 512), generator=g, device="cuda").to(dtype)
+        clean = decode.matvec_w4(x, codes, scales)
+        x[1, 201] = float("inf")
+        y = decode.matvec_w4(x, codes, scales)
+        assert torch.equal(y[[0, 2]], clean[[0, 2]])
+        want = weight * float("inf")
+        assert torch.equal(y[1].cpu().double().nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
