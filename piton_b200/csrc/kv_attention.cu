@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 // The reference of the exponents: the largest score so far; 16-bit rows let a score pass it by up to 2^SLACK, so
                 // that O is rarely rescaled, which LIFT leaves room for in the weights' fp16.
-                const float now = SPLIT ? fmaxf(m[n][e], top) : top > m[n][e] + SLACK ? top : m[n][e];
-                const float ref = (now == -INFINITY ? 0.0f : now) - LIFT;
+                const float now = SPLIT ? fmaxf(m[n][e], top) : top - m[n][e] > SLACK ? top : m[n][e];
+                const float ref = now == -INFINITY ? 0.0f : now;
                 alpha[n][e] = now == m[n][e] ? 1.0f : ex2(m[n][e] - now);
                 m[n][e] = now;
                 float sum = 0.0f;
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
                 for (int t = 0; t < TILES; ++t)
 #pragma unroll
                     for (int x = e; x < 4; x += 2) {
-                        c[t][n][x] = ex2(c[t][n][x] - ref);
+                        c[t][n][x] = ex2(c[t][n][x] - ref + LIFT);  // (ref - LIFT could be rounded to less, and the weight pass fp16)
                         sum += c[t][n][x];
                     }
                 l[n][e] = l[n][e] * alpha[n][e] + sum;

@@ -9,7 +9,7 @@ import torch
 
 import decode_ref as ref
 from piton_b200 import decode
-from test_gpu_decode import EPS, ROUND, TYPES, gen
+from test_gpu_decode import EPS, ROUND, TYPES, gen, page_table, random_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +116,43 @@ def test_matvec_infinite_elements(cuda):
         assert torch.equal(y[[0, 2]], clean[[0, 2]])
         want = weight * float("inf")
         assert torch.equal(y[1].cpu().double().nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+
+
+# ---- attention ----
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim,group", [(32, 1), (64, 5), (128, 16)])
+def test_attention_scores_of_any_size(cuda, dtype, dim, group):
+    # scores from 2^20 to 2^60, where a step of fp32 is more than the weights' whole range: rows stay averages of values
+    lengths = [300, 77, 900]
+    table, pages = page_table([-(-n // 16) for n in lengths], 60, 3)
+    cache = random_cache(pages, 1, 16, dim, 3)
+    top = float((cache[1].float() * cache[3][..., None, None]).abs().max())
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for power in range(20, 61):
+        q = torch.randn((3, group, dim), generator=gen(power), device="cuda") * 2.0 ** (power - 3)
+        out, lse = decode.kv_attention(q.to(dtype), tuple(cache), table.cuda(), lens, return_lse=True)
+        assert float(out.float().abs().max()) <= top * (1 + 2.0 ** -6), power      # (also false for NaN)
+        assert bool(torch.isfinite(lse).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_score_one_step_above_a_large_one(cuda, dtype):
+    # scores of 2^p and the next fp32 number above, 256 keys apart (the same warp's next keys): the reference of the weights may lag
+    # the maximum, but by what the weights' fp16 has room for
+    for power in range(20, 32):
+        cache = [torch.zeros((33, 1, 16, 32), dtype=torch.uint8, device="cuda").view(ref.E4M3) for _ in range(2)]
+        scales = [torch.ones((33, 1), device="cuda") for _ in range(2)]
+        cache[0][0, 0, 3, 0], cache[0][16, 0, 5, 0], cache[0][16, 0, 5, 1] = 128.0, 128.0, 16.0
+        cache[1][0, 0, 3], cache[1][16, 0, 5] = 1.0, 3.0
+        step = 2.0 ** (power - 23)
+        if step / 16 < 2.0 ** -9 or (dtype == torch.float16 and power > 22):
+            continue
+        q = torch.zeros((1, 1, 32), device="cuda")
+        q[0, 0, 0], q[0, 0, 1] = 2.0 ** (power - 7), step / 16
+        table = torch.arange(33, dtype=torch.int32, device="cuda")[None]
+        out = decode.kv_attention(q.to(dtype), (*cache, *scales), table, torch.tensor([500], dtype=torch.int32, device="cuda"),
+                                  scale=0.6931471805599453, max_length=1).float()
+        w = 2.0 ** -step
+        want = (w * 1.0 + 3.0) / (w + 1.0)
+        assert float((out - want).abs().max()) <= 2.0 ** -7 * want, (power, out.flatten()[0].item(), want)
