@@ -13,7 +13,10 @@
 // The weights p become fp16 too: an 11-bit rounding of each for 16-bit rows, no coarser than the output's for fp16, and two halves
 // for fp32.  Products are exact in the fp32 accumulators.  Weights are kept as 2^LIFT p relative to a reference that may lag the running
 // maximum by 2^SLACK (16-bit rows), so O is rarely rescaled and the products add straight into its registers; fp32 rows add a
-// stage's sums to O in fp32 instead.
+// stage's sums to O in fp32 instead.  The pages' V scales go into the weights relative to a reference
+// that a tile's scale passes by no more than 2^6 downwards: weights down to 2^-19 of the row's largest keep their 11 bits, those
+// below 2^-30 are lost. The reference moves with the scales, up or down, and the sums so far move in fp32, so what a row
+// adds up from pages of small values does not depend on larger ones that it does not see or hardly weighs (within 2^80 of them).
 //
 // The order of dimensions inside an MMA's k index is free as long as K and Q agree, so a lane copies (cp.async) the 16 bytes
 // of a key row that its own fragment holds, or whole rows go into one copy where they are 128 bytes, and the same for V with
@@ -39,6 +42,8 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// V scales more than 2^NEAR below their reference move it, though not 2^MOST below the largest: what has been added up stays in fp32's range.
+constexpr int NEAR = 6, MOST = 80;
 constexpr uint32_t BAD_PAGE = 0x7FC0DEADu;   // in a stage's scale slot: the tile's page was not followed
 
 struct CachedParams {
@@ -144,6 +149,15 @@ template <typename T> __device__ __forceinline__ void load_four(float (&x)[4], c
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = to_float(v[e]);
 }
+// The biased exponent of a positive normal number up to 2^126, 0 for anything else.
+__device__ __forceinline__ int exponent(float x) {
+    const uint32_t e = __float_as_uint(x) >> 23;
+    return e <= 253 ? (int)e : 0;
+}
+__device__ __forceinline__ float power(int e) { return __int_as_float(e + 127 << 23); }      // 2^e, -126 <= e <= 127
+// An exponent to move sums by as a byte, and the factor: sums that move down by more than 2^126 are none.
+__device__ __forceinline__ uint32_t move_by(int e) { return (uint32_t)(max(e, -127) + 128); }
+__device__ __forceinline__ float move_of(uint32_t byte) { return __uint_as_float(byte - 1 << 23); }
 // NaN codes (7F and FF) of a word: a set high bit in each such byte.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
@@ -161,7 +175,7 @@ template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_attention_kernel(const CachedParams p) {
     using G = Geometry<D>;
     constexpr bool SPLIT = sizeof(T) == 4;              // fp32 rows: queries and weights as pairs of halves
-    constexpr float LIFT = SPLIT ? 14.0f : 6.0f, SLACK = SPLIT ? 0.0f : 8.0f;
+    constexpr float LIFT = SPLIT ? 14.0f : 11.0f, SLACK = SPLIT ? 0.0f : 4.0f, UNLIFT = SPLIT ? 0x1p-14f : 0x1p-11f;
     constexpr int R = 8 * NQ, KW = G::KB / 4, VW = G::VB / 4, MT = D / 16, KT = D / 16, TILES = G::TILES, KEYS = G::KEYS;
     extern __shared__ __align__(16) uint8_t ring[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
@@ -360,7 +374,9 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.0f;
-    float vref = 0.0f;                                  // 16-bit rows: O is kept relative to the largest V scale so far
+    // O (fp32 rows: a stage's sums) is kept relative to a power of two that the tiles' V scales lie close below: its exponent as in the bits of
+    // a float, 0 before the first, and the largest it has been.
+    int vref = 0, vmax = 0;
 
 #pragma unroll 1
     for (int s = 0; s < stages; ++s) {
@@ -368,7 +384,8 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
         const uint32_t at = (s & 1) * G::BYTES;
         wait<2>();                                      // the next stage's keys and this one's values may be on their way
         __syncwarp();                                   // copies of other lanes
-        float kscale[TILES], weight[TILES], vtop = 0.0f;
+        float kscale[TILES], weight[TILES];
+        int vtop = 0, vlow = 255;
         uint32_t bad = 0;                               // tiles whose page was not followed
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
@@ -377,21 +394,36 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
             bad |= (uint32_t)(sc[0] == BAD_PAGE) << t;
             kscale[t] = __uint_as_float(sc[0]);
             weight[t] = sc[0] == BAD_PAGE ? 0.0f : __uint_as_float(sc[1]);
-            vtop = fmaxf(vtop, weight[t]);
+            const int e = exponent(weight[t]);
+            if (e > 0) vtop = max(vtop, e), vlow = min(vlow, e);
         }
-        // the tiles' V scales relative to the largest, so that the weights keep fp16's range
-        if (!(vtop > 0.0f && vtop < INFINITY)) vtop = vref > 0.0f ? vref : 1.0f;
-        float shrink = 1.0f;
-        if constexpr (!SPLIT) {
-            if (vtop > vref) shrink = vref / vtop, vref = vtop;
-            vtop = vref;
-        }
+        // The tiles' V scales relative to the reference go into the weights. It moves, and what has been added up with it, when a tile's
+        // scale is above it or too far below for fp16.
+        uint32_t moves = 0;                             // byte t: 128 more than the exponent that the sums move by before tile t, 0: they do not
+        const int rtop = SPLIT ? vtop : max(vtop, vref);
         bool level = true;
+        if (vlow >= rtop - NEAR) {                      // close together (or no scale at all)
+            if (!SPLIT && vref && rtop > vref) moves = move_by(vref - rtop);
+            vref = rtop;
+            vmax = max(vmax, vref);
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) level = level && weight[t] == vtop;
-        if (!level) {
+            for (int t = 0; t < TILES; ++t) level = level && __float_as_int(weight[t]) == vref << 23;
+            if (!level && vref) {
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) weight[t] = weight[t] == vtop ? 1.0f : weight[t] / vtop;
+                for (int t = 0; t < TILES; ++t) weight[t] *= power(127 - vref);
+            }
+            level = level && vref;                      // without a reference the weights are the scales: zeros, or not numbers
+        } else {
+            level = false;
+            if (SPLIT) vref = vmax = 0;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                const int e = exponent(weight[t]), next = !e ? vref : e > vref ? e : e < vref - NEAR ? max(e, vmax - MOST) : vref;
+                if (vref && next != vref) moves |= move_by(vref - next) << (8 * t);
+                vref = next;
+                vmax = max(vmax, next);
+                if (vref) weight[t] *= power(127 - vref);
+            }
         }
 
         // ---- scores ----
@@ -482,7 +514,8 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
         wait<1>();                                      // the keys after the next may be on their way
         float acc[SPLIT ? MT : 1][NQ][4];               // fp32 rows: a stage's sums, added to O in fp32
         if constexpr (!SPLIT) {
-            bool moved = shrink != 1.0f;
+            const float shrink = moves & 255 ? move_of(moves & 255) : 1.0f;
+            bool moved = moves & 255;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) moved = moved || alpha[n][0] != 1.0f || alpha[n][1] != 1.0f;
             if (__any_sync(0xffffffffu, moved)) {
@@ -548,6 +581,18 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
                     }
                 }
             }
+            if (t > 0 && moves >> (8 * t) & 255) {
+                const float move = move_of(moves >> (8 * t) & 255);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (SPLIT) acc[i][n][e] *= move;
+                            else o[i][n][e] *= move;
+                        }
+            }
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
                 uint32_t a[2][4];
@@ -567,12 +612,13 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
             }
         }
         if constexpr (SPLIT) {
+            const float back = (vref ? power(vref - 127) : 1.0f) * UNLIFT;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(o[i][n][e], alpha[n][e & 1], acc[i][n][e] * vtop);
+                    for (int e = 0; e < 4; ++e) o[i][n][e] = fmaf(o[i][n][e], alpha[n][e & 1], acc[i][n][e] * back);
         }
         issue_v(s + 1);
     }
@@ -583,7 +629,7 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            m[n][e] -= LIFT;                            // l and O are 2^LIFT times what belongs to m
+            l[n][e] *= UNLIFT;
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
@@ -597,7 +643,7 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
         for (int e = 0; e < 2; ++e) {
             const int r = 8 * n + 2 * j + e;
             if (g == 0) sml[warp * R + r] = make_float2(m[n][e], l[n][e]);
-            const float back = SPLIT ? 1.0f : vref;
+            const float back = SPLIT ? 1.0f : (vref ? power(vref - 127) : 1.0f) * UNLIFT;
             float *to = so + (warp * R + r) * D + g * G::VB;
 #pragma unroll
             for (int i = 0; i < MT; ++i) *reinterpret_cast<float2 *>(to + 2 * i) = make_float2(o[i][n][e] * back, o[i][n][e + 2] * back);

@@ -9,7 +9,7 @@ import torch
 
 import decode_ref as ref
 from piton_b200 import decode
-from test_gpu_decode import EPS, ROUND, TYPES, gen, page_table, random_cache
+from test_gpu_decode import EPS, ROUND, TYPES, bound, gen, offsets, page_table, random_cache, status
 
 pytestmark = pytest.mark.gpu
 
@@ -156,3 +156,97 @@ def test_attention_score_one_step_above_a_large_one(cuda, dtype):
         w = 2.0 ** -step
         want = (w * 1.0 + 3.0) / (w + 1.0)
         assert float((out - want).abs().max()) <= 2.0 ** -7 * want, (power, out.flatten()[0].item(), want)
+
+
+def attention_tops(q, cache, table, lengths, cu, window):
+    """The largest |v| of each output element's row among the keys that the row sees, dimension by dimension, float64 [tokens, heads, dim]."""
+    page, kv_heads, dim = cache[0].shape[2], cache[0].shape[1], cache[0].shape[3]
+    group = q.shape[1] // kv_heads
+    values = (cache[1].view(ref.E4M3).double() * cache[3].double()[..., None, None]).cpu().abs()
+    top = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(len(lengths)):
+        v = torch.cat([values[int(i)] for i in table[b, :-(-lengths[b] // page)]], 1)      # [kv_heads, keys, dim]
+        for t in range(int(cu[b]), int(cu[b + 1])):
+            end = lengths[b] - int(cu[b + 1]) + t + 1
+            first = max(0, end - window) if window else 0
+            if end > first:
+                top[t] = v[:, first:end].amax(1).repeat_interleave(group, 0)
+    return top
+
+
+def check_far(q, cache, table, lengths, news, window):
+    cu, lens = offsets(news), torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = decode.kv_attention(q, tuple(cache), table.cuda(), lens, cu=cu.cuda(), window=window).cpu().double()
+    want, _, spread = ref.attention(q, cache, table, lens, cu, None, window)
+    tol = bound(q.dtype, q.shape[2], spread, attention_tops(q, cache, table, lengths, cu, window))
+    if q.dtype == torch.float16:                                # below the type's normal numbers, and past its largest
+        tol = tol + 2.0 ** -24
+        out, want = (x.clamp(-65504.0, 65504.0) for x in (out, want))
+    assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,page", [(32, 16), (64, 16), (64, 128), (128, 16), (128, 64)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_scales_far_apart_row_by_row(cuda, dtype, dim, page, window):
+    # random scales over 2^60; every row's tolerance is that of the values which it sees
+    lengths, news = [400, 333, 17], [1, 2, 1]
+    table, pages = page_table([-(-n // page) for n in lengths], -(-400 // page), 3)
+    cache = random_cache(pages, 2, page, dim, 3)
+    cache[3].copy_(torch.ldexp(torch.ones(pages, 2, device="cuda"), torch.randint(-30, 30, (pages, 2), generator=gen(4), device="cuda")))
+    q = torch.randn((4, 8, dim), generator=gen(1), device="cuda").to(dtype)
+    check_far(q, cache, table, lengths, news, window)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,page", [(32, 16), (64, 32), (128, 16), (128, 64)])
+@pytest.mark.parametrize("where", ["later token", "before the window", "first page", "one dimension"])
+@pytest.mark.parametrize("far", [8, 24, 30, 60])
+def test_attention_beside_a_page_of_large_values(cuda, dtype, dim, page, where, far):
+    # one page's scale is 2^far times the others'.  Its large values belong to a later query token, lie before the window of a page
+    # that is partly visible, face a weight that underflows, or lie in one dimension; the other elements keep their own precision
+    table, pages = page_table([20], 20, 7)
+    cache = random_cache(pages, 1, page, dim, 7)
+    raw = cache[1].view(torch.uint8)
+    cache[3].fill_(2.0 ** -9)
+    length, news, window = 20 * page, [2], 0
+    q = torch.randn((2, 4, dim), generator=gen(2), device="cuda")
+    if where == "later token":
+        length = 19 * page + 1                                  # the last token alone is in the last page
+        big = int(table[0, 19])
+    elif where == "before the window":
+        window, big = 10 * page + page // 2, int(table[0, 9])   # half of that page is seen by token 0, one key fewer by token 1
+        raw[big, :, page // 2 - 1:] = 0
+    elif where == "first page":                                 # its keys score far below the others
+        big = int(table[0, 0])
+        cache[0].view(torch.uint8)[big] = 0xFE                  # -448
+        q = q.abs()
+        for p in range(1, 20):
+            codes = cache[0].view(torch.uint8)[int(table[0, p])]
+            cache[0].view(torch.uint8)[int(table[0, p])] = codes & 0x3F
+        cache[2].fill_(2.0 ** -2)
+        raw[big] = 0
+    else:
+        big = int(table[0, 5])
+        raw[big, :, :, 1:] = 0
+    cache[3][big] = 2.0 ** (far - 9)
+    check_far(q.to(dtype), cache, table, [length], news, window)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,page", [(32, 64), (64, 64), (128, 32), (128, 128)])
+def test_attention_small_values_after_pages_that_are_not_followed(cuda, dtype, dim, page):
+    # the first 512 keys are on pages that do not exist, the others' values are around 2^-40 (fp16: 2^-12)
+    bad, good = 512 // page, 1 + 300 // page
+    table, pages = page_table([good], good, 1)
+    cache = random_cache(pages, 1, page, dim, 1)
+    cache[3].fill_(2.0 ** (-20 if dtype == torch.float16 else -48))
+    holes = torch.cat((torch.full((1, bad), -1, dtype=torch.int32), table), 1)
+    q = torch.randn((1, 4, dim), generator=gen(2), device="cuda").to(dtype)
+    length = good * page - 3
+    out = decode.kv_attention(q, tuple(cache), holes.cuda(), torch.tensor([512 + length], dtype=torch.int32, device="cuda"),
+                              max_length=1).cpu().double()
+    assert status() == 16
+    want, _, spread = ref.attention(q, cache, table, torch.tensor([length]), [0, 1])
+    tol = bound(dtype, dim, spread, attention_tops(q, cache, table, [length], [0, 1], 0)) + (2.0 ** -24 if dtype == torch.float16 else 0.0)
+    assert ((out - want).abs() <= tol).all()
