@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(THREADS) kv_attention_join_few_kernel(const Ca
             if (s0 + i >= p.splits) break;
             const float f = __shfl_sync(0xffffffffu, factor, s0 + i);
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum[e] += f == 0.0f ? 0.0f : held[i][e] * f;
+            for (int e = 0; e < E; ++e) sum[e] += held[i][e] * f;   // (a NaN stays one when its weight is 0)
         }
     }
     const int64_t t = row / p.q_heads, h = row % p.q_heads;
@@ -766,14 +766,14 @@ __global__ void __launch_bounds__(THREADS) kv_attention_join_kernel(const Cached
         const int s = warp + WARPS * i;
         const float f = s < p.splits ? factor[s] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += f == 0.0f ? 0.0f : held[i][e] * f;
+        for (int e = 0; e < E; ++e) sum[e] += held[i][e] * f;   // (a NaN stays one when its weight is 0)
     }
 #pragma unroll 4
     for (int s = warp + WARPS * HELD; s < p.splits; s += WARPS) {
         const float f = factor[s];
         const float *from = p.part_o + (s * rows + row) * D + lane * E;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] += f == 0.0f ? 0.0f : from[e] * f;
+        for (int e = 0; e < E; ++e) sum[e] += from[e] * f;
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[warp * D + lane * E + e] = sum[e];

@@ -250,3 +250,19 @@ def test_attention_small_values_after_pages_that_are_not_followed(cuda, dtype, d
     want, _, spread = ref.attention(q, cache, table, torch.tensor([length]), [0, 1])
     tol = bound(dtype, dim, spread, attention_tops(q, cache, table, [length], [0, 1], 0)) + (2.0 ** -24 if dtype == torch.float16 else 0.0)
     assert ((out - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("length,max_length", [(1500, 0), (1500, 1), (20000, 0)])
+def test_attention_nan_value_of_a_key_without_weight(cuda, dtype, length, max_length):
+    # 0 times NaN is NaN, in whichever split of the keys it is (several, one, many), and in its own dimension alone
+    pages = -(-length // 64)
+    cache = [torch.zeros((pages, 1, 64, 64), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    cache[0].fill_(0x38), cache[1].fill_(0x38)                  # ones
+    cache[0][:pages // 2], cache[1][0, 0, 7, 11] = 0xB8, 0x7F   # the first half of the keys: minus one; a NaN in a value of theirs
+    scales = [torch.ones((pages, 1), device="cuda") for _ in range(2)]
+    q = torch.full((1, 3, 64), 100.0, device="cuda").to(dtype)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    out = decode.kv_attention(q, (cache[0].view(ref.E4M3), cache[1].view(ref.E4M3), *scales), table,
+                              torch.tensor([length], dtype=torch.int32, device="cuda"), max_length=max_length)
+    assert bool(torch.isnan(out[:, :, 11]).all()) and int(torch.isnan(out).sum()) == 3
