@@ -395,10 +395,10 @@ PITON_B200_API int piton_b200_kv_append(const piton_kv_append_args *args, void *
    [cu[b], cu[b + 1]) (tokens / batch each when cu is 0): query i of n is at position p = lengths[b] - n + i
    and attends keys p - window < j <= p (window 0: all up to p).  Query head h uses key head
    h / (q_heads / kv_heads).  out = softmax(sm_scale q k) v, rows without keys 0; lse (optional): the natural
-   logarithm of the row's sum of exponentials, -inf for rows without keys.  max_length and max_new are
-   bounds of the lengths and of the query tokens a sequence, used to size the launch (0: the table's width
-   and `tokens`); a longer sequence is still attended in full, more query tokens than max_new are not
-   computed. */
+   logarithm of the row's sum of exponentials, -inf for rows without keys; tokens outside [cu[0], cu[batch])
+   are rows without keys.  max_length and max_new are bounds of the lengths and of the query tokens a
+   sequence, used to size the launch (0: the table's width and `tokens`); a longer sequence and more query
+   tokens are still computed in full. */
 typedef struct {
     uint64_t q, out;            /* [tokens, q_heads, head_dim] of `type`, unit stride along head_dim */
     uint64_t lse;               /* float [tokens, q_heads] or 0 */

@@ -55,7 +55,7 @@ struct CachedParams {
     const int32_t *table, *lengths, *cu;
     float *part_o;                       // [splits][tokens * q_heads][D], splits > 1 only
     float2 *part_ml;                     // [splits][tokens * q_heads]
-    int64_t tokens, num_pages, table_stride, sqt, sqh, sot, soh, window, uniform, chunk;
+    int64_t batch, tokens, num_pages, table_stride, sqt, sqh, sot, soh, window, uniform, chunk;
     int32_t q_heads, kv_heads, group, page_log2, table_width, row_tiles, splits, q_aligned;
     float scale;
 };
@@ -171,20 +171,33 @@ template <int NQ> struct Rows {
     int32_t first[NQ][2], pos[NQ][2];
 };
 
+// Tokens [lo, hi) of the query are those that the offsets `cu` name; the outputs of the others are those of rows that see no key.
+__device__ __forceinline__ Span named(const CachedParams &p) {
+    const int64_t lo = min(max((int64_t)p.cu[0], (int64_t)0), p.tokens), hi = min(max((int64_t)p.cu[p.batch], (int64_t)0), p.tokens);
+    return {lo, max(hi - lo, (int64_t)0)};
+}
+template <typename T, int D> __device__ void clear_unnamed(const CachedParams &p, int64_t b, int kvh) {
+    const Span sp = named(p);
+    for (int64_t u = b; u < p.tokens - sp.n; u += p.batch) {
+        const int64_t t = u < sp.t0 ? u : u + sp.n;
+        for (int x = threadIdx.x; x < p.group * D; x += THREADS) {
+            const int h = kvh * p.group + x / D;
+            reinterpret_cast<T *>(p.out)[t * p.sot + h * p.soh + x % D] = from_float<T>(0.0f);
+            if (p.lse && x % D == 0) p.lse[t * p.q_heads + h] = -INFINITY;
+        }
+    }
+}
+
+// The rows row0 ... of a sequence's tokens times group over one split of its keys.
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_attention_kernel(const CachedParams p) {
+__device__ __forceinline__ void attend(const CachedParams &p, const int64_t b, const int kvh, const int split, const Span &sp, const uint32_t row0) {
     using G = Geometry<D>;
     constexpr bool SPLIT = sizeof(T) == 4;              // fp32 rows: queries and weights as pairs of halves
     constexpr float LIFT = SPLIT ? 14.0f : 11.0f, SLACK = SPLIT ? 0.0f : 4.0f, UNLIFT = SPLIT ? 0x1p-14f : 0x1p-11f;
     constexpr int R = 8 * NQ, KW = G::KB / 4, VW = G::VB / 4, MT = D / 16, KT = D / 16, TILES = G::TILES, KEYS = G::KEYS;
     extern __shared__ __align__(16) uint8_t ring[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-    if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;");    // the join may take its place, and waits
-    const int64_t b = blockIdx.z;
-    const int kvh = blockIdx.y, tile = blockIdx.x % p.row_tiles, split = blockIdx.x / p.row_tiles;
-    const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
-    const uint32_t group = p.group, rows = (uint32_t)sp.n * group, row0 = (uint32_t)tile * R;   // below 2^31, as tokens * heads is
-    if (row0 >= rows) return;
+    const uint32_t group = p.group, rows = (uint32_t)sp.n * group;     // below 2^31, as tokens * heads is
     const uint32_t live = min((uint32_t)R, rows - row0);
     // positions are below 2^31 (lengths are int32); a row past the tile's last repeats the last one
     const int32_t length = p.lengths[b];
@@ -674,6 +687,23 @@ __global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_atten
     }
 }
 
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(THREADS, ctas(NQ, D, sizeof(T) == 4)) kv_attention_kernel(const CachedParams p) {
+    constexpr uint32_t R = 8 * NQ;
+    if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;");    // the join may take its place, and waits
+    const int64_t b = blockIdx.z;
+    const int kvh = blockIdx.y, tile = blockIdx.x % p.row_tiles, split = blockIdx.x / p.row_tiles;
+    const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
+    if (p.cu && p.splits == 1 && tile == 0) clear_unnamed<T, D>(p, b, kvh);
+    // (more tiles than the launch was sized for, by too small a bound of the query tokens, are taken in turn)
+    const uint32_t rows = (uint32_t)sp.n * p.group;
+#pragma unroll 1
+    for (uint32_t row0 = tile * R; row0 < rows; row0 += p.row_tiles * R) {
+        if (row0 != tile * R) __syncthreads();          // the last tile's sums have been read
+        attend<T, D, NQ>(p, b, kvh, split, sp, row0);
+    }
+}
+
 // Joins a few (up to 32) splits of the keys: a warp per row, lane s holds split s's maximum and sum.
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS) kv_attention_join_few_kernel(const CachedParams p) {
@@ -681,6 +711,17 @@ __global__ void __launch_bounds__(THREADS) kv_attention_join_few_kernel(const Ca
     const int lane = threadIdx.x & 31;
     const int64_t rows = p.tokens * p.q_heads, row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
     if (row >= rows) return;
+    const int64_t t = row / p.q_heads, h = row % p.q_heads;
+    T *out = reinterpret_cast<T *>(p.out) + t * p.sot + h * p.soh + lane * E;
+    if (p.cu) {                                         // a token of no sequence: the splits have nothing of it
+        const Span sp = named(p);
+        if (t < sp.t0 || t >= sp.t0 + sp.n) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) out[e] = from_float<T>(0.0f);
+            if (p.lse && lane == 0) p.lse[row] = -INFINITY;
+            return;
+        }
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' results are there
     const float2 ml = lane < p.splits ? p.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
     const float *from = p.part_o + row * D + lane * E;
@@ -713,8 +754,6 @@ __global__ void __launch_bounds__(THREADS) kv_attention_join_few_kernel(const Ca
             for (int e = 0; e < E; ++e) sum[e] += held[i][e] * f;   // (a NaN stays one when its weight is 0)
         }
     }
-    const int64_t t = row / p.q_heads, h = row % p.q_heads;
-    T *out = reinterpret_cast<T *>(p.out) + t * p.sot + h * p.soh + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) out[e] = from_float<T>(total == 0.0f ? 0.0f : sum[e] / total);
     if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
@@ -729,6 +768,16 @@ __global__ void __launch_bounds__(THREADS) kv_attention_join_kernel(const Cached
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t rows = p.tokens * p.q_heads, row = blockIdx.x;
     float *sums = factor + p.splits;
+    const int64_t t = row / p.q_heads, h = row % p.q_heads;
+    T *out = reinterpret_cast<T *>(p.out) + t * p.sot + h * p.soh;
+    if (p.cu) {                                         // a token of no sequence: the splits have nothing of it
+        const Span sp = named(p);
+        if (t < sp.t0 || t >= sp.t0 + sp.n) {
+            if (threadIdx.x < D) out[threadIdx.x] = from_float<T>(0.0f);
+            if (p.lse && threadIdx.x == 0) p.lse[row] = -INFINITY;
+            return;
+        }
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the splits' results are there
     // up to 16 splits a warp are on their way while the factors are found
     constexpr int HELD = 16;
@@ -778,12 +827,11 @@ __global__ void __launch_bounds__(THREADS) kv_attention_join_kernel(const Cached
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[warp * D + lane * E + e] = sum[e];
     __syncthreads();
-    const int64_t t = row / p.q_heads, h = row % p.q_heads;
     if (threadIdx.x < D) {
         float all = 0.0f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) all += sums[w * D + threadIdx.x];
-        reinterpret_cast<T *>(p.out)[t * p.sot + h * p.soh + threadIdx.x] = from_float<T>(total == 0.0f ? 0.0f : all / total);
+        out[threadIdx.x] = from_float<T>(total == 0.0f ? 0.0f : all / total);
     }
     if (p.lse && threadIdx.x == 0) p.lse[row] = total == 0.0f ? -INFINITY : (top + log2f(total)) * LN2;
 }
@@ -796,7 +844,7 @@ struct Plan {
 
 Plan plan_of(const piton_kv_attention_args *a) {
     Plan plan;
-    const int64_t most_new = a->cu ? (a->max_new ? a->max_new : a->tokens) : a->tokens / a->batch;
+    const int64_t most_new = !a->cu ? a->tokens / a->batch : a->max_new && a->max_new < a->tokens ? a->max_new : a->tokens;
     const int64_t rows = most_new * (a->q_heads / a->kv_heads);
     plan.nq = rows <= 8 ? 1 : 2;
     plan.row_tiles = cdiv(rows, 8 * plan.nq);
@@ -926,7 +974,7 @@ extern "C" int piton_b200_kv_attention(const piton_kv_attention_args *a, void *s
     p.cu = reinterpret_cast<const int32_t *>(a->cu);
     p.part_o = reinterpret_cast<float *>(a->workspace);
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + plan.splits * rows * a->head_dim);
-    p.tokens = a->tokens; p.num_pages = a->num_pages; p.table_stride = a->table_stride;
+    p.batch = a->batch; p.tokens = a->tokens; p.num_pages = a->num_pages; p.table_stride = a->table_stride;
     p.sqt = a->stride_qt; p.sqh = a->stride_qh; p.sot = a->stride_ot; p.soh = a->stride_oh;
     p.window = a->window; p.uniform = a->cu ? 0 : a->tokens / a->batch; p.chunk = plan.chunk;
     p.q_heads = (int32_t)a->q_heads; p.kv_heads = (int32_t)a->kv_heads; p.group = p.q_heads / p.kv_heads;

@@ -213,9 +213,10 @@ def kv_attention(q, cache, table, lengths, *, cu=None, scale: Optional[float] = 
     Sequence b holds ``lengths[b]`` tokens (appended before), the last of them its query tokens, rows
     ``cu[b]:cu[b + 1]`` of q (``tokens / batch`` each without ``cu``).  The query at position p sees the keys up to
     p, with ``window`` only the last ``window`` of them.  heads is a multiple of the cache's kv_heads; ``scale``
-    is 1 / sqrt(head_dim) by default.  Rows that see no key are 0.  ``max_length`` (an upper bound of the
-    lengths known to the host) and ``max_new`` (of the query tokens a sequence, with ``cu``) size the launch;
-    by default the table's width and the number of tokens bound them.  With ``return_lse`` also the float32
+    is 1 / sqrt(head_dim) by default.  Rows that see no key are 0, and so are rows of tokens that no sequence's
+    range names.  ``max_length`` (an upper bound of the lengths known to the host) and ``max_new`` (of the query
+    tokens a sequence, with ``cu``) size the launch and change no result; by default the table's width and the
+    number of tokens bound them.  With ``return_lse`` also the float32
     [tokens, heads] logarithms of the rows' sums of exponentials (-inf for rows that see no key)."""
     args = (q, cache, table, lengths, cu, scale, window, max_length, max_new, return_lse)
     result = (_bound or _calls()).kv_attention(*args)

@@ -1,0 +1,64 @@
+"""What the decode operators return for rows that no sequence names, that bounds did not count or that are refused:
+never what the memory held before.  Tolerances are those of test_gpu_decode.py.
+"""
+
+import math
+
+import pytest
+import torch
+
+import decode_ref as ref
+from piton_b200 import decode
+from test_gpu_decode import TYPES, bound, gen, page_table, random_cache, status
+
+pytestmark = pytest.mark.gpu
+
+
+def litter():
+    """Leaves blocks of NaN for the allocator to hand out again."""
+    blocks = [torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda") for n in (512, 4096, 65536, 1 << 20, 1 << 22, 1 << 24) for _ in range(3)]
+    torch.cuda.synchronize()
+    del blocks
+
+
+def check(lengths, cu, tokens, *, dtype, dim=64, page=32, kv_heads=2, group=3, **kw):
+    table, pages = page_table([-(-n // page) for n in lengths], -(-max(lengths) // page), 1)
+    cache = random_cache(pages, kv_heads, page, dim, 1)
+    q = torch.randn((tokens, kv_heads * group, dim), generator=gen(2), device="cuda").to(dtype)
+    lens, cu = torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.tensor(cu, dtype=torch.int32, device="cuda")
+    table = table.cuda()
+    litter()
+    out, lse = decode.kv_attention(q, tuple(cache), table, lens, cu=cu, return_lse=True, **kw)
+    want, want_lse, spread = ref.attention(q, cache, table, lens, cu)
+    top = float((cache[1].float() * cache[3][..., None, None]).abs().max())
+    assert ((out.cpu().double() - want).abs() <= bound(dtype, dim, spread, top)).all()
+    empty = want_lse == -math.inf
+    assert bool((out.cpu()[empty] == 0).all()) and torch.equal(lse.cpu() == -math.inf, empty)
+    assert bool(torch.isfinite(lse.cpu()[~empty]).all())
+    assert status() == 0
+    return empty
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("max_length", [0, 1])                 # with and without splits of the keys
+@pytest.mark.parametrize("lengths", [[300, 90, 41], [6000, 700, 2500]])
+@pytest.mark.parametrize("dim", [32, 128])
+def test_attention_of_more_query_tokens_than_max_new(cuda, dtype, max_length, lengths, dim):
+    for max_new in (1, 2, 5):
+        empty = check(lengths, [0, 4, 5, 45], 45, dtype=dtype, dim=dim, max_length=max_length, max_new=max_new)
+        assert not bool(empty.any())
+
+
+def test_attention_max_new_past_32_bits(cuda):
+    check([300, 90], [0, 4, 5], 5, dtype=torch.float16, max_new=1 << 40)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("max_length", [0, 1])
+@pytest.mark.parametrize("lengths", [[300, 90], [6000, 700], [40000, 31]])
+@pytest.mark.parametrize("cu,tokens", [([3, 5, 6], 11), ([0, 0, 0], 4), ([0, 2, 2], 3), ([4, 4, 5], 5)])
+def test_attention_of_tokens_that_no_sequence_names(cuda, dtype, max_length, lengths, cu, tokens):
+    empty = check(lengths, cu, tokens, dtype=dtype, max_length=max_length)
+    named = torch.zeros(tokens, dtype=torch.bool)
+    named[cu[0]:cu[-1]] = True
+    assert torch.equal(empty, ~named[:, None].expand(empty.shape))
