@@ -361,7 +361,7 @@ PITON_B200_API int piton_b200_graph_cache_clear(void);
    code * scale of its page and head, scales are powers of two in [2^-120, 2^120].  page_size 16, 32, 64
    or 128; head_dim 32, 64 or 128 (ENOTSUP otherwise).  Token p of sequence b is in page
    table[b * table_stride + p / page_size], slot p % page_size.  A table entry outside [0, num_pages) or a
-   position past the table is not followed: those tokens are neither written nor attended, and
+   position past the page table is not followed: those tokens are neither written nor attended, and
    piton_b200_device_status reports it. */
 #define PITON_B200_TYPE_F32 0  /* element types of activations */
 #define PITON_B200_TYPE_F16 1
@@ -375,7 +375,8 @@ PITON_B200_API int piton_b200_graph_cache_clear(void);
    A block (page, head) takes the least scale that holds its new values and is at least its old one while
    the page holds older tokens; those are requantised when it grows.  A non-finite value is stored as NaN
    and leaves the scale alone.  A page that is written belongs to one sequence.  lengths[b] (optional, not
-   `starts`) = starts[b] + new tokens of b. */
+   `starts`) = starts[b] + new tokens of b.  The rotated query of a token at a position past cos and sin is zeros
+   (piton_b200_device_status reports it).  Rotated queries outside [cu[0], cu[batch]) are zeros. */
 typedef struct {
     uint64_t k, v;              /* [tokens, kv_heads, head_dim] of `type`, unit stride along head_dim */
     uint64_t q, q_out;          /* [tokens, q_heads, head_dim], or both 0 */

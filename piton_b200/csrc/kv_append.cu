@@ -86,6 +86,14 @@ __device__ __forceinline__ int64_t first_unit(const AppendParams &p, int64_t b) 
     return (p.cu ? max((int64_t)p.cu[b], (int64_t)0) / p.page_size : 0) + 2 * b;
 }
 
+// Whether query token t is rotated: it has to belong to the sequence and to have a position that the tables hold; it is 0 otherwise.
+__device__ __forceinline__ bool rotates(const AppendParams &p, const Span &sp, int64_t t, int64_t start, bool report) {
+    if (t < sp.t0 || t >= sp.t0 + sp.n) return false;                // a token of no sequence
+    if (start >= 0 && (p.rot == 0 || start + t - sp.t0 < p.rope_len)) return true;
+    if (report) record_status(STATUS_BAD_POSITION);
+    return false;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendParams p) {
     const int tid = threadIdx.x;
@@ -95,13 +103,12 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendParams p
         const int64_t t = row / p.q_heads, h = row % p.q_heads, b = sequence_of_token(p, t);
         const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
         const int64_t pos = (int64_t)p.starts[b] + t - sp.t0;
-        const bool ok = p.rot == 0 || (pos >= 0 && pos < p.rope_len && t >= sp.t0 && t < sp.t0 + sp.n);
-        if (!ok) {
-            if ((tid & 31) == 0) record_status(STATUS_BAD_POSITION);
-            return;
-        }
         const T *x = reinterpret_cast<const T *>(p.q) + t * p.sqt + h * p.sqh;
         T *y = reinterpret_cast<T *>(p.q_out) + t * p.sot + h * p.soh;
+        if (!rotates(p, sp, t, p.starts[b], (tid & 31) == 0)) {
+            for (int d = tid & 31; d < p.dim; d += 32) y[d] = from_float<T>(0.0f);
+            return;
+        }
         const float *c = p.cos_table + pos * (p.rot >> 1), *s = p.sin_table + pos * (p.rot >> 1);
         for (int d = tid & 31; d < p.dim; d += 32) y[d] = from_float<T>(rotated(x, d, c, s, p.rot, p.interleaved));
         return;
@@ -301,15 +308,12 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
         const int64_t b = sequence_of_token(p, t);
         const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
         const int64_t pos = (int64_t)p.starts[b] + t - sp.t0;
-        if (p.rot != 0 && (pos < 0 || pos >= p.rope_len || t < sp.t0 || t >= sp.t0 + sp.n)) {
-            if (lane == 0) record_status(STATUS_BAD_POSITION);
-            return;
-        }
+        const bool named = rotates(p, sp, t, p.starts[b], lane == 0);
         constexpr int SIDE = 32 / UPH;                               // heads at once
         const int u = lane % UPH;
         const PairPlace at = place_of<T>(u, p.rot, p.interleaved);
         float c[V], s[V];
-        if (at.turns) {
+        if (at.turns && named) {
             load_row(c, p.cos_table + pos * (p.rot >> 1) + V * u);
             load_row(s, p.sin_table + pos * (p.rot >> 1) + V * u);
         }
@@ -317,6 +321,10 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
         T *y = reinterpret_cast<T *>(p.q_out) + t * p.sot;
         const int heads = (int)p.q_heads, step = SIDE * q_pieces;
         int h = (int)(item % q_pieces) * SIDE + lane / UPH;
+        if (!named) {
+            for (; h < heads; h += step) *reinterpret_cast<uint4 *>(y + h * p.soh + at.a) = *reinterpret_cast<uint4 *>(y + h * p.soh + at.b) = uint4();
+            return;
+        }
         for (; h < heads; h += 2 * step) {                           // two heads in flight
             const bool more = h + step < heads;
             const T *x0 = x + h * p.sqh, *x1 = x + (int64_t)(h + step) * p.sqh;
@@ -550,6 +558,7 @@ extern "C" int piton_b200_kv_append(const piton_kv_append_args *a, void *stream)
         return set_error(PITON_B200_ENOTSUP, "head_dim %lld (32, 64, 128) or page_size %lld (16, 32, 64, 128)",
                          (long long)a->head_dim, (long long)a->page_size);
     PITON_REQUIRE(a->rot_dim >= 0 && a->rot_dim <= a->head_dim && a->rot_dim % 2 == 0, "rot_dim %lld", (long long)a->rot_dim);
+    PITON_REQUIRE(a->batch > 0 || a->tokens == 0, "%lld tokens of no sequence", (long long)a->tokens);
     if (a->batch == 0) return PITON_B200_OK;
     PITON_REQUIRE(a->cu || a->tokens % a->batch == 0, "%lld tokens are not the same number for %lld sequences",
                   (long long)a->tokens, (long long)a->batch);

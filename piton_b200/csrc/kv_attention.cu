@@ -934,6 +934,7 @@ int check_attention(const piton_kv_attention_args *a) {
         (a->page_size != 16 && a->page_size != 32 && a->page_size != 64 && a->page_size != 128))
         return set_error(PITON_B200_ENOTSUP, "head_dim %lld (32, 64, 128) or page_size %lld (16, 32, 64, 128)",
                          (long long)a->head_dim, (long long)a->page_size);
+    PITON_REQUIRE(a->batch > 0 || a->tokens == 0, "%lld tokens of no sequence", (long long)a->tokens);
     PITON_REQUIRE(a->batch == 0 || a->cu || a->tokens % a->batch == 0, "%lld tokens are not the same number for %lld sequences",
                   (long long)a->tokens, (long long)a->batch);
     return PITON_B200_OK;

@@ -9,7 +9,7 @@ import torch
 
 import decode_ref as ref
 from piton_b200 import decode
-from test_gpu_decode import TYPES, bound, gen, page_table, random_cache, status
+from test_gpu_decode import TYPES, bound, cpu, gen, page_table, random_cache, status, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,39 @@ def test_attention_of_tokens_that_no_sequence_names(cuda, dtype, max_length, len
     named = torch.zeros(tokens, dtype=torch.bool)
     named[cu[0]:cu[-1]] = True
     assert torch.equal(empty, ~named[:, None].expand(empty.shape))
+
+
+# ---- append ----
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rot", [0, 34, 64])
+@pytest.mark.parametrize("cu,tokens", [([3, 5, 6], 9), ([0, 0, 0], 4), ([0, 40, 40], 43), ([4, 4, 5], 5)])
+def test_append_queries_that_no_sequence_names(cuda, dtype, rot, cu, tokens):
+    table, pages = page_table([4, 4], 4, 3)
+    cache = random_cache(pages, 2, 16, 64, 5)
+    before = cpu(cache)
+    qkv = torch.randn((tokens, 10, 64), generator=gen(6), device="cuda").to(dtype)
+    q, k, v = qkv.split((6, 2, 2), 1)
+    cos, sin = tables(rot, 80) if rot else (None, None)
+    cu_t = torch.tensor(cu, dtype=torch.int32)
+    starts = torch.tensor([9, 5], dtype=torch.int32)
+    named = torch.zeros(tokens, dtype=torch.bool)
+    named[cu[0]:cu[-1]] = True
+    host = [None if t is None else t.cpu() for t in (cos, sin)]
+    want_q, want_l = ref.append(k.cpu(), v.cpu(), before, table, starts, cu_t, *host, False, q.cpu())
+    litter()
+    got_q, got_l = decode.kv_append(k, v, tuple(cache), table.cuda(), starts.cuda(), cu=cu_t.cuda(), cos=cos, sin=sin, q=q)
+    assert status() == 0
+    assert torch.equal(got_q.cpu()[named], want_q[named]) and bool((got_q.cpu()[~named] == 0).all())
+    assert torch.equal(got_l.cpu(), want_l)
+    assert all(ref.same_codes(a, b) for a, b in zip(cache[:2], before[:2]))
+
+
+def test_tokens_of_no_sequence_are_refused(cuda):
+    cache = decode.PagedKV.empty(2, 1, 32, 16)
+    table, none = torch.zeros((0, 1), dtype=torch.int32, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda")
+    k, cu = torch.ones((2, 1, 32), device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        decode.kv_append(k, k, cache, table, none, cu=cu, q=k)
+    with pytest.raises(ValueError):
+        decode.kv_attention(k, cache, table, none, cu=cu)
