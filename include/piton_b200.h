@@ -375,8 +375,9 @@ PITON_B200_API int piton_b200_graph_cache_clear(void);
    A block (page, head) takes the least scale that holds its new values and is at least its old one while
    the page holds older tokens; those are requantised when it grows.  A non-finite value is stored as NaN
    and leaves the scale alone.  A page that is written belongs to one sequence.  lengths[b] (optional, not
-   `starts`) = starts[b] + new tokens of b.  The rotated query of a token at a position past cos and sin is zeros
-   (piton_b200_device_status reports it).  Rotated queries outside [cu[0], cu[batch]) are zeros. */
+   `starts`) = starts[b] + new tokens of b.  A token at a position past cos and sin has no rotation: its key, value
+   and rotated query are zeros (piton_b200_device_status reports it); the other tokens of its page are stored as
+   usual.  Rotated queries outside [cu[0], cu[batch]) are zeros. */
 typedef struct {
     uint64_t k, v;              /* [tokens, kv_heads, head_dim] of `type`, unit stride along head_dim */
     uint64_t q, q_out;          /* [tokens, q_heads, head_dim], or both 0 */

@@ -86,6 +86,19 @@ __device__ __forceinline__ int64_t first_unit(const AppendParams &p, int64_t b) 
     return (p.cu ? max((int64_t)p.cu[b], (int64_t)0) / p.page_size : 0) + 2 * b;
 }
 
+// Tokens at positions [lo, hi) that the rotation tables have rows for.
+__device__ __forceinline__ int live_tokens(const AppendParams &p, int64_t lo, int64_t hi) {
+    return (int)((p.rot ? min(max(p.rope_len, lo), hi) : hi) - lo);
+}
+
+// Zeros to bytes [from, to) of a page's heads.
+__device__ __forceinline__ void clear_codes(const AppendParams &p, int which, int64_t page, int head0, int head1, int from, int to, int worker, int workers) {
+    const int64_t bytes = p.page_size * p.dim;
+    for (int h = head0; h < head1; ++h)
+        for (int i = from + 16 * worker; i < to; i += 16 * workers)
+            *reinterpret_cast<uint4 *>(p.codes[which] + (page * p.kv_heads + h) * bytes + i) = uint4();
+}
+
 // Whether query token t is rotated: it has to belong to the sequence and to have a position that the tables hold; it is 0 otherwise.
 __device__ __forceinline__ bool rotates(const AppendParams &p, const Span &sp, int64_t t, int64_t start, bool report) {
     if (t < sp.t0 || t >= sp.t0 + sp.n) return false;                // a token of no sequence
@@ -143,7 +156,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendParams p
     const int64_t page0 = place * p.page_size;
     const int64_t lo = max(start, page0), hi = min(end, page0 + p.page_size);
     if (lo >= hi) return;
-    if (place >= p.table_width || (which == 0 && p.rot && hi > p.rope_len)) {
+    if (place >= p.table_width) {
         if (tid == 0) record_status(STATUS_BAD_POSITION);
         return;
     }
@@ -157,8 +170,11 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendParams p
     uint8_t *codes = p.codes[which] + (page * p.kv_heads + h) * p.page_size * p.dim;
     float *scale = p.scale[which] + page * p.kv_heads + h;
     const int count = (int)(hi - lo) * p.dim, held = (int)(lo - page0);
+    const int live = live_tokens(p, lo, hi);                         // the others have no rotation: zeros
+    if (lo + live < hi && tid == 0) record_status(STATUS_BAD_POSITION);
     auto value = [&](int i) {
         const int t = i / p.dim, d = i % p.dim;
+        if (t >= live) return 0.0f;
         const int64_t row = (lo + t) * (rot >> 1);
         return rotated(x + t * p.st[which], d, p.cos_table + row, p.sin_table + row, rot, p.interleaved);
     };
@@ -379,7 +395,7 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
     const int64_t place = start / p.page_size + j, page0 = place * p.page_size;
     const int64_t lo = max(start, page0), hi = min(end, page0 + p.page_size);
     if (lo >= hi) return;
-    if (place >= p.table_width || (which == 0 && p.rot && hi > p.rope_len)) {
+    if (place >= p.table_width) {
         if (worker == 0) record_status(STATUS_BAD_POSITION);
         return;
     }
@@ -388,7 +404,11 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
         if (worker == 0) record_status(STATUS_BAD_PAGE);
         return;
     }
-    const int rot = which == 0 ? p.rot : 0, count = (int)(hi - lo), held = (int)(lo - page0), u = worker % UPH;
+    const int rot = which == 0 ? p.rot : 0, count = live_tokens(p, lo, hi), held = (int)(lo - page0), u = worker % UPH;
+    if (lo + count < hi) {                                           // tokens that have no rotation
+        if (worker == 0) record_status(STATUS_BAD_POSITION);
+        clear_codes(p, which, page, head0, min(head0 + heads_each, (int)p.kv_heads), (held + count) * D, (int)(hi - page0) * D, worker, TT);
+    }
     const PairPlace at = place_of<T>(u, rot, p.interleaved);
     constexpr int TOKENS = TT / UPH;                                 // a pass
     const int token = worker / UPH;

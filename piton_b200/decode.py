@@ -194,8 +194,8 @@ def kv_append(k, v, cache, table, starts, *, cu=None, cos=None, sin=None, interl
     with ``interleaved``; without them nothing is rotated.  ``q`` [tokens, heads, head_dim] is rotated the
     same way.  Any token and head strides, unit stride along head_dim.  Returns ``(q, lengths)``: the
     rotated queries in a new contiguous tensor of q's type (None without q) and int32 ``starts`` plus the
-    new tokens.  The rotated query of a token past the rows of ``cos`` and ``sin`` is 0 (device status 17),
-    and so is that of a token that no sequence's range names.
+    new tokens.  A token past the rows of ``cos`` and ``sin`` is stored as zeros and its rotated query is 0
+    (device status 17); so is the rotated query of a token that no sequence's range names.
 
     A block (page and head) has one scale: the least power of two that holds its values within e4m3's 448;
     when new values make it grow, the block's older codes are requantised.  Non-finite values are stored

@@ -67,6 +67,35 @@ def test_attention_of_tokens_that_no_sequence_names(cuda, dtype, max_length, len
 # ---- append ----
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,page,rot,interleaved", [(64, 16, 64, False), (128, 128, 64, True), (32, 32, 32, False), (64, 64, 34, False)])
+@pytest.mark.parametrize("rows", [1, 37, 40, 80])
+def test_append_past_the_rotation_tables(cuda, dtype, dim, page, rot, interleaved, rows):
+    # tables end inside a block of new tokens, before one, at one token: the tokens before that are stored as ever, the others are zeros
+    starts, news = [30, 0, 39, 200, 36], [45, 70, 1, 2, 3]
+    table, pages = page_table([-(-(s + n) // page) for s, n in zip(starts, news)], -(-202 // page), 3)
+    cache = random_cache(pages, 2, page, dim, 5)
+    cu = torch.tensor([0, *news]).cumsum(0).to(torch.int32)
+    tokens = int(cu[-1])
+    qkv = torch.randn((tokens, 8, dim), generator=gen(6), device="cuda").to(dtype)
+    q, k, v = qkv.split((4, 2, 2), 1)
+    cos, sin = tables(rot, 300)
+    held = torch.cat([torch.arange(s, s + n) for s, n in zip(starts, news)]) < rows
+    starts = torch.tensor(starts, dtype=torch.int32)
+    want = cpu(cache)
+    cleared = [torch.where(held[:, None, None], t.cpu(), 0) for t in (k, v, q)]
+    want_q, want_l = ref.append(*cleared[:2], want, table, starts, cu, cos.cpu(), sin.cpu(), interleaved, cleared[2])
+    litter()
+    got_q, got_l = decode.kv_append(k, v, tuple(cache), table.cuda(), starts.cuda(), cu=cu.cuda(), cos=cos[:rows].contiguous(),
+                                    sin=sin[:rows].contiguous(), interleaved=interleaved, q=q)
+    assert status() == (0 if bool(held.all()) else 17)
+    assert torch.equal(got_q.cpu(), want_q) and torch.equal(got_l.cpu(), want_l)
+    for got, w in zip(cache[:2], want[:2]):                     # (zeros of either sign are the same)
+        assert ref.same_codes(got, w) or bool(((got.view(torch.uint8).cpu() == w) | ((got.view(torch.uint8).cpu() | w) & 127 == 0)).all())
+    for got, w in zip(cache[2:], want[2:]):
+        assert torch.equal(got.cpu(), w)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rot", [0, 34, 64])
 @pytest.mark.parametrize("cu,tokens", [([3, 5, 6], 9), ([0, 0, 0], 4), ([0, 40, 40], 43), ([4, 4, 5], 5)])
 def test_append_queries_that_no_sequence_names(cuda, dtype, rot, cu, tokens):
