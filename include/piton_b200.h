@@ -377,7 +377,8 @@ PITON_B200_API int piton_b200_graph_cache_clear(void);
    and leaves the scale alone.  A page that is written belongs to one sequence.  lengths[b] (optional, not
    `starts`) = starts[b] + new tokens of b.  A token at a position past cos and sin has no rotation: its key, value
    and rotated query are zeros (piton_b200_device_status reports it); the other tokens of its page are stored as
-   usual.  Rotated queries outside [cu[0], cu[batch]) are zeros. */
+   usual.  Of a sequence that starts below 0 nothing is stored, its length is 0 and its rotated queries are zeros
+   (reported).  Rotated queries outside [cu[0], cu[batch]) are zeros. */
 typedef struct {
     uint64_t k, v;              /* [tokens, kv_heads, head_dim] of `type`, unit stride along head_dim */
     uint64_t q, q_out;          /* [tokens, q_heads, head_dim], or both 0 */

@@ -83,7 +83,16 @@ __device__ __forceinline__ int64_t sequence_of_token(const AppendParams &p, int6
 // start at cu[b] / page_size + 2 b, which leaves it at least the n / page_size + 2 pages that n
 // tokens can touch.
 __device__ __forceinline__ int64_t first_unit(const AppendParams &p, int64_t b) {
-    return (p.cu ? max((int64_t)p.cu[b], (int64_t)0) / p.page_size : 0) + 2 * b;
+    return (p.cu ? min(max((int64_t)p.cu[b], (int64_t)0), p.tokens) / p.page_size : 0) + 2 * b;
+}
+
+// The sequences' new lengths, a thread each; 0 for one that is refused because it starts below 0, so that none of its keys is attended.
+__device__ __forceinline__ void write_lengths(const AppendParams &p) {
+    for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < p.batch; b += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t start = p.starts[b];
+        if (p.lengths) p.lengths[b] = start < 0 ? 0 : (int32_t)min(start + span_of(p.cu, b, p.uniform, p.tokens).n, (int64_t)INT32_MAX);
+        if (start < 0 || (p.cu && (p.cu[b] < 0 || p.cu[b + 1] < p.cu[b] || p.cu[b + 1] > p.tokens))) record_status(STATUS_BAD_POSITION);
+    }
 }
 
 // Tokens at positions [lo, hi) that the rotation tables have rows for.
@@ -110,6 +119,7 @@ __device__ __forceinline__ bool rotates(const AppendParams &p, const Span &sp, i
 template <typename T>
 __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendParams p) {
     const int tid = threadIdx.x;
+    write_lengths(p);
     if (blockIdx.x >= p.unit_blocks) {                               // queries: a warp per (token, head)
         const int64_t row = ((int64_t)blockIdx.x - p.unit_blocks) * (THREADS / 32) + (tid >> 5);
         if (row >= p.tokens * p.q_heads) return;
@@ -147,11 +157,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendParams p
     }
     const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
     const int64_t start = p.starts[b], end = start + sp.n;
-    if (j == 0 && h == 0 && which == 0 && tid == 0 && p.lengths) p.lengths[b] = (int32_t)end;
-    if (start < 0) {
-        if (tid == 0) record_status(STATUS_BAD_POSITION);
-        return;
-    }
+    if (start < 0) return;                                           // (reported with the lengths)
     const int64_t place = start / p.page_size + j;                   // this unit's page of the sequence
     const int64_t page0 = place * p.page_size;
     const int64_t lo = max(start, page0), hi = min(end, page0 + p.page_size);
@@ -317,6 +323,7 @@ template <typename T, int D, int TT, int PASSES>
 __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASSES == 4 ? 2 : 1) kv_append_wide_kernel(const AppendParams p, int heads_each, int q_pieces) {
     constexpr int V = 16 / sizeof(T), UPH = D / (2 * V);             // pairs of a head
     const int tid = threadIdx.x, lane = tid & 31;
+    write_lengths(p);
     if (blockIdx.x >= p.unit_blocks) {                               // queries: a warp per token and piece of the heads
         const int64_t item = ((int64_t)blockIdx.x - p.unit_blocks) * (WIDE / 32) + (tid >> 5);
         const int64_t t = item / q_pieces;
@@ -387,11 +394,7 @@ __global__ void __launch_bounds__(WIDE, PASSES == 1 ? 4 : PASSES == 2 ? 3 : PASS
     }
     const Span sp = span_of(p.cu, b, p.uniform, p.tokens);
     const int64_t start = p.starts[b], end = start + sp.n;
-    if (j == 0 && head0 == 0 && which == 0 && worker == 0 && p.lengths) p.lengths[b] = (int32_t)end;
-    if (start < 0) {
-        if (worker == 0) record_status(STATUS_BAD_POSITION);
-        return;
-    }
+    if (start < 0) return;                                           // (reported with the lengths)
     const int64_t place = start / p.page_size + j, page0 = place * p.page_size;
     const int64_t lo = max(start, page0), hi = min(end, page0 + p.page_size);
     if (lo >= hi) return;

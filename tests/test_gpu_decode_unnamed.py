@@ -119,6 +119,27 @@ def test_append_queries_that_no_sequence_names(cuda, dtype, rot, cu, tokens):
     assert all(ref.same_codes(a, b) for a, b in zip(cache[:2], before[:2]))
 
 
+@pytest.mark.parametrize("rot", [0, 34, 64])
+def test_append_below_zero_and_offsets_past_the_tokens(cuda, rot):
+    cos, sin = tables(rot, 80) if rot else (None, None)
+    k = torch.randn((6, 2, 64), generator=gen(1), device="cuda")
+    table, pages = page_table([4, 4, 4], 4, 3)
+    cache = random_cache(pages, 2, 16, 64, 5)
+    before = cpu(cache)
+    litter()
+    q, lengths = decode.kv_append(k, k, tuple(cache), table.cuda(), torch.tensor([3, -1, 8], dtype=torch.int32, device="cuda"), cos=cos, sin=sin, q=k)
+    assert status() == 17 and lengths.tolist() == [5, 0, 10]
+    assert bool((q[2:4] == 0).all()) and bool((q[[0, 1, 4, 5]] != 0).any(-1).all())
+    for a, b in zip(cache, before):
+        a = a.view(torch.uint8) if a.dtype == ref.E4M3 else a
+        assert torch.equal(a.cpu()[table[1].long()], b[table[1].long()])
+    litter()
+    cu = torch.tensor([0, 60, 70, 80], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([3, 7, 8], dtype=torch.int32, device="cuda")
+    _, lengths = decode.kv_append(k, k, tuple(cache), table.cuda(), starts, cu=cu, cos=cos, sin=sin, q=k)
+    assert status() == 17 and lengths.tolist() == [9, 7, 8]
+
+
 def test_tokens_of_no_sequence_are_refused(cuda):
     cache = decode.PagedKV.empty(2, 1, 32, 16)
     table, none = torch.zeros((0, 1), dtype=torch.int32, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda")
