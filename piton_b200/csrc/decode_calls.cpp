@@ -10,6 +10,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -39,6 +40,9 @@ int type_of(const at::Tensor &t) {
         default: return -1;
     }
 }
+
+// Whether an output would have to carry a gradient, which these operators have none of.
+template <typename... T> bool wants_gradient(const T *...t) { return c10::GradMode::is_enabled() && (... || (t && t->requires_grad())); }
 
 // The four tensors of a cache, of `device`.
 struct Cache {
@@ -125,6 +129,7 @@ PyObject *kv_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
                 Py_RETURN_NONE;
         }
         if (o[9] != Py_None && !rows(q = tensor(o[9]), type, device, tokens, -1, c.dim)) Py_RETURN_NONE;
+        if (wants_gradient(k, v, q, cos, sin, c.t[2], c.t[3])) Py_RETURN_NONE;
         const int interleaved = PyObject_IsTrue(o[8]);
         if (interleaved < 0) return nullptr;
         at::Tensor out, lengths = empty({s.batch}, at::kInt, *k);
@@ -161,7 +166,7 @@ PyObject *kv_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
         Cache c;
         Sequences s;
         if (!c.take(o[1], device) || !rows(q, q->scalar_type(), device, q->size(0), -1, c.dim) ||
-            !s.take(o[2], o[3], o[4], q->size(0), device))
+            !s.take(o[2], o[3], o[4], q->size(0), device) || wants_gradient(q, c.t[2], c.t[3]))
             Py_RETURN_NONE;
         piton_kv_attention_args a = {};
         a.sm_scale = o[5] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AsDouble(o[5]);
@@ -215,6 +220,7 @@ PyObject *matvec_w4(PyObject *, PyObject *const *o, Py_ssize_t n) {
         if (o[5] != Py_None && (!is_a(bias = tensor(o[5]), x->scalar_type(), device, 1) || bias->size(0) != outer ||
                                 (outer > 1 && bias->stride(0) != 1)))
             Py_RETURN_NONE;
+        if (wants_gradient(x, scales, bias)) Py_RETURN_NONE;
         piton_matvec_w4_args a = {};
         a.rows = flat ? 1 : x->size(0), a.inner = inner, a.outer = outer;
         at::Tensor y = flat ? empty({outer}, x->scalar_type(), *x) : empty({a.rows, outer}, x->scalar_type(), *x);

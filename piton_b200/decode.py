@@ -18,6 +18,8 @@ page ``table[b, p // page_size]``, slot ``p % page_size``.  A page that is appen
 one sequence.  Table entries and positions live on the device, so a bad one cannot raise here: the
 kernels do not follow it (the token is neither stored nor attended) and ``piton_b200_device_status``
 reports 16 (page) or 17 (position or offset).
+
+There is no backward: inputs that require grad are refused unless gradients are off (``torch.no_grad()``).
 """
 
 from __future__ import annotations
@@ -86,6 +88,12 @@ def _need(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
+def _refuse_gradient(*tensors) -> None:
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise RuntimeError("the serving operators have no backward and an input requires grad: call them under torch.no_grad(), or "
+                           "detach it")
+
+
 def _type_of(name: str, t) -> int:
     if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dtype not in _TYPES:
         raise TypeError(f"{name}: expected a float32, float16 or bfloat16 CUDA tensor, got "
@@ -135,6 +143,7 @@ def _refuse_table(table, index: int) -> int:
 
 def _refuse_append(k, v, cache, table, starts, cu, cos, sin, interleaved, q) -> None:
     _type_of("k", k)
+    _refuse_gradient(k, v, q, cos, sin, *(cache if isinstance(cache, tuple) else ()))
     index, dtype = k.get_device(), k.dtype
     _refuse_cache(cache, index)
     heads, dim = cache[0].shape[1], cache[0].shape[3]
@@ -158,6 +167,7 @@ def _refuse_append(k, v, cache, table, starts, cu, cos, sin, interleaved, q) -> 
 
 def _refuse_attention(q, cache, table, lengths, cu, scale, window, max_length, max_new, return_lse) -> None:
     _type_of("q", q)
+    _refuse_gradient(q, *(cache if isinstance(cache, tuple) else ()))
     index = q.get_device()
     _refuse_cache(cache, index)
     _refuse_rows("q", q, q.dtype, None, cache[0].shape[3], index)
@@ -168,6 +178,7 @@ def _refuse_attention(q, cache, table, lengths, cu, scale, window, max_length, m
 
 def _refuse_matvec(x, codes, scales, group, zeros, bias) -> None:
     _type_of("x", x)
+    _refuse_gradient(x, scales, bias)
     index = x.get_device()
     if group not in (32, 64, 128):
         raise NotImplementedError(f"group {group}: 32, 64 or 128")
@@ -243,6 +254,7 @@ def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
     return result
 
 
+@torch.no_grad()
 def quantize_w4(weight, group: int = 128, zeros: bool = True, dtype=None):
     """Codes, scales and zero points (None if not ``zeros``) of a weight matrix [outer, inner], for
     :func:`matvec_w4`: each group of ``group`` elements spans its own range in 16 steps.  Plain torch, done
