@@ -85,10 +85,16 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &l
     return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
+// Makes `device` current while it lives: a workspace's size and the launch that checks it are made of the same device's SM count.
+struct On {
+    c10::cuda::OptionalCUDAGuard guard;
+    explicit On(int device) {
+        if (c10::cuda::current_device() != device) guard.set_index((c10::DeviceIndex)device);
+    }
+};
+
 // Runs an entry point on the current stream of `device`; its status.
 template <typename Entry, typename Args> int enter(Entry entry, const Args &a, int device) {
-    const c10::cuda::OptionalCUDAGuard guard(c10::cuda::current_device() == device ? std::nullopt
-                                                                                  : std::optional<c10::Device>(c10::Device(c10::kCUDA, device)));
     return entry(&a, c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream());
 }
 
@@ -130,6 +136,7 @@ PyObject *kv_append(PyObject *, PyObject *const *o, Py_ssize_t n) {
         }
         if (o[9] != Py_None && !rows(q = tensor(o[9]), type, device, tokens, -1, c.dim)) Py_RETURN_NONE;
         if (wants_gradient(k, v, q, cos, sin, c.t[2], c.t[3])) Py_RETURN_NONE;
+        const On on(device);
         const int interleaved = PyObject_IsTrue(o[8]);
         if (interleaved < 0) return nullptr;
         at::Tensor out, lengths = empty({s.batch}, at::kInt, *k);
@@ -168,6 +175,7 @@ PyObject *kv_attention(PyObject *, PyObject *const *o, Py_ssize_t n) {
         if (!c.take(o[1], device) || !rows(q, q->scalar_type(), device, q->size(0), -1, c.dim) ||
             !s.take(o[2], o[3], o[4], q->size(0), device) || wants_gradient(q, c.t[2], c.t[3]))
             Py_RETURN_NONE;
+        const On on(device);
         piton_kv_attention_args a = {};
         a.sm_scale = o[5] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AsDouble(o[5]);
         a.window = PyLong_AsLongLong(o[6]), a.max_length = PyLong_AsLongLong(o[7]), a.max_new = PyLong_AsLongLong(o[8]);
@@ -221,6 +229,7 @@ PyObject *matvec_w4(PyObject *, PyObject *const *o, Py_ssize_t n) {
                                 (outer > 1 && bias->stride(0) != 1)))
             Py_RETURN_NONE;
         if (wants_gradient(x, scales, bias)) Py_RETURN_NONE;
+        const On on(device);
         piton_matvec_w4_args a = {};
         a.rows = flat ? 1 : x->size(0), a.inner = inner, a.outer = outer;
         at::Tensor y = flat ? empty({outer}, x->scalar_type(), *x) : empty({a.rows, outer}, x->scalar_type(), *x);
