@@ -27,7 +27,7 @@ def rotation_tables(dim: int, positions: int, device, base: float = 10000.0):
 
 
 class PageTable:
-    """Pages of a pool handed to sequences in the order they are asked for (on the host)."""
+    """Pages of a pool handed to sequences in the order they are asked for, and given back (on the host)."""
 
     def __init__(self, batch: int, pages: int, page_size: int, width: int, device):
         self.page_size = page_size
@@ -37,13 +37,26 @@ class PageTable:
         self.table = self.host.to(device)
 
     def reserve(self, lengths) -> None:
-        """Gives sequence b the pages that ``lengths[b]`` tokens need."""
+        """Gives sequence b the pages that ``lengths[b]`` tokens need; where one cannot have them (MemoryError) none gets any."""
+        needs = list(self.owned)
         for b, length in enumerate(lengths):
-            for place in range(self.owned[b], -(-int(length) // self.page_size)):
-                if place >= self.host.shape[1] or not self.free:
-                    raise MemoryError(f"sequence {b}: no page for {length} tokens")
+            needs[b] = max(needs[b], -(-int(length) // self.page_size))
+        for b, need in enumerate(needs):
+            if need > self.host.shape[1]:
+                raise MemoryError(f"sequence {b}: {need} pages, the table holds {self.host.shape[1]}")
+        if sum(needs) - sum(self.owned) > len(self.free):
+            raise MemoryError(f"{sum(needs) - sum(self.owned)} pages wanted, {len(self.free)} free")
+        for b, need in enumerate(needs):
+            for place in range(self.owned[b], need):
                 self.host[b, place] = self.free.pop()
-                self.owned[b] = place + 1
+            self.owned[b] = need
+        self.table.copy_(self.host)
+
+    def release(self, b: int) -> None:
+        """Takes sequence b's pages back; calls already made on the current stream still find its tokens in them."""
+        self.free += reversed(self.host[b, :self.owned[b]].tolist())
+        self.host[b, :self.owned[b]] = -1
+        self.owned[b] = 0
         self.table.copy_(self.host)
 
 
