@@ -401,7 +401,8 @@ PITON_B200_API int piton_b200_kv_append(const piton_kv_append_args *args, void *
    logarithm of the row's sum of exponentials, -inf for rows without keys; tokens outside [cu[0], cu[batch])
    are rows without keys.  max_length and max_new are bounds of the lengths and of the query tokens a
    sequence, used to size the launch (0: the table's width and `tokens`); a longer sequence and more query
-   tokens are still computed in full. */
+   tokens are still computed in full.  Scores, sums and the softmax are held in 32 bits; inside the products fp32
+   queries and the softmax's weights have 22 bits, the weights of bf16 rows 11. */
 typedef struct {
     uint64_t q, out;            /* [tokens, q_heads, head_dim] of `type`, unit stride along head_dim */
     uint64_t lse;               /* float [tokens, q_heads] or 0 */

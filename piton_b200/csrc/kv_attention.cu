@@ -9,12 +9,13 @@
 // another before the end.  With the scores computed as S^T = K Q^T and the output as O^T = V^T P^T, keys and
 // dimensions are the 16-row side of mma.m16n8k16 and the rows its 8-column side, so one query token's group of
 // heads fills an instruction.  Every e4m3 code is exact in fp16: queries are scaled by a power of two per row
-// and rounded to fp16 (exact for 16-bit rows down to 2^-28 of the row's largest; fp32 ones split into two halves, 22 bits).
-// The weights p become fp16 too: an 11-bit rounding of each for 16-bit rows, no coarser than the output's for fp16, and two halves
-// for fp32.  Products are exact in the fp32 accumulators.  Weights are kept as 2^LIFT p relative to a reference that may lag the running
+// and rounded to fp16 (exact for 16-bit rows down to 2^-28 of the row's largest; fp32 ones split into two halves, 22 bits down to
+// 2^-17 of it).  The weights p become fp16 too: two halves, 22 bits, for fp32 rows and for fp16 ones, whose output one half's
+// rounding would show in (64 sequences of 2000 keys: two halves 60 us, one 58; error against 64 bits 2.1e-4 and 2.8e-4); one, 11 bits, for bf16 rows,
+// three more than the output's.  Products are exact in the fp32 accumulators.  Weights are kept as 2^LIFT p relative to a reference that may lag the running
 // maximum by 2^SLACK (16-bit rows), so O is rarely rescaled and the products add straight into its registers; fp32 rows add a
 // stage's sums to O in fp32 instead.  The pages' V scales go into the weights relative to a reference
-// that a tile's scale passes by no more than 2^6 downwards: weights down to 2^-19 of the row's largest keep their 11 bits, those
+// that a tile's scale passes by no more than 2^6 downwards: weights down to 2^-19 of the row's largest keep a half's 11 bits, those
 // below 2^-30 are lost. The reference moves with the scales, up or down, and the sums so far move in fp32, so what a row
 // adds up from pages of small values does not depend on larger ones that it does not see or hardly weighs (within 2^80 of them).
 //
@@ -28,7 +29,7 @@
 // (24 sequences, 4 new tokens, window 2048: 240 CTAs 32.4 us, 360 CTAs 44.8).
 //
 // Measured: 268 MB of codes, one sequence, bf16: 63 us (4.2 TB/s); 32 sequences, fp32, 538 MB: 109 us (4.9 TB/s); 64
-// sequences of 2000 keys, fp16: 59 us (3.4 TB/s); one of 1000 keys: 9.0 us, of 100 keys and 4 heads: 4.7. Up to 8 rows a tile the copies bound it once a
+// sequences of 2000 keys, fp16: 60 us (3.3 TB/s); one of 1000 keys: 9.0 us, of 100 keys and 4 heads: 4.7. Up to 8 rows a tile the copies bound it once a
 // warp has several stages; with 16 rows the chain of products, softmax and products of 8 warps an SM does (instructions issue in
 // 30 % of the cycles: 32.1 us where the bytes take 9.8).
 #include "decode.cuh"
@@ -193,6 +194,7 @@ template <typename T, int D, int NQ>
 __device__ __forceinline__ void attend(const CachedParams &p, const int64_t b, const int kvh, const int split, const Span &sp, const uint32_t row0) {
     using G = Geometry<D>;
     constexpr bool SPLIT = sizeof(T) == 4;              // fp32 rows: queries and weights as pairs of halves
+    constexpr bool PAIRS = !std::is_same_v<T, __nv_bfloat16>;   // of weights, also for fp16
     constexpr float LIFT = SPLIT ? 14.0f : 11.0f, SLACK = SPLIT ? 0.0f : 4.0f, UNLIFT = SPLIT ? 0x1p-14f : 0x1p-11f;
     constexpr int R = 8 * NQ, KW = G::KB / 4, VW = G::VB / 4, MT = D / 16, KT = D / 16, TILES = G::TILES, KEYS = G::KEYS;
     extern __shared__ __align__(16) uint8_t ring[];
@@ -550,7 +552,7 @@ __device__ __forceinline__ void attend(const CachedParams &p, const int64_t b, c
         };
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            uint32_t v[4][VW], ph[NQ][2], pl[SPLIT ? NQ : 1][2];
+            uint32_t v[4][VW], ph[NQ][2], pl[PAIRS ? NQ : 1][2];
 #pragma unroll
             for (int r = 0; r < 4; ++r) load_words(v[r], v_slot + (4 * t + r) * 32 * G::VB);
 #pragma unroll
@@ -559,7 +561,7 @@ __device__ __forceinline__ void attend(const CachedParams &p, const int64_t b, c
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t hi = pack(c[t][n][2 * e], c[t][n][2 * e + 1]);
                     ph[n][e] = transposed(hi);
-                    if constexpr (SPLIT) pl[n][e] = transposed(pack_rest(hi, c[t][n][2 * e], c[t][n][2 * e + 1]));
+                    if constexpr (PAIRS) pl[n][e] = transposed(pack_rest(hi, c[t][n][2 * e], c[t][n][2 * e + 1]));
                 }
             if (edge) {                                 // NaN codes: 0 * NaN must not reach a row that does not see the key
                 uint32_t any = 0;
@@ -620,6 +622,7 @@ __device__ __forceinline__ void attend(const CachedParams &p, const int64_t b, c
                             mma(acc[2 * w + i][n], a[i], pl[n][0], pl[n][1]);
                         } else {
                             mma(o[2 * w + i][n], a[i], ph[n][0], ph[n][1]);
+                            if constexpr (PAIRS) mma(o[2 * w + i][n], a[i], pl[n][0], pl[n][1]);
                         }
                     }
             }

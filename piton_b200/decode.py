@@ -228,7 +228,8 @@ def kv_attention(q, cache, table, lengths, *, cu=None, scale: Optional[float] = 
     is 1 / sqrt(head_dim) by default.  Rows that see no key are 0, and so are rows of tokens that no sequence's
     range names.  ``max_length`` (an upper bound of the lengths known to the host) and ``max_new`` (of the query
     tokens a sequence, with ``cu``) size the launch and change no result; by default the table's width and the
-    number of tokens bound them.  With ``return_lse`` also the float32
+    number of tokens bound them.  Scores, sums and the softmax are held in 32 bits; inside the products float32
+    queries and the softmax's weights have 22 bits, the weights of bfloat16 rows 11.  With ``return_lse`` also the float32
     [tokens, heads] logarithms of the rows' sums of exponentials (-inf for rows that see no key)."""
     args = (q, cache, table, lengths, cu, scale, window, max_length, max_new, return_lse)
     result = (_bound or _calls()).kv_attention(*args)

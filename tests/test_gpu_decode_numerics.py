@@ -266,3 +266,22 @@ def test_attention_nan_value_of_a_key_without_weight(cuda, dtype, length, max_le
     out = decode.kv_attention(q, (cache[0].view(ref.E4M3), cache[1].view(ref.E4M3), *scales), table,
                               torch.tensor([length], dtype=torch.int32, device="cuda"), max_length=max_length)
     assert bool(torch.isnan(out[:, :, 11]).all()) and int(torch.isnan(out).sum()) == 3
+
+
+@pytest.mark.parametrize("dim,group,new", [(32, 4, 1), (64, 8, 1), (128, 4, 4), (128, 16, 1)])
+def test_attention_fp16_rows_keep_the_weights(cuda, dim, group, new):
+    # a few keys whose values nearly cancel: what is left is rounded once, to the output, beside the bound of fp32 rows (2^-17 of the
+    # largest |v|, half an ulp of fp16 there is 2^-11)
+    lengths = [5, 6, 7, 9, 30]
+    table, pages = page_table([2] * 5, 2, 1)
+    cache = random_cache(pages, 2, 16, dim, 1)
+    raw = cache[1].view(torch.uint8)
+    raw[:, :, 1::2] = raw[:, :, 0::2] ^ 0x80                    # every other value is its neighbour's negative
+    cache[2].fill_(2.0 ** -12)                                  # nearly equal weights
+    q = torch.randn((5 * new, 2 * group, dim), generator=gen(dim), device="cuda").half()
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = decode.kv_attention(q, tuple(cache), table.cuda(), lens).cpu().double()
+    want, _, spread = ref.attention(q, cache, table, lens, offsets([new] * 5))
+    top = float((cache[1].float() * cache[3][..., None, None]).abs().max())
+    tol = bound(torch.float32, dim, spread, top) + 2.0 ** -11 * want.abs() + 2.0 ** -25
+    assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
