@@ -148,3 +148,23 @@ def test_tokens_of_no_sequence_are_refused(cuda):
         decode.kv_append(k, k, cache, table, none, cu=cu, q=k)
     with pytest.raises(ValueError):
         decode.kv_attention(k, cache, table, none, cu=cu)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("grow", [1e-3, 1.0, 40.0])
+def test_append_again_changes_nothing(cuda, dtype, grow):
+    # the same tokens at the same places a second time: scales that grew stay, old codes are not requantised again
+    starts, news, page = [0, 5, 31, 64], [40, 1, 9, 16], 16
+    table, pages = page_table([-(-(s + n) // page) for s, n in zip(starts, news)], 5, 2)
+    cache = random_cache(pages, 2, page, 64, 3)
+    k, v = (torch.randn((sum(news), 2, 64), generator=gen(i), device="cuda").to(dtype) * grow for i in range(2))
+    cu = torch.tensor([0, *news]).cumsum(0).to(torch.int32).cuda()
+    cos, sin = tables(64, 100)
+    args = tuple(cache), table.cuda(), torch.tensor(starts, dtype=torch.int32, device="cuda")
+    decode.kv_append(k, v, *args, cu=cu, cos=cos, sin=sin)
+    once = cpu(cache)
+    decode.kv_append(k, v, *args, cu=cu, cos=cos, sin=sin)
+    assert all(torch.equal(a, b) for a, b in zip(once, cpu(cache)))
+    # and the second call does write: other tokens change the codes
+    decode.kv_append(v, k, *args, cu=cu, cos=cos, sin=sin)
+    assert not any(torch.equal(a, b) for a, b in zip(once[:2], cpu(cache)[:2]))
