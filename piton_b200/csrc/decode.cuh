@@ -37,6 +37,22 @@ __device__ __forceinline__ uint8_t float_to_e4m3(float x) {
     return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
 
+// WORDS words of shared memory in one load.
+template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], uint32_t at) {
+    if constexpr (WORDS == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    else if constexpr (WORDS == 2)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+}
+
+// A copy of N bytes (4, 8 or 16) from global to shared memory that is waited for later.
+template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+
 // Query (or new) tokens [t0, t0 + n) of sequence b: from the offsets `cu`, clamped to the tensor,
 // or `uniform` each.
 struct Span {

@@ -75,10 +75,6 @@ template <int D> struct Geometry {
     static constexpr int RUN = 32 / TILES;              // stages whose page numbers the lanes hold at a time
 };
 
-template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
-    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
-}
 template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool on) {
     const int size = on ? N : 0;                        // the rest of the N bytes is filled with zeros
     if constexpr (N == 16)
@@ -89,14 +85,6 @@ template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const 
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], uint32_t at) {
-    if constexpr (WORDS == 4)
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-    else if constexpr (WORDS == 2)
-        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
-    else
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
-}
 // Two e4m3 codes, bytes 0 and 1 (or 2 and 3) of a word, as two fp16 values: exact.
 __device__ __forceinline__ uint32_t halves(uint32_t word) {
     uint32_t d;

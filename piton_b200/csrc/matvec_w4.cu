@@ -120,24 +120,10 @@ template <> struct Zero<__half> {
     }
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ uint4 load16(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
-}
-template <int WORDS> __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], uint32_t at) {
-    if constexpr (WORDS == 4)
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-    else if constexpr (WORDS == 2)
-        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
-    else
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
 
 // Two floats in one 64-bit register, and the instructions that take two at a time: half as many to issue.
@@ -267,14 +253,14 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                 const uint32_t dst[2] = {fill + copy_at, (fill + copy_at) ^ 64};     // rows r and r + 4: pieces exchanged by 4
 #pragma unroll
                 for (int i = 0; i < 4 * R; ++i) {
-                    if (R > 1 || 4 * i + (lane >> 3) < rows) copy16(dst[i & 1] + 512 * i, src);
+                    if (R > 1 || 4 * i + (lane >> 3) < rows) copy_async<16>(dst[i & 1] + 512 * i, src);
                     src += 4 * p.sc;
                 }
             } else if (whole && p.codes_align == 4) {                   // a row a copy
                 const uint8_t *src = codes + 4 * lane;
 #pragma unroll 8
                 for (int r = 0; r < 16 * R; ++r) {
-                    if (R > 1 || r < rows) copy4(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src);
+                    if (R > 1 || r < rows) copy_async<4>(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src);
                     src += p.sc;
                 }
             } else {                                                    // the last step, or rows that are not aligned: words that hold a byte of the row
@@ -283,12 +269,12 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 #pragma unroll 4
                 for (int r = 0; r < rows; ++r) {
                     const int before = (int)(reinterpret_cast<uintptr_t>(src) & 3);
-                    if (4 * lane - before < left) copy4(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src - before + 4 * lane);
+                    if (4 * lane - before < left) copy_async<4>(fill + 128 * r + ((lane >> 2) ^ (r & 7)) * 16 + 4 * (lane & 3), src - before + 4 * lane);
                     src += p.sc;
                 }
                 src = codes + lane * p.sc;
                 const int before = (int)(reinterpret_cast<uintptr_t>(src) & 3);
-                if (before && lane < rows && LINE - before < left) copy4(fill + 16 * R * LINE + 4 * lane, src - before + LINE);
+                if (before && lane < rows && LINE - before < left) copy_async<4>(fill + 16 * R * LINE + 4 * lane, src - before + LINE);
             }
             codes += STRIDE * LINE;
             ++issued;
@@ -364,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
             const uint32_t to = (uint32_t)__cvta_generic_to_shared(xs);
             for (int m = warp; m < x_rows; m += WARPS)
 #pragma unroll 4
-                for (int i = 16 * lane; i < count * S::STEP_BYTES; i += 512) copy16(to + m * S::pitch(p.phase) + i, src + m * pitch + i);
+                for (int i = 16 * lane; i < count * S::STEP_BYTES; i += 512) copy_async<16>(to + m * S::pitch(p.phase) + i, src + m * pitch + i);
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
         } else {
             lay_out<T, WORDS>(p, m0, x_rows, step0 + phase0, count, xs, S::pitch(p.phase));
