@@ -75,7 +75,7 @@ template <int D> struct Geometry {
     static constexpr int RUN = 32 / TILES;              // stages whose page numbers the lanes hold at a time
 };
 
-template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void *src, bool on) {
+template <int N> __device__ __forceinline__ void copy_or_clear(uint32_t dst, const void *src, bool on) {
     const int size = on ? N : 0;                        // the rest of the N bytes is filled with zeros
     if constexpr (N == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
@@ -280,7 +280,7 @@ __device__ __forceinline__ void attend(const CachedParams &p, const int64_t b, c
                     for (int i = 0; i < 2 * G::KC; ++i) {
                         const int row = k_row + i * K_STEP;
                         const bool on = id >= 0 && key + row >= lo && key < span - row;
-                        copy_async<G::KB>(at + (2 * t * G::KC + i) * 32 * G::KB, on ? src + i * K_STEP * D : p.kc, on);
+                        copy_or_clear<G::KB>(at + (2 * t * G::KC + i) * 32 * G::KB, on ? src + i * K_STEP * D : p.kc, on);
                     }
                 }
             }
@@ -318,7 +318,7 @@ __device__ __forceinline__ void attend(const CachedParams &p, const int64_t b, c
                     for (int r = 0; r < 4; ++r) {
                         const int row = 2 * j + (r & 1) + 8 * (r >> 1);
                         const bool on = id >= 0 && key + row >= lo && key < span - row;
-                        copy_async<G::VB>(at + (4 * t + r) * 32 * G::VB, on ? src + ((r & 1) + 8 * (r >> 1)) * D : p.vc, on);
+                        copy_or_clear<G::VB>(at + (4 * t + r) * 32 * G::VB, on ? src + ((r & 1) + 8 * (r >> 1)) * D : p.vc, on);
                     }
                 }
             }
