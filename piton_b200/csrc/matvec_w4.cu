@@ -17,8 +17,8 @@
 // may split the inner dimension further, and adds its parts through distributed shared memory in a fixed order.
 //
 // Measured: 28000 x 8192, groups of 128: 1 row, bf16 38 us (3.1 TB/s), fp16 35.5; 8 rows of bf16, groups of 32 with zero points 70;
-// 16 rows of fp32, groups of 64 with zero points 112. 4096 x 4096: 1 row, bf16 6.0 us, 16 rows 9.9; fp32, 8 rows 12.3, 16 rows 20.5; 32768 x
-// 8192, bf16, 16 rows 57 us (2.5 TB/s). Rows of codes on any byte: 4096 x 4098 9.0 us, copies of 4 bytes a lane where whole rows take
+// 16 rows of fp32, groups of 64 with zero points 112. 4096 x 4096: 1 row, bf16 6.0 us, 16 rows 9.9; fp32, 8 rows 12.6, 16 rows 13.7; 32768 x
+// 8192, bf16, 16 rows 54 us (2.6 TB/s). Rows of codes on any byte: 4096 x 4098 9.0 us, copies of 4 bytes a lane where whole rows take
 // 16. A call has 4 to 5 us that do not depend on the matrix (launches, x, the cluster's sums); one row is bound by the instructions that SMs with two
 // CTAs issue (28000 x 8192 fills 220 of 296 places: 53 % of the issue slots over the SMs, DRAM at 37 %), 16 rows by the legacy tensor path besides.
 #include <cooperative_groups.h>
@@ -143,9 +143,8 @@ __device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
 template <typename T, int NT, int R, int GROUPS> struct Shape {
     // Of each group's 32 WORDS elements in a block lane j takes the 8 WORDS from 8 WORDS j on: WORDS words of codes.
     static constexpr int WORDS = 4 / GROUPS;
-    // Two stages of 32 weight rows (three: 28000 x 8192 30.0 us, two 28.6 at the time); of 16, three with one tile of x and two with two, whose x
-    // takes the room (4096 x 4096, fp32: 8 rows with 4 / 3 / 2 stages 9.7 / 7.9 / 8.1 us, 16 rows with 4 / 2 18.1 / 13.1)
-    static constexpr int SLOT = 16 * R * LINE + 128, STAGES = R == 1 && NT == 1 ? 3 : 2, QUEUES = WARPS * STAGES * SLOT;
+    // Two stages (three: one row of 28000 x 8192, bf16, 39.5 us, two 37.8; 16 rows of 32768 x 8192 64 and 54; 4096 x 4096 6.0 either way)
+    static constexpr int SLOT = 16 * R * LINE + 128, STAGES = 2, QUEUES = WARPS * STAGES * SLOT;
     static constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;               // of x
     static constexpr int SUMS = 8 * NT * 16 * R;                        // outputs of a warp's tile
     // x in shared memory, per row: 16 bytes for every 8 elements of a piece; the padding puts rows that are read together into
@@ -534,8 +533,8 @@ template <typename T, int NT, int R, int GROUPS, bool ALONG_K, bool BYTES> int l
     const int all_steps = (int)cdiv(p.inner, 2 * BLOCK);
     p.span = (int32_t)cdiv(all_steps, plan.parts);
     // x whole, or as many of its steps as leave room for a second CTA
-    p.phase = p.span > 0 ? p.span : 1;
-    while (S::smem(x_rows, p.phase) > 113 * 1024 && p.phase > 1) p.phase = (p.phase + 1) / 2;
+    const int64_t phases = cdiv(p.span, (113 * 1024 - S::smem(x_rows, 0)) / (x_rows * S::STEP_BYTES));
+    p.phase = phases > 0 ? (int32_t)cdiv(p.span, phases) : 1;
     static bool known[64];
     int dev = 0, launches = 1;
     PITON_CUDA(cudaGetDevice(&dev));
@@ -582,14 +581,17 @@ template <typename T, int NT> int launch(const MatvecParams &p, const Plan &plan
 
 Plan plan_of(const piton_matvec_w4_args *a) {
     Plan plan = {true, 1, 0};
+    const bool fp32 = a->type == PITON_B200_TYPE_F32;
+    const int64_t together = fp32 ? 8 : 16, row_groups = cdiv(a->rows, together);   // rows of x that a CTA takes, CTAs over them
     const int64_t tiles = cdiv(a->outer, 16), sms = num_sms(), steps = cdiv(a->inner, 2 * BLOCK);
     const int64_t most = steps < MAX_PARTS ? steps : MAX_PARTS;
     int64_t parts = 1;                      // a power of two: clusters of 7 took longer than of 4
-    // Warps along the rows from 2 x 148 tiles of 16 weight rows on, in as many parts of the inner dimension as two CTAs an SM
-    // take in one wave (28000 x 8192, bf16, one row: 2 parts 29.4 us, 1 part 36.6, 4 parts 32.2; warps along the inner
-    // dimension 40); below that along the inner dimension (4096 x 4096: 6.2 us, along the rows 6.2 to 9), split
-    // further only while SMs are idle and every warp keeps two steps (1024 x 8192: 4 parts 5.5 us, 1 part 7.8).
-    if (tiles >= 2 * sms) {
+    // Warps along the rows from 2 x 148 tiles of 16 weight rows on (for every group of rows of x), in as many parts of the inner
+    // dimension as two CTAs an SM take in one wave for one such group (28000 x 8192, bf16, one row: 2 parts 37.8 us, 1 part 39.7, 4 parts
+    // 41.5; warps along the inner dimension 43.8; fp32, two groups: 2 parts 112, 1 part 135); below that along the inner dimension (4096 x 4096, bf16: 6.0 us, along the rows 8.1; 16 rows of
+    // fp32, two groups: 20.4 and 13.7), split further only while SMs are idle and every warp keeps two steps (1024 x 8192: 4
+    // parts 5.7 us, 2 parts 6.1).
+    if (tiles * row_groups >= 2 * sms && a->outer >= 32) {     // (a warp's 32 weight rows have to exist)
         plan.along_k = false;
         const int64_t groups = cdiv(tiles, 2 * WARPS);
         while (2 * parts <= most && groups * 2 * parts <= 2 * sms) parts *= 2;
@@ -599,8 +601,7 @@ Plan plan_of(const piton_matvec_w4_args *a) {
     plan.parts = (int)parts;
     // More than 8192 elements of x a CTA are laid out once, in the workspace, by a kernel of their own (bf16, 16 rows by 4096 x 4096: 9.9 us,
     // in every CTA 11.8; fewer do not repay its launch), and more than 2048 of fp32, whose split into pieces is ten times the work.
-    const bool fp32 = a->type == PITON_B200_TYPE_F32;
-    const int64_t together = fp32 ? 8 : 16, x_rows = a->rows < together ? a->rows : together;
+    const int64_t x_rows = a->rows < together ? a->rows : together;
     if (x_rows * cdiv(steps, parts) * 2 * BLOCK > (fp32 ? 2048 : 8192)) plan.laid = (size_t)(a->rows * steps) * (fp32 ? 1536 : 512);
     return plan;
 }

@@ -285,3 +285,17 @@ def test_attention_fp16_rows_keep_the_weights(cuda, dim, group, new):
     top = float((cache[1].float() * cache[3][..., None, None]).abs().max())
     tol = bound(torch.float32, dim, spread, top) + 2.0 ** -11 * want.abs() + 2.0 ** -25
     assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,inner,outer,group", [(4800, 96, 1, 32), (5000, 130, 17, 64), (4800, 128, 31, 128), (2500, 256, 32, 128),
+                                                    (3000, 300, 33, 32), (24, 2304, 2050, 64), (64, 700, 700, 128)])
+def test_matvec_many_rows(cuda, dtype, rows, inner, outer, group):
+    # the weight rows of a launch of many rows of x are cut by how many CTAs there are in all; a few outputs stay whole
+    g = gen(rows)
+    x = torch.randn((rows, inner), generator=g, device="cuda").to(dtype)
+    codes = torch.randint(0, 256, (outer, (inner + 1) // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand((outer, -(-inner // group)), generator=g, device="cuda") * 0.1).to(dtype)
+    y = decode.matvec_w4(x, codes, scales, group=group)
+    want, size = ref.matvec_w4(x, codes, scales, None, None, group)
+    assert ((y.cpu().double() - want).abs() <= product_bound(dtype, inner, want, size)).all()
