@@ -12,9 +12,9 @@
 // block's scale is known, and reads its rows of the rotation tables once for all heads that it walks.
 // Rows that do not lie on 16 bytes, or rotate in pairs of pieces that do not, take the element-by-element kernel.
 //
-// Measured: long prompts, 742 MB in and out: 148 us (5.0 TB/s); ragged prompts, 304 MB: 58 us (5.2 TB/s); 256 sequences, a token
-// each: 6.3 us; one token: 3.3 us. A launch of its own for the queries: 205 us for the long prompts; no load of the next head while the
-// last is stored: 215.
+// Measured: long prompts, 742 MB in and out: 152 us (4.9 TB/s); ragged prompts, 304 MB: 59 us (5.2 TB/s); 256 sequences, a token
+// each: 6.5 us; one token: 3.4 us. Where the long prompts took 148 us, a launch of its own for the queries took 205, no load of the next
+// head while the last is stored 215.
 #include "decode.cuh"
 
 namespace piton {
@@ -520,7 +520,7 @@ template <typename T, int D, int TT, int PASSES> int launch_wide(AppendParams p,
     constexpr int UPH = D / (2 * (16 / (int)sizeof(T))), SIDE = 32 / UPH;
     const int64_t sms = num_sms();
     // A CTA walks a unit's heads, whose rows share what it read of the rotation tables, as far as that leaves two CTAs an SM
-    // (10,500 tokens at most, 32 + 32 heads of 64, fp32: 58 us; at most 4 heads a CTA 76, one 135).
+    // (10,500 tokens at most, 32 + 32 heads of 64, fp32: 59 us; at most 4 heads a CTA 78, one 146).
     int64_t heads_each = 1;
     if (TT == WIDE) {
         heads_each = p.units * 2 * p.kv_heads / (2 * sms);
@@ -528,8 +528,8 @@ template <typename T, int D, int TT, int PASSES> int launch_wide(AppendParams p,
     }
     const int64_t tasks = p.units * 2 * cdiv(p.kv_heads, heads_each);
     p.unit_blocks = cdiv(tasks, WIDE / TT);
-    // A warp walks a token's query heads, in pieces while there are not 8 warps an SM (64 tokens of 32 heads: 4.2 us, whole 4.6;
-    // 1600 tokens: whole 8.0, in pieces up to 32 warps an SM 9.4).
+    // A warp walks a token's query heads, in pieces while there are not 8 warps an SM (64 tokens of 32 heads: 4.3 us, whole 5.2;
+    // 1600 tokens: whole 8.2, in pieces up to 32 warps an SM 10.1).
     int64_t q_pieces = 1;
     while (q_pieces * SIDE < p.q_heads && p.tokens * q_pieces < 8 * sms) q_pieces *= 2;
     const int64_t blocks = p.unit_blocks + (p.q_heads ? cdiv(p.tokens * q_pieces, WIDE / 32) : 0);
@@ -541,7 +541,7 @@ template <typename T, int D, int TT, int PASSES> int launch_wide(AppendParams p,
 template <typename T, int D> int launch_wide(const AppendParams &p, cudaStream_t s) {
     constexpr int UPH = D / (2 * (16 / (int)sizeof(T)));
     // Pairs of a task at most: what a warp's four passes hold is a warp's, more is a CTA's (1600 tokens in pages of 16, 64
-    // dimensions, bf16, 64 pairs: a warp 9.4 us, a CTA 10.0).
+    // dimensions, bf16, 64 pairs: a warp 8.2 us, a CTA 9.1).
     const int64_t most = (p.cu || p.uniform > p.page_size ? p.page_size : p.uniform) * UPH;
     if (most <= 32) return launch_wide<T, D, 32, 1>(p, s);
     if (most <= 128) return launch_wide<T, D, 32, 4>(p, s);

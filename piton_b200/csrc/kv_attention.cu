@@ -26,12 +26,14 @@
 //
 // When there are fewer (sequence, key head, row tile) units than CTAs fit the GPU at once, the keys are split into ranges that
 // fill one wave, and a second kernel, launched while the first finishes, joins them in a fixed order. More splits than one wave were slower
-// (24 sequences, 4 new tokens, window 2048: 240 CTAs 32.4 us, 360 CTAs 44.8).
+// (24 sequences, 4 new tokens, window 2048: 240 CTAs 34.3 us, 360 CTAs 45.4).
 //
-// Measured: 268 MB of codes, one sequence, bf16: 63 us (4.2 TB/s); 32 sequences, fp32, 538 MB: 109 us (4.9 TB/s); 64
-// sequences of 2000 keys, fp16: 60 us (3.3 TB/s); one of 1000 keys: 9.0 us, of 100 keys and 4 heads: 4.7. Up to 8 rows a tile the copies bound it once a
-// warp has several stages; with 16 rows the chain of products, softmax and products of 8 warps an SM does (instructions issue in
-// 30 % of the cycles: 32.1 us where the bytes take 9.8).
+// Measured: 268 MB of codes, one sequence, bf16: 63 us (4.3 TB/s); 32 sequences, fp32, 538 MB: 113 us (4.8 TB/s); 64
+// sequences of 2000 keys, fp16: 60.5 us (3.3 TB/s); one of 1000 keys: 8.5 us, of 100 keys and 4 heads: 4.5. Up to 8 rows a tile the copies bound it
+// once a warp has several stages; with 16 rows the chain of products, softmax and products of 8 warps an SM does (34.3 us
+// where the bytes take 9.8; instructions issue in 30 % of the cycles).
+#include <type_traits>
+
 #include "decode.cuh"
 
 namespace piton {
@@ -150,8 +152,10 @@ __device__ __forceinline__ float move_of(uint32_t byte) { return __uint_as_float
 // NaN codes (7F and FF) of a word: a set high bit in each such byte.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
-// CTAs an SM holds: registers bound it. Three of 16 rows a tile would spill at 128 dimensions or in fp32 (24 sequences, 4 new
-// tokens, window 2048, fp32: 2 CTAs 40.5 us, 3 CTAs 55; 16 bits, 64 dimensions, 2000 keys: 28.1 and 26.0).
+// CTAs an SM holds: registers bound it. Two of 16 rows a tile at 128 dimensions or in fp32, where three spill more than they hide (24
+// sequences, 4 new tokens, window 2048, fp32: 2 CTAs, which spill 264 bytes a thread, 40.0 us, 3 CTAs 57.4); three below that, which
+// short sequences gain from and long ones pay for (16 bits, 64 dimensions, 230 sequences of 200 keys: 3 CTAs 47 us, 2 CTAs 57.5; 64 of
+// 2000 keys: 57.6 and 51).
 constexpr int ctas(int nq, int dim, bool fp32) { return nq == 1 || (dim <= 64 && !fp32) ? 3 : 2; }
 
 // The rows of a tile that a lane holds in its score and output fragments: columns 2 j and 2 j + 1 of each of the NQ
@@ -872,8 +876,8 @@ template <typename T, int D, int NQ> int launch(const CachedParams &p, int64_t b
     // launched while the splits finish (programmatic dependent launch); it waits for them before it reads
     cudaLaunchConfig_t cfg = {};
     const int64_t rows = p.tokens * p.q_heads;
-    // a warp a row for few splits (2 splits of 1920 rows: 32.3 us a call, a CTA a row 40.6), a CTA a row for more (16 splits of 32
-    // rows: 9.9 us, a warp a row 10.3), unless there are many rows (13 splits of 128 rows: a warp a row 16.4, a CTA 17.2)
+    // a warp a row for few splits (2 splits of 1920 rows: 34.3 us a call, a CTA a row 40.2), a CTA a row for more (16 splits of 32
+    // rows: 9.3 us, a warp a row 9.6), unless there are many rows (13 splits of 128 rows: a warp a row 13.6, a CTA 14.0)
     const bool few = p.splits <= (rows < 128 ? 8 : 16);
     cfg.gridDim = dim3((unsigned)(few ? cdiv(rows, WARPS) : rows));
     cfg.blockDim = dim3(THREADS);

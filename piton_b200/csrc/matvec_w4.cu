@@ -19,8 +19,8 @@
 // Measured: 28000 x 8192, groups of 128: 1 row, bf16 38 us (3.1 TB/s), fp16 35.5; 8 rows of bf16, groups of 32 with zero points 70;
 // 16 rows of fp32, groups of 64 with zero points 112. 4096 x 4096: 1 row, bf16 6.0 us, 16 rows 9.9; fp32, 8 rows 12.6, 16 rows 13.7; 32768 x
 // 8192, bf16, 16 rows 54 us (2.6 TB/s). Rows of codes on any byte: 4096 x 4098 9.0 us, copies of 4 bytes a lane where whole rows take
-// 16. A call has 4 to 5 us that do not depend on the matrix (launches, x, the cluster's sums); one row is bound by the instructions that SMs with two
-// CTAs issue (28000 x 8192 fills 220 of 296 places: 53 % of the issue slots over the SMs, DRAM at 37 %), 16 rows by the legacy tensor path besides.
+// 16. A call has 4 to 5 us that do not depend on the matrix (launches, x, the cluster's sums). One row of 28000 x 8192 issues in 52 % of an
+// SM's cycles and reads at 36 % of DRAM's, with 220 CTAs for 296 places; 16 rows of 32768 x 8192 in 47 %, waiting for the tensor pipe.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -159,7 +159,7 @@ template <typename T, int NT, int R, int GROUPS> struct Shape {
 // Lays out `steps` steps from step0 on of the rows m0 ...: per row and block 16 units of 8 elements, unit 4 c + j for word c of lane
 // j (word w of group q: c = q WORDS + w), which faces elements 32 WORDS q + 8 WORDS j + 8 w ... of the block. A unit's elements lie as the
 // codes of a word come out: 0, 4, 1, 5, 2, 6, 3, 7. An fp32 element is the sum of three bf16 ones, its upper, middle and lower 8 bits of
-// significand, exactly; they lie in 16 bytes a piece.
+// significand, exactly (but for what lies below 2^-133); they lie in 16 bytes a piece.
 template <typename T, int WORDS>
 __device__ __forceinline__ void lay_out(const MatvecParams &p, int64_t m0, int x_rows, int step0, int steps, uint8_t *to, int64_t pitch) {
     constexpr int PIECES = sizeof(T) == 4 ? 3 : 1, AT_ONCE = PIECES == 1 ? 4 : 2;    // units that a thread has on their way

@@ -247,7 +247,7 @@ def matvec_w4(x, codes, scales, *, group: int = 128, zeros=None, bias=None):
     [outer] of x's type.  Rows of every operand may be strided.  Accumulates in 32 bits, returns x's type.
     Meant for few rows: the weights are read again for every 16.
 
-    Codes less their zero points and x enter the products as they are (fp32 as three parts that add up to it), so only the 32-bit
+    Codes less their zero points and x enter the products as they are (fp32 as three parts that add up to it, down to 2^-133), so only the 32-bit
     sums are rounded.  Infinities and NaN in x and in the scales reach the outputs that the formula says, no other rows."""
     result = (_bound or _calls()).matvec_w4(x, codes, scales, group, zeros, bias)
     if result is None or result.__class__ is int:
