@@ -92,20 +92,23 @@ __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t 
 // A weight row's zero point, made ready for its codes, and eight codes less the zero point: pairs of elements 0 and 4, 1 and 5,
 // 2 and 6, 3 and 7 of a word. A masked code is the low end of the significand of 1024 (fp16, where the codes four bits up
 // count 16) or of 128 (bf16); taking 1024 + zero or 128 + zero from it is exact. In bf16 that holds for zero points up to 127;
-// what larger ones are more than their low seven bits is taken off afterwards.
+// what larger ones are more than their low seven bits is taken off afterwards. There a code counts 2^-8, so that sums of elements near the
+// type's largest stay in range until the scale is applied; the outputs are multiplied by UP.
 template <typename T> struct Zero {
-    uint32_t low;                                                       // -(128 + zero), twice
+    static constexpr float UP = 256.0f;
+    uint32_t low;                                                       // -(128 + zero) / 256, twice
     // byte i of a word of zero points below 128
-    __device__ __forceinline__ Zero(uint32_t z, int i) { low = __byte_perm(z, 0xC3, 0x4040 | 0x101 * i); }
+    __device__ __forceinline__ Zero(uint32_t z, int i) { low = __byte_perm(z, 0xBF, 0x4040 | 0x101 * i); }
     __device__ __forceinline__ void less(uint32_t (&a)[4], uint32_t w) const {
-        constexpr uint32_t ONE = 0x3F803F80u;
-        a[0] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w), ONE, low);
-        a[1] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 4), ONE, low);
-        a[2] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 8), ONE, low);
-        a[3] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 12), ONE, low);
+        constexpr uint32_t DOWN = 0x3B803B80u;                          // 1 / 256
+        a[0] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w), DOWN, low);
+        a[1] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 4), DOWN, low);
+        a[2] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 8), DOWN, low);
+        a[3] = fma_bf16x2(masked<0x000F000Fu, 0x43004300u>(w >> 12), DOWN, low);
     }
 };
 template <> struct Zero<__half> {
+    static constexpr float UP = 1.0f;
     uint32_t low, low16;                                                // 1024 + zero; -(64 + zero), twice
     __device__ __forceinline__ Zero(uint32_t z, int i) {
         low = __byte_perm(z, 0x64, 0x4040 | 0x101 * i);
@@ -448,8 +451,8 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
                                         const uint4 x = load16(x_at[t] + (b0 + b) * (256 * PIECES) + (q * WORDS + i) * (64 * PIECES) + 16 * piece);
 #pragma unroll
                                         for (int r = 0; r < R; ++r) {
-                                            const uint32_t d0 = z >> (16 * r + 7) & 1 ? 0xC300C300u : 0u, d1 = z >> (16 * r + 15) & 1 ? 0xC300C300u : 0u;
-                                            const uint32_t a[4] = {d0, d1, d0, d1};                     // -128 or 0
+                                            const uint32_t d0 = z >> (16 * r + 7) & 1 ? 0xBF00BF00u : 0u, d1 = z >> (16 * r + 15) & 1 ? 0xBF00BF00u : 0u;
+                                            const uint32_t a[4] = {d0, d1, d0, d1};                     // -128 / 256 or 0
                                             mma<T, false>(piece ? small[r][t] : sum[r][t], a, x.x, x.y);
                                             mma<T, false>(piece ? small[r][t] : sum[r][t], a, x.z, x.w);
                                         }
@@ -514,6 +517,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_w4_kernel(const MatvecParam
 #pragma unroll
             for (int x = 0; x < ADD; ++x) sum += from[x * S::SUMS];
         }
+        sum *= Zero<T>::UP;
         if (p.bias) sum += to_float(reinterpret_cast<const T *>(p.bias)[at]);
         reinterpret_cast<T *>(p.y)[(m0 + m) * p.sy + at] = from_float<T>(sum);
     }

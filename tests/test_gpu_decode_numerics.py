@@ -299,3 +299,18 @@ def test_matvec_many_rows(cuda, dtype, rows, inner, outer, group):
     y = decode.matvec_w4(x, codes, scales, group=group)
     want, size = ref.matvec_w4(x, codes, scales, None, None, group)
     assert ((y.cpu().double() - want).abs() <= product_bound(dtype, inner, want, size)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,inner,outer,group", [(1, 1024, 40, 128), (4, 4096, 64, 32), (9, 1280, 4800, 128)])
+def test_matvec_of_elements_near_the_largest(cuda, dtype, rows, inner, outer, group):
+    # |x| up to 3e38, weights around 1e-3: the outputs are far from the type's largest, and so must the sums on the way be
+    g = gen(rows)
+    x = ((2 * torch.rand((rows, inner), generator=g, device="cuda") - 1) * 3e38).to(dtype)
+    x[:, ::2] = x[:, ::2].abs()
+    codes = torch.randint(0, 256, (outer, inner // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand((outer, inner // group), generator=g, device="cuda") * 1e-5).to(dtype)
+    y = decode.matvec_w4(x, codes, scales, group=group)
+    want, size = ref.matvec_w4(x, codes, scales, None, None, group)
+    assert float(size.max()) < 3e38
+    assert ((y.cpu().double() - want).abs() <= product_bound(dtype, inner, want, size)).all()
